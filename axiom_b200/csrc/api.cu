@@ -12,10 +12,13 @@
 #include "qgemv.cuh"
 #include "qskinny_tc.cuh"
 #include "kv_attend.cuh"
+#include "kv_tree.cuh"
+#include "rope.cuh"
 #include "sdpa.cuh"
 #include "skinny.cuh"
 
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -51,6 +54,8 @@ struct Engine {
     // grow-only buffer for intermediate results a fused route cannot avoid (the unfused qkv projection)
     void *aux = nullptr;
     size_t aux_bytes = 0;
+    // workspace of the ragged-batch attention calls that bring none: one size, made once, never moved
+    void *attn_ws = nullptr;
     // host-operand GEMM: device staging (grow-only), copy streams and the events that order them
     void *hp_buf = nullptr;
     size_t hp_bytes = 0;
@@ -399,6 +404,7 @@ extern "C" void axb_shutdown(void)
         if (en.gemm_counters) cudaFree(en.gemm_counters);
         if (en.hp_buf) cudaFree(en.hp_buf);
         if (en.aux) cudaFree(en.aux);
+        if (en.attn_ws) cudaFree(en.attn_ws);
         if (en.hp_in) cudaStreamDestroy(en.hp_in);
         if (en.hp_out) cudaStreamDestroy(en.hp_out);
         for (auto &ev : en.hp_ev)
@@ -493,7 +499,9 @@ extern "C" int axb_device_error(void)
     if (cudaMemcpy(&v, cur().err_word, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
     if (v) {
         cudaMemset(cur().err_word, 0, sizeof(int));
-        fail(AXB_ERR_BACKEND, "a kernel gave up on a bounded wait (code %d)", v);
+        if (v == AXB_DEVERR_ROWS) fail(AXB_ERR_INVALID_SHAPE, "a sequence's length and new tokens do not fit its cache rows (code %d)", v);
+        else if (v == AXB_DEVERR_KEEP) fail(AXB_ERR_INVALID_SHAPE, "an accepted-token list is not ascending indices of the drafted rows (code %d)", v);
+        else fail(AXB_ERR_BACKEND, "a kernel gave up on a bounded wait (code %d)", v);
     }
     return v;
 }
@@ -1365,6 +1373,268 @@ extern "C" int axb_kv_cache_attend(const float *K_cache, const float *V_cache, c
     mark(2);
     cur().launches++;
     return e ? cuda_fail("kv_cache_attend", e) : AXB_OK;
+}
+
+// ------------------------------------- rotary positions, per-head norms, ragged-batch KV cache
+
+namespace {
+
+// The engine's device for the time of a call: a host that moved on to another device since axb_init gets its choice back.
+struct OnDevice {
+    int before = -1;
+    OnDevice()
+    {
+        int d = -1;
+        if (cudaGetDevice(&d) == cudaSuccess && d != cur().device && cudaSetDevice(cur().device) == cudaSuccess) before = d;
+    }
+    ~OnDevice()
+    {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// a skinny GEMM after this call must not request its weights before the call has finished: it may be multiplying by the
+// cache or the queries written here
+inline void wrote_operands()
+{
+    cur().chain_lo = nullptr;
+    cur().chain_lo += 1;
+    cur().chain_hi = reinterpret_cast<const char *>(UINTPTR_MAX);
+}
+
+inline bool overlaps(const void *p, int64_t n, const void *q, int64_t m)   // n, m floats
+{
+    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+    return p && q && a < b + (size_t)m * sizeof(float) && b < a + (size_t)n * sizeof(float);
+}
+
+// counters first (zero between calls), then room for either call's partial results
+constexpr size_t kAttnCounters = 4096;
+static_assert(sizeof(int) * 1024 <= kAttnCounters, "a counter per SM");
+
+size_t attn_workspace_bytes()
+{
+    const size_t tree = kv_tree_workspace_bytes(cur().sm_count), bwd = (size_t)cur().sm_count * 4 * 2 * 256 * sizeof(float);
+    return kAttnCounters + (tree > bwd ? tree : bwd);
+}
+
+int attn_workspace(const char *what, void *&ws)
+{
+    if (ws) {
+        if ((uintptr_t)ws & 15) return fail(AXB_ERR_INVALID_SHAPE, "%s: workspace not 16-byte aligned", what);
+        return AXB_OK;
+    }
+    if (!cur().attn_ws) {
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(cur().stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone)
+            return fail(AXB_ERR_ALLOC, "%s: the first call that needs the engine's workspace may not be captured", what);
+        const size_t bytes = attn_workspace_bytes();
+        cudaError_t e = cudaMalloc(&cur().attn_ws, bytes);
+        if (e != cudaSuccess) {
+            cur().attn_ws = nullptr;
+            return fail(AXB_ERR_ALLOC, "%s: workspace of %zu bytes: %s", what, bytes, cudaGetErrorString(e));
+        }
+        // before any call on any stream: the counters start at zero
+        if ((e = cudaMemset(cur().attn_ws, 0, kAttnCounters)) == cudaSuccess) e = cudaDeviceSynchronize();
+        if (e != cudaSuccess) return cuda_fail(what, e);
+    }
+    ws = cur().attn_ws;
+    return AXB_OK;
+}
+
+// the arguments that the forward, backward and cache forms share; T: tokens per sequence, rows: of a key head's buffer
+int rope_args(const char *what, RopeArgs &a, const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
+              const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos, int64_t B, int64_t T, int64_t H,
+              int64_t Hkv, int64_t dk)
+{
+    if (B < 0 || T < 0 || H <= 0 || Hkv <= 0 || dk <= 0 || H % Hkv) return fail(AXB_ERR_INVALID_SHAPE, "%s: bad shape", what);
+    if (dk > 256) return fail(AXB_ERR_NOT_IMPLEMENTED, "%s: head dim %lld > 256", what, (long long)dk);
+    if (H > 65535 || B > INT32_MAX || T > INT32_MAX || (B && T > INT32_MAX / B))
+        return fail(AXB_ERR_INVALID_SHAPE, "%s: more than 65535 heads or 2^31-1 tokens", what);
+    if (rot < 0 || rot % 2 || rot > dk) return fail(AXB_ERR_INVALID_SHAPE, "%s: rotated part %lld of a head of %lld", what, (long long)rot, (long long)dk);
+    if (rot && !freq) return fail(AXB_ERR_NULL_ARG, "%s: NULL frequencies", what);
+    if (pairing != AXB_ROPE_HALF && pairing != AXB_ROPE_INTERLEAVED) return fail(AXB_ERR_INVALID_SHAPE, "%s: unknown pairing %d", what, pairing);
+    if (!(eps >= 0.0f) || !isfinite(eps)) return fail(AXB_ERR_INVALID_SHAPE, "%s: eps %g", what, (double)eps);
+    memset(&a, 0, sizeof a);
+    a.qkv = qkv; a.bias = bqkv; a.gq = gq; a.gk = gk; a.freq = freq; a.pos = pos;
+    a.eps = eps; a.amplitude = amplitude;
+    a.B = (int)B; a.T = (int)T; a.H = (int)H; a.Hkv = (int)Hkv; a.dk = (int)dk; a.pairs = (int)(rot / 2);
+    a.interleaved = pairing == AXB_ROPE_INTERLEAVED;
+    a.kv_rows = T;
+    return AXB_OK;
+}
+
+}  // namespace
+
+extern "C" int axb_rope_frequencies(int64_t rot, double base, int scaling, double factor, double low, double high,
+                                    int64_t original_len, double *freq_host)
+{
+    if (!freq_host && rot > 0) return fail(AXB_ERR_NULL_ARG, "rope_frequencies: NULL");
+    if (rot < 0 || rot % 2 || !(base > 0.0) || !isfinite(base)) return fail(AXB_ERR_INVALID_SHAPE, "rope_frequencies: rot %lld, base %g", (long long)rot, base);
+    if (scaling < AXB_ROPE_PLAIN || scaling > AXB_ROPE_RAMP_INDEX) return fail(AXB_ERR_INVALID_SHAPE, "rope_frequencies: unknown scaling %d", scaling);
+    if (scaling != AXB_ROPE_PLAIN && !(factor > 0.0 && isfinite(factor))) return fail(AXB_ERR_INVALID_SHAPE, "rope_frequencies: factor %g", factor);
+    const bool ramp = scaling == AXB_ROPE_RAMP_TURNS || scaling == AXB_ROPE_RAMP_INDEX;
+    if (ramp && !(low > 0.0 && high > low && isfinite(high) && original_len > 0))
+        return fail(AXB_ERR_INVALID_SHAPE, "rope_frequencies: ramp from %g to %g turns over %lld tokens", low, high, (long long)original_len);
+    if (scaling == AXB_ROPE_RAMP_INDEX && !(base > 1.0)) return fail(AXB_ERR_INVALID_SHAPE, "rope_frequencies: base %g", base);
+    const double two_pi = 6.283185307179586477;
+    double first = 0.0, last = 0.0;
+    if (scaling == AXB_ROPE_RAMP_INDEX) {
+        first = floor((double)rot * log((double)original_len / (high * two_pi)) / (2.0 * log(base)));
+        last = ceil((double)rot * log((double)original_len / (low * two_pi)) / (2.0 * log(base)));
+        if (first < 0.0) first = 0.0;
+        if (last > (double)rot - 1.0) last = (double)rot - 1.0;
+    }
+    for (int64_t i = 0; i < rot / 2; ++i) {
+        double f = pow(base, -2.0 * (double)i / (double)rot);
+        double w = 0.0;   // the share of the unchanged frequency
+        if (scaling == AXB_ROPE_PLAIN) w = 1.0;
+        else if (scaling == AXB_ROPE_RAMP_TURNS) w = ((double)original_len * f / two_pi - low) / (high - low);
+        else if (scaling == AXB_ROPE_RAMP_INDEX) w = 1.0 - ((double)i - first) / (last - first > 1e-3 ? last - first : 1e-3);
+        w = w < 0.0 ? 0.0 : w > 1.0 ? 1.0 : w;
+        freq_host[i] = scaling == AXB_ROPE_PLAIN ? f : f * (w + (1.0 - w) / factor);
+    }
+    return AXB_OK;
+}
+
+extern "C" size_t axb_attention_workspace_bytes(void)
+{
+    if (ensure_ready()) return 0;
+    return attn_workspace_bytes();
+}
+
+extern "C" int axb_qkv_norm_rope(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
+                                 const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos, int64_t B,
+                                 int64_t S, int64_t H, int64_t Hkv, int64_t dk, float *Qh, float *Kh, float *Vh)
+{
+    RopeArgs a;
+    int st = rope_args("qkv_norm_rope", a, qkv, bqkv, gq, gk, eps, freq, rot, pairing, amplitude, pos, B, S, H, Hkv, dk);
+    if (st) return st;
+    if (B == 0 || S == 0) return ensure_ready();   // nothing to read or write: the pointers may be NULL
+    if (!qkv || !Qh || !Kh || !Vh) return fail(AXB_ERR_NULL_ARG, "qkv_norm_rope: NULL");
+    const int64_t nq = B * S * H * dk, nk = B * S * Hkv * dk, n = nq + 2 * nk;
+    if (overlaps(qkv, n, Qh, nq) || overlaps(qkv, n, Kh, nk) || overlaps(qkv, n, Vh, nk))
+        return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope: an output overlaps qkv");
+    if ((st = ensure_ready())) return st;
+    OnDevice on;
+    a.q = Qh; a.k = Kh; a.v = Vh;
+    int e = launch_qkv_norm_rope(a, cur().sm_count, cur().stream);
+    cur().launches++;
+    wrote_operands();
+    return e ? cuda_fail("qkv_norm_rope", e) : AXB_OK;
+}
+
+extern "C" int axb_qkv_norm_rope_bwd(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
+                                     const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos,
+                                     const float *dQh, const float *dKh, const float *dVh, int64_t B, int64_t S, int64_t H,
+                                     int64_t Hkv, int64_t dk, float *dqkv, float *dgq, float *dgk, void *workspace)
+{
+    if ((dgq && !gq) || (dgk && !gk)) return fail(AXB_ERR_NULL_ARG, "qkv_norm_rope_bwd: the gradient of a norm weight that is not given");
+    RopeArgs a;
+    int st = rope_args("qkv_norm_rope_bwd", a, qkv, bqkv, gq, gk, eps, freq, rot, pairing, amplitude, pos, B, S, H, Hkv, dk);
+    if (st) return st;
+    if (B == 0 || S == 0) return ensure_ready();
+    if (!dQh || !dKh || !dVh || !dqkv || ((gq || gk) && !qkv)) return fail(AXB_ERR_NULL_ARG, "qkv_norm_rope_bwd: NULL");
+    const int64_t nq = B * S * H * dk, nk = B * S * Hkv * dk, n = nq + 2 * nk;
+    if (overlaps(dqkv, n, dQh, nq) || overlaps(dqkv, n, dKh, nk) || overlaps(dqkv, n, dVh, nk) || ((gq || gk) && overlaps(dqkv, n, qkv, n)))
+        return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope_bwd: dqkv overlaps an input");
+    if ((st = ensure_ready())) return st;
+    OnDevice on;
+    a.q = const_cast<float *>(dQh); a.k = const_cast<float *>(dKh); a.v = const_cast<float *>(dVh);
+    a.dqkv = dqkv;
+    if (dgq || dgk) {
+        if ((st = attn_workspace("qkv_norm_rope_bwd", workspace))) return st;
+        a.partial = reinterpret_cast<float *>((char *)workspace + kAttnCounters);
+    }
+    int launched = 0;
+    int e = launch_qkv_norm_rope_bwd(a, dgq, dgk, cur().sm_count, cur().stream, &launched);
+    cur().launches += launched;
+    wrote_operands();
+    return e ? cuda_fail("qkv_norm_rope_bwd", e) : AXB_OK;
+}
+
+extern "C" int axb_kv_cache_extend(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
+                                   const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos,
+                                   const int32_t *lens, const int32_t *n_new, int64_t B, int64_t T, int64_t H, int64_t Hkv,
+                                   int64_t max_seq, int64_t dk, float *Qh, float *K_cache, float *V_cache)
+{
+    if (max_seq <= 0 || max_seq > INT32_MAX) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_extend: %lld cache rows", (long long)max_seq);
+    RopeArgs a;
+    int st = rope_args("kv_cache_extend", a, qkv, bqkv, gq, gk, eps, freq, rot, pairing, amplitude, pos, B, T, H, Hkv, dk);
+    if (st) return st;
+    if (B == 0 || T == 0) return ensure_ready();
+    if (!qkv || !lens || !Qh || !K_cache || !V_cache) return fail(AXB_ERR_NULL_ARG, "kv_cache_extend: NULL");
+    const int64_t nq = B * T * H * dk, n = nq + 2 * B * T * Hkv * dk, nc = B * Hkv * max_seq * dk;
+    if (overlaps(qkv, n, Qh, nq) || overlaps(qkv, n, K_cache, nc) || overlaps(qkv, n, V_cache, nc))
+        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_extend: an output overlaps qkv");
+    if ((st = ensure_ready())) return st;
+    OnDevice on;
+    a.lens = lens; a.n_new = n_new;
+    a.q = Qh; a.k = K_cache; a.v = V_cache;
+    a.kv_rows = max_seq;
+    a.err = cur().err_word;
+    int e = launch_qkv_norm_rope(a, cur().sm_count, cur().stream);
+    cur().launches++;
+    wrote_operands();
+    return e ? cuda_fail("kv_cache_extend", e) : AXB_OK;
+}
+
+extern "C" int axb_kv_cache_attend_tree(const float *K_cache, const float *V_cache, const float *Q, const uint64_t *mask,
+                                        int mask_per_seq, const int32_t *lens, const int32_t *n_new, float *out, int64_t B,
+                                        int64_t H, int64_t Hkv, int64_t T, int64_t max_seq, int64_t dk, float scale,
+                                        void *workspace)
+{
+    if (B < 0 || T < 0 || H <= 0 || Hkv <= 0 || H % Hkv || dk <= 0 || max_seq <= 0) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: bad shape");
+    if (dk > 128) return fail(AXB_ERR_NOT_IMPLEMENTED, "kv_cache_attend_tree: head dim %lld > 128", (long long)dk);
+    if (H > 65535 || B > INT32_MAX / Hkv || max_seq > INT32_MAX - 64 || T > INT32_MAX / H || (B && T * H > INT32_MAX / B))
+        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: dimension too large");
+    if (!isfinite(scale)) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: scale %g", (double)scale);
+    if (B == 0 || T == 0) return ensure_ready();
+    if (!K_cache || !V_cache || !Q || !lens || !out) return fail(AXB_ERR_NULL_ARG, "kv_cache_attend_tree: NULL");
+    const int64_t nq = B * H * T * dk, nc = B * Hkv * max_seq * dk;
+    if (overlaps(out, nq, Q, nq) || overlaps(out, nq, K_cache, nc) || overlaps(out, nq, V_cache, nc))
+        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: out overlaps an input");
+    int st = ensure_ready();
+    if (st) return st;
+    OnDevice on;
+    if ((st = attn_workspace("kv_cache_attend_tree", workspace))) return st;
+    KvTreeArgs a;
+    a.K = K_cache; a.V = V_cache; a.Q = Q; a.mask = mask; a.lens = lens; a.n_new = n_new; a.out = out;
+    a.counters = (int *)workspace;
+    a.slots = reinterpret_cast<float *>((char *)workspace + kAttnCounters);
+    a.words = (int)((T + 63) / 64);
+    a.mask_stride = mask_per_seq ? T * a.words : 0;
+    a.max_seq = max_seq; a.err = cur().err_word; a.c_log2 = scale * 1.4426950408889634f;
+    a.B = (int)B; a.H = (int)H; a.Hkv = (int)Hkv; a.T = (int)T; a.dk = (int)dk;
+    mark(0);
+    mark(1);
+    int e = launch_kv_cache_attend_tree(a, cur().sm_count, cur().stream);
+    mark(2);
+    cur().launches++;
+    wrote_operands();
+    return e ? cuda_fail("kv_cache_attend_tree", e) : AXB_OK;
+}
+
+extern "C" int axb_kv_cache_compact(float *K_cache, float *V_cache, const int32_t *keep, const int32_t *n_keep,
+                                    const int32_t *lens, int32_t *lens_out, int64_t B, int64_t Hkv, int64_t T, int64_t max_seq,
+                                    int64_t dk)
+{
+    if (B < 0 || T < 0 || Hkv <= 0 || dk <= 0 || max_seq <= 0) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_compact: bad shape");
+    if (B > INT32_MAX || T > INT32_MAX - 8 || max_seq > INT32_MAX || Hkv > 65535 || dk > 65535 / 8 || Hkv * dk > INT32_MAX / 4)
+        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_compact: dimension too large");
+    if (B == 0) return ensure_ready();
+    if (!K_cache || !V_cache || (!keep && T > 0) || !n_keep || !lens) return fail(AXB_ERR_NULL_ARG, "kv_cache_compact: NULL");
+    if (lens_out == lens || overlaps(lens_out, B, lens, B) || overlaps(lens_out, B, n_keep, B) || overlaps(lens_out, B, keep, B * T))
+        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_compact: lens_out overlaps an input");
+    const int64_t nc = B * Hkv * max_seq * dk;
+    if (overlaps(K_cache, nc, V_cache, nc)) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_compact: the caches overlap");
+    int st = ensure_ready();
+    if (st) return st;
+    OnDevice on;
+    int e = launch_kv_cache_compact(K_cache, V_cache, keep, n_keep, lens, lens_out, B, Hkv, T, max_seq, dk, cur().err_word, cur().stream);
+    cur().launches++;
+    wrote_operands();
+    return e ? cuda_fail("kv_cache_compact", e) : AXB_OK;
 }
 
 // ------------------------------------------------------- attention projections

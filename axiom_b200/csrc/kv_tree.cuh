@@ -1,0 +1,31 @@
+// kv_tree.cuh — launchers of the ragged-batch KV-cache kernels (kv_tree.cu): attention of T new tokens of every sequence
+// over its cached rows and over one another (a chain or a drafted tree), and the move of accepted rows.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace axb {
+
+struct KvTreeArgs {
+    const float *K, *V;          // [B*Hkv, max_seq, dk]
+    const float *Q;              // [B*H, T, dk]
+    const uint64_t *mask;        // [B or 1][T][words] bit j of token t: t attends to new token j; nullptr: j <= t
+    const int32_t *lens, *n_new; // [B]; n_new nullptr: T for every sequence
+    float *out;                  // [B*H, T, dk]
+    int *counters;               // one per SM, zero on entry and on exit
+    float *slots;                // kv_tree_workspace_bytes(): partial results, two slots per SM
+    int64_t max_seq, mask_stride;
+    int *err;
+    float c_log2;                // scale * log2(e)
+    int B, H, Hkv, T, dk, words;
+};
+
+size_t kv_tree_workspace_bytes(int sm_count);
+int launch_kv_cache_attend_tree(const KvTreeArgs &a, int sm_count, cudaStream_t st);
+
+// rows lens[b] + keep[b][i] -> lens[b] + i for i < n_keep[b] in both caches; lens_out[b] = lens[b] + n_keep[b] (or nullptr)
+int launch_kv_cache_compact(float *K, float *V, const int32_t *keep, const int32_t *n_keep, const int32_t *lens, int32_t *lens_out,
+                            int64_t B, int64_t Hkv, int64_t T, int64_t max_seq, int64_t dk, int *err, cudaStream_t st);
+
+}  // namespace axb

@@ -15,6 +15,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ENGINE_SO = os.path.join(PKG, "lib", "libaxiom_b200.so")
 
 ACT = {"none": 0, None: 0, "relu": 1, "gelu": 2}
+ROPE_SCALING = {"none": 0, None: 0, "linear": 1, "turns": 2, "index": 3}
+ROPE_PAIRING = {"half": 0, "interleaved": 1}
 FP32_MODES = {"3xtf32": 0, "bf16x3": 1, "bf16": 2}
 
 # every symbol include/axiom_b200.h declares
@@ -31,6 +33,8 @@ EXPORTS = [
     "axb_qgemm_w8a32_qw", "axb_bias_add_nd", "axb_head_interleave_qkv_split", "axb_head_interleave", "axb_head_deinterleave",
     "axb_head_deinterleave_qkv_merge", "axb_qkv_cache_build", "axb_bias_cache_build", "axb_pointer_on_device",
     "axb_weight_prepare", "axb_weight_release", "axb_gemm_prepared",
+    "axb_rope_frequencies", "axb_qkv_norm_rope", "axb_qkv_norm_rope_bwd", "axb_kv_cache_extend", "axb_kv_cache_attend_tree",
+    "axb_kv_cache_compact", "axb_attention_workspace_bytes",
     "axb_mgpu_create", "axb_mgpu_destroy", "axb_mgpu_size", "axb_mgpu_device", "axb_mgpu_alloc", "axb_mgpu_free", "axb_mgpu_h2d",
     "axb_mgpu_d2h", "axb_mgpu_synchronize", "axb_mgpu_gemm_rows", "axb_mgpu_qgemm_w8a8_rows", "axb_mgpu_gemm_cols_allgather",
 ]
@@ -79,6 +83,15 @@ class Engine:
         L.axb_gemm_prepared.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_float, C.c_int]
         for name in ("axb_memcpy_h2d", "axb_memcpy_d2h", "axb_memcpy_d2d"):
             getattr(L, name).argtypes = [C.c_void_p, C.c_void_p, C.c_size_t]
+        vp, i64 = C.c_void_p, C.c_int64
+        L.axb_attention_workspace_bytes.restype = C.c_size_t
+        L.axb_rope_frequencies.argtypes = [i64, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, i64, vp]
+        rope = [vp, vp, vp, vp, C.c_float, vp, i64, C.c_int, C.c_float, vp]
+        L.axb_qkv_norm_rope.argtypes = rope + [i64] * 5 + [vp] * 3
+        L.axb_qkv_norm_rope_bwd.argtypes = rope + [vp] * 3 + [i64] * 5 + [vp] * 4
+        L.axb_kv_cache_extend.argtypes = rope + [vp] * 2 + [i64] * 6 + [vp] * 3
+        L.axb_kv_cache_attend_tree.argtypes = [vp] * 4 + [C.c_int] + [vp] * 3 + [i64] * 6 + [C.c_float, vp]
+        L.axb_kv_cache_compact.argtypes = [vp] * 6 + [i64] * 5
         if device is not None:
             self._check(L.axb_init(int(device)))
 
@@ -384,6 +397,119 @@ class Engine:
         self._check(self.lib.axb_kv_cache_attend(_ptr(K_cache), _ptr(V_cache), _ptr(Q_new), _ptr(out), _i64(BH),
                                                  _i64(cur_len), _i64(max_seq), _i64(dk), _f(scale)))
         return out
+
+    # ---- rotary positions, per-head norms, KV cache of a ragged batch ----
+    def rope_frequencies(self, rot, base=10000.0, scaling="none", factor=1.0, low=1.0, high=32.0, original_len=0):
+        """Radians per position of the rot/2 pairs (a list of floats; make it a CUDA double tensor once)."""
+        out = (C.c_double * max(rot // 2, 1))()
+        self._check(self.lib.axb_rope_frequencies(rot, base, ROPE_SCALING[scaling], factor, low, high, original_len, out))
+        return list(out[:rot // 2])
+
+    @staticmethod
+    def _addr(t, dtype=None):
+        # dtype: the name of the element type a buffer must have ("float32" unless said otherwise)
+        if t is None or isinstance(t, int):
+            return t
+        if not t.is_contiguous() or str(t.dtype) != "torch." + (dtype or "float32"):
+            raise ValueError(f"a contiguous {dtype or 'float32'} tensor is wanted, got {t.dtype}, strides {tuple(t.stride())}")
+        return t.data_ptr()
+
+    def _rope(self, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos):
+        p = self._addr
+        return (p(qkv), p(bias), p(gq), p(gk), eps, p(freq, "float64"), 0 if freq is None else 2 * freq.numel(), ROPE_PAIRING[pairing],
+                amplitude, p(pos, "int32"))
+
+    @staticmethod
+    def _shape(ok, what):
+        if not ok:
+            raise ValueError(what)
+
+    def _check_rope(self, rows, H, Hkv, dk, qkv, bias, gq, gk, pos):
+        width = (H + 2 * Hkv) * dk
+        self._shape(qkv is None or tuple(qkv.shape) == (rows, width) or qkv.shape[0] == rows == 0, f"qkv: [{rows}, {width}] is wanted")
+        self._shape(bias is None or bias.numel() == width, f"bias: [{width}] is wanted")
+        self._shape(all(g is None or g.numel() == dk for g in (gq, gk)), f"norm weights: [{dk}] is wanted")
+        self._shape(pos is None or pos.numel() == rows, f"pos: {rows} positions are wanted")
+
+    def qkv_norm_rope(self, qkv, Qh, Kh, Vh, B, bias=None, gq=None, gk=None, eps=1e-6, freq=None, pairing="half", amplitude=1.0,
+                      pos=None):
+        """qkv [B*S, (H + 2*Hkv)*dk] -> head-major Qh [B*H, S, dk], Kh, Vh [B*Hkv, S, dk]: bias, per-head RMS norm, rotation."""
+        (BH, S, dk), BHkv = Qh.shape, Kh.shape[0]
+        H, Hkv = (BH // B, BHkv // B) if B else (1, 1)
+        self._shape(B * H == BH and B * Hkv == BHkv and tuple(Kh.shape) == tuple(Vh.shape) == (BHkv, S, dk), "Qh, Kh, Vh: head-major shapes")
+        self._check_rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, pos)
+        p = self._addr
+        self._check(self.lib.axb_qkv_norm_rope(*self._rope(qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos), B, S, H, Hkv, dk,
+                                               p(Qh), p(Kh), p(Vh)))
+        return Qh, Kh, Vh
+
+    def qkv_norm_rope_bwd(self, dQh, dKh, dVh, dqkv, B, qkv=None, bias=None, gq=None, gk=None, eps=1e-6, freq=None, pairing="half",
+                          amplitude=1.0, pos=None, dgq=None, dgk=None, workspace=None):
+        """dqkv from the head-major gradients; dgq, dgk (the norm weights' gradients) are added to."""
+        (BH, S, dk), BHkv = dQh.shape, dKh.shape[0]
+        H, Hkv = (BH // B, BHkv // B) if B else (1, 1)
+        self._shape(B * H == BH and B * Hkv == BHkv and tuple(dKh.shape) == tuple(dVh.shape) == (BHkv, S, dk), "dQh, dKh, dVh: head-major shapes")
+        self._check_rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, pos)
+        self._shape(tuple(dqkv.shape) == (B * S, (H + 2 * Hkv) * dk) and all(g is None or g.numel() == dk for g in (dgq, dgk)),
+                    "dqkv, dgq, dgk: shapes")
+        p = self._addr
+        self._check(self.lib.axb_qkv_norm_rope_bwd(*self._rope(qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos), p(dQh), p(dKh), p(dVh),
+                                                   B, S, H, Hkv, dk, p(dqkv), p(dgq), p(dgk), self._workspace(workspace)))
+        return dqkv
+
+    def attention_workspace_bytes(self):
+        n = int(self.lib.axb_attention_workspace_bytes())
+        if n == 0:
+            raise EngineError(9, self.last_error())
+        return n
+
+    def _workspace(self, ws):
+        if ws is None or isinstance(ws, int):
+            return ws
+        self._shape(ws.is_contiguous() and ws.numel() * ws.element_size() >= self.attention_workspace_bytes(), "workspace: too small")
+        return ws.data_ptr()
+
+    def kv_cache_extend(self, qkv, Qh, K_cache, V_cache, lens, n_new=None, bias=None, gq=None, gk=None, eps=1e-6, freq=None,
+                        pairing="half", amplitude=1.0, pos=None):
+        """The tokens qkv [B*T, (H + 2*Hkv)*dk] of a ragged batch: queries to Qh [B*H, T, dk], keys and values to cache rows
+        lens[b] + t of K_cache, V_cache [B*Hkv, max_seq, dk]."""
+        B, (BH, T, dk), (BHkv, max_seq, _) = lens.numel(), Qh.shape, K_cache.shape
+        H, Hkv = (BH // B, BHkv // B) if B else (1, 1)
+        self._shape(B * H == BH and B * Hkv == BHkv and tuple(K_cache.shape) == tuple(V_cache.shape) == (BHkv, max_seq, dk),
+                    "Qh, K_cache, V_cache: head-major shapes")
+        self._check_rope(B * T, H, Hkv, dk, qkv, bias, gq, gk, pos)
+        self._shape(n_new is None or n_new.numel() == B, "n_new: one count for each sequence")
+        p = self._addr
+        self._check(self.lib.axb_kv_cache_extend(*self._rope(qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos), p(lens, "int32"),
+                                                 p(n_new, "int32"), B, T, H, Hkv, max_seq, dk, p(Qh), p(K_cache), p(V_cache)))
+        return Qh
+
+    def kv_cache_attend_tree(self, K_cache, V_cache, Q, out, lens, scale, n_new=None, mask=None, workspace=None):
+        """Attention of Q [B*H, T, dk] over cache rows [0, lens[b]) and the new rows lens[b] + j that mask (int64 bit words
+        [B, T, ceil(T/64)], or [T, ceil(T/64)] for all sequences; None: j <= t) lets token t see."""
+        B, (BH, T, dk), (BHkv, max_seq, _) = lens.numel(), Q.shape, K_cache.shape
+        H, Hkv = (BH // B, BHkv // B) if B else (1, 1)
+        self._shape(B * H == BH and B * Hkv == BHkv and tuple(K_cache.shape) == tuple(V_cache.shape) == (BHkv, max_seq, dk) and
+                    tuple(out.shape) == tuple(Q.shape), "Q, out, K_cache, V_cache: head-major shapes")
+        words = (T + 63) // 64
+        self._shape(mask is None or tuple(mask.shape) in ((B, T, words), (T, words)), f"mask: [{B}, {T}, {words}] or [{T}, {words}] is wanted")
+        self._shape(n_new is None or n_new.numel() == B, "n_new: one count for each sequence")
+        p = self._addr
+        self._check(self.lib.axb_kv_cache_attend_tree(p(K_cache), p(V_cache), p(Q), p(mask, "int64"), int(mask is not None and mask.dim() == 3),
+                                                      p(lens, "int32"), p(n_new, "int32"), p(out), B, H, Hkv, T, max_seq, dk, scale,
+                                                      self._workspace(workspace)))
+        return out
+
+    def kv_cache_compact(self, K_cache, V_cache, keep, n_keep, lens, lens_out=None):
+        """Cache rows lens[b] + keep[b, i] move to lens[b] + i for i < n_keep[b]; lens_out[b] = lens[b] + n_keep[b]."""
+        B, T, (BHkv, max_seq, dk) = lens.numel(), keep.shape[-1], K_cache.shape
+        Hkv = BHkv // B if B else 1
+        self._shape(B * Hkv == BHkv and tuple(K_cache.shape) == tuple(V_cache.shape) and keep.numel() == B * T and n_keep.numel() == B and
+                    (lens_out is None or lens_out.numel() == B), "K_cache, V_cache, keep, n_keep, lens_out: shapes")
+        p = self._addr
+        self._check(self.lib.axb_kv_cache_compact(p(K_cache), p(V_cache), p(keep, "int32"), p(n_keep, "int32"), p(lens, "int32"),
+                                                  p(lens_out, "int32"), B, Hkv, T, max_seq, dk))
+        return lens_out
 
 
 class MultiGpu:

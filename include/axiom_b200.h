@@ -40,6 +40,12 @@ extern "C" {
 #define AXB_ERR_BACKEND 9
 #define AXB_ERR_NOT_IMPLEMENTED 10
 
+/* axb_device_error codes of the ragged-batch entry points: a sequence whose length and new tokens do not fit its
+   rows of the cache, and an accepted-token list that is not strictly ascending or leaves the drafted rows.  The kernel
+   leaves everything of such a sequence as it was and serves the others. */
+#define AXB_DEVERR_ROWS 101
+#define AXB_DEVERR_KEEP 102
+
 /* activation selectors for the fused epilogues */
 #define AXB_ACT_NONE 0
 #define AXB_ACT_RELU 1
@@ -70,7 +76,8 @@ AXB_API void axb_set_stream(void *cuda_stream); /* NULL = legacy default stream 
 AXB_API int axb_set_fp32_mode(int mode);        /* AXB_FP32_* */
 AXB_API int axb_get_fp32_mode(void);
 AXB_API const char *axb_last_error(void);
-/* Non-zero when a kernel gave up on a bounded wait (its code); reading clears it. */
+/* Non-zero when a kernel gave up on a bounded wait (its code) or refused values that only the device sees
+   (AXB_DEVERR_*); reading clears it. */
 AXB_API int axb_device_error(void);
 /* Kernels enqueued by this library since the counter was last reset. */
 AXB_API int64_t axb_launch_count(int reset);
@@ -420,6 +427,84 @@ AXB_API int axb_kv_cache_append(float *K_cache, float *V_cache, const float *new
                                 int64_t cur_len, int64_t max_seq, int64_t dk);
 AXB_API int axb_kv_cache_attend(const float *K_cache, const float *V_cache, const float *Q_new, float *out,
                                 int64_t BH, int64_t cur_len, int64_t max_seq, int64_t dk, float scale);
+
+/* ---- rotary positions and per-head norms of queries and keys (no counterpart in the reference) ---------------
+   Radians per position of the rot/2 rotated pairs of a head, in 64 bits, into the HOST array freq_host (copy it to the
+   device once and hand it to the calls below): base^(-2i/rot), changed for contexts longer than trained on by
+     AXB_ROPE_LINEAR      f / factor
+     AXB_ROPE_RAMP_TURNS  f * (w + (1 - w) / factor), w = clamp((turns - low) / (high - low), 0, 1), where
+                          turns = original_len * f / 2 pi
+     AXB_ROPE_RAMP_INDEX  the same blend with w falling linearly in the pair's index, from the index at which a pair
+                          makes `high` turns over original_len (rounded down) to that of `low` turns (rounded up)
+   factor > 0; the ramps want 0 < low < high and original_len > 0.  Needs no device. */
+#define AXB_ROPE_PLAIN 0
+#define AXB_ROPE_LINEAR 1
+#define AXB_ROPE_RAMP_TURNS 2
+#define AXB_ROPE_RAMP_INDEX 3
+AXB_API int axb_rope_frequencies(int64_t rot, double base, int scaling, double factor, double low, double high,
+                                 int64_t original_len, double *freq_host);
+
+/* which elements of a head form pair i: (i, i + rot/2), or (2i, 2i + 1); elements from rot on are not rotated */
+#define AXB_ROPE_HALF 0
+#define AXB_ROPE_INTERLEAVED 1
+
+/* q | k | v of a projection, flat [B*S, (H + 2*Hkv)*dk], to head-major Qh [B*H, S, dk], Kh, Vh [B*Hkv, S, dk] — the pass
+   of axb_head_interleave_qkv_split — with, on the way, per element or head of q and k:
+     + bqkv [(H + 2*Hkv)*dk]                       (v too; NULL: none)
+     * g / sqrt(mean(x^2) + eps), g = gq, gk [dk]  (NULL: that tensor is not normed)
+     rotation of the first rot elements by p * freq[i], the results times amplitude   (rot == 0: none, freq may be NULL)
+   p = pos[b*S + s] (int32), or s when pos is NULL.  freq: [rot/2] doubles on the device.  H is a multiple of Hkv; rot is
+   even and at most dk; dk <= 256.  The outputs may not overlap qkv. */
+AXB_API int axb_qkv_norm_rope(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
+                              const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos, int64_t B,
+                              int64_t S, int64_t H, int64_t Hkv, int64_t dk, float *Qh, float *Kh, float *Vh);
+/* Its gradient: dQh, dKh, dVh head-major -> dqkv flat (overwritten), and the norm weights' gradients, ACCUMULATED:
+   dgq [dk], dgk [dk] += ... (each may be NULL).  qkv, bqkv, gq, gk and the rest are those of the forward call; qkv may be
+   NULL when neither gq nor gk is given.  The gradient of bqkv is the column sums of dqkv (axb_gemm with a row of ones).
+   dqkv may not overlap an input.  workspace: see axb_attention_workspace_bytes; needed only when dgq or dgk is wanted.
+   Bitwise repeatable. */
+AXB_API int axb_qkv_norm_rope_bwd(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
+                                  const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos,
+                                  const float *dQh, const float *dKh, const float *dVh, int64_t B, int64_t S, int64_t H,
+                                  int64_t Hkv, int64_t dk, float *dqkv, float *dgq, float *dgk, void *workspace);
+
+/* ---- KV cache of a ragged batch (no counterpart in the reference, whose cache takes one token at one length) -------
+   The cache layout is axb_kv_cache_append's, [B*Hkv, max_seq, dk] for K and V; lens [B] (int32, device) holds the cached rows of
+   every sequence and n_new [B] (int32, device; NULL: T for all) how many of the T new-token slots of a sequence are in
+   use.  New token t of sequence b has cache row lens[b] + t.  What belongs to slots behind n_new[b] is neither read nor
+   written.  Lengths are checked on the device (0 <= lens, 0 <= n_new <= T, lens + n_new <= max_seq; AXB_DEVERR_ROWS).
+   The caller owns lens: none of these calls changes it.  T new tokens of a step, in order:
+     axb_kv_cache_extend -> axb_kv_cache_attend_tree -> (accept) -> axb_kv_cache_compact. */
+
+/* axb_qkv_norm_rope of qkv [B*T, (H + 2*Hkv)*dk] whose keys and values go to their cache rows; queries to Qh [B*H, T, dk].
+   pos [B*T], or NULL for lens[b] + t (in a drafted tree a token's position is lens[b] + its depth). */
+AXB_API int axb_kv_cache_extend(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
+                                const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos,
+                                const int32_t *lens, const int32_t *n_new, int64_t B, int64_t T, int64_t H, int64_t Hkv,
+                                int64_t max_seq, int64_t dk, float *Qh, float *K_cache, float *V_cache);
+/* out [B*H, T, dk] = softmax(scale * Q.K^T) . V of the new tokens over the cached rows [0, lens[b]) and the new rows they
+   see; query head h uses key head h / (H / Hkv).  mask: bit j % 64 of word j / 64 of mask[b][t][ceil(T/64)] says whether
+   token t sees new token j (its ancestors and itself, in a drafted tree; bits from n_new[b] on are ignored); mask_per_seq
+   == 0: one [T][ceil(T/64)] mask for all sequences.  mask NULL: token t sees new tokens 0 .. t.  A token that sees
+   nothing gets 0.  Values in rows a token does not see do not reach it, infinities and NaN included.  T = 1 is
+   single-token decode at every sequence's own length.  dk <= 128.  workspace: below.  Bitwise repeatable. */
+AXB_API int axb_kv_cache_attend_tree(const float *K_cache, const float *V_cache, const float *Q, const uint64_t *mask,
+                                     int mask_per_seq, const int32_t *lens, const int32_t *n_new, float *out, int64_t B,
+                                     int64_t H, int64_t Hkv, int64_t T, int64_t max_seq, int64_t dk, float scale,
+                                     void *workspace);
+/* After a step of drafted tokens: rows lens[b] + keep[b][i] of both caches move to lens[b] + i, i < n_keep[b].
+   keep: int32 [B][T], strictly ascending indices below T with their rows inside the cache; n_keep: int32 [B], 0 .. T
+   (AXB_DEVERR_KEEP otherwise).  Every other row is left as it was.  lens_out [B] (may be NULL, may not be lens) receives
+   lens[b] + n_keep[b], or lens[b] for a sequence that was refused. */
+AXB_API int axb_kv_cache_compact(float *K_cache, float *V_cache, const int32_t *keep, const int32_t *n_keep,
+                                 const int32_t *lens, int32_t *lens_out, int64_t B, int64_t Hkv, int64_t T, int64_t max_seq,
+                                 int64_t dk);
+/* Bytes of the workspace that axb_qkv_norm_rope_bwd and axb_kv_cache_attend_tree take (one size for every call; 0
+   without a device).  workspace = NULL takes the engine's own, made by the first call that needs it (not inside a stream
+   capture) and never moved: right for calls that follow one another on a stream.  Calls that may overlap on the GPU —
+   other streams, or captured graphs replayed side by side — need a workspace each: 16-byte aligned, zero-filled once
+   before its first use (axb_storage_alloc's memory is), then left to the calls. */
+AXB_API size_t axb_attention_workspace_bytes(void);
 
 #ifdef __cplusplus
 }
