@@ -5,27 +5,29 @@
 // A row that sees nothing gives 0.  The tokens and heads that share a key head are the rows of one small product, so K
 // and V are read once for all of them: HBM-bound while those rows are few, bound by the tensor cores when they are many.
 //
-// Both products run as three tf32 products over hi/lo parts (lo.hi + hi.lo + hi.hi, fp32-accurate; hi is the value as it
-// lies, of which the tensor core reads the tf32 part, lo the exact remainder) with warp-level mma.m16n8k8: 16 query
-// rows fit decode far better than the 128 rows of a tcgen05 tile.  Measured rate of that instruction: 512 multiply-adds
-// a clock and SM, so three products of 16 rows need 0.55 of the time in which HBM delivers the keys, of 32 rows 1.1.
-// Its layouts cost nothing here:
-//   * the contraction index is free, so a lane's 16-byte load of a K row (elements 4t .. 4t+3 of 16) serves two k steps;
-//   * the accumulator of Q.K^T (row g, key columns 2t, 2t+1) IS the A operand of P.V with keys 2t, 2t+1 as k = t, t+4;
-//   * tiles lie as TMA leaves them (128-byte rows, 16-byte chunks XOR-ed with the row's low bits); key column c of an
-//     8-key group is row perm(c) = {0,5,2,7,4,1,6,3}, which makes both the K loads (two rows a phase, their halves
-//     of the 128 bytes swapped by bit 2) and the V loads (four rows a phase, two chunks each) conflict-free.
-// The tensor core's truncating accumulation never spans more than a tile: every tile's P.V starts from zero and is folded
+// Both products run transposed, S^T = K.Q^T and O^T = V^T.P^T, as three tf32 products over hi/lo parts (lo.hi + hi.lo +
+// hi.hi, fp32-accurate) with warp-level mma.m16n8k8: keys (and head dims) fill the 16 side, query rows come in eights —
+// a decode step has 1 to 32 of them, far from the 128 rows of a tcgen05 tile.  Measured rate of that instruction: 512
+// multiply-adds a clock and SM, so three products of 8 rows take 0.27 of the time in which HBM delivers the keys, of 32
+// rows 1.1.  Every element of K and V is split once for all rows of the warp.  The layouts cost nothing:
+//   * the contraction index is free, so a lane's 16-byte load of a K row (elements 4t .. 4t+3 of 16) serves two k steps, and
+//     that of a V row (columns 4g .. 4g+3 of 32) serves rows g and g+8 of two 16-column tiles;
+//   * tiles lie as TMA leaves them (128-byte rows, 16-byte chunks XOR-ed with the row's low bits).  Row g of an 8-key
+//     group is key perm(g) = {0,5,2,7,4,1,6,3}: the two rows of a load phase then differ in bit 2 and take the two halves
+//     of the 128 bytes; V is read in key order (2t, 2t+1 as k = t, t+4), four rows a phase, two chunks each.  Neither
+//     meets a bank twice;
+//   * P^T changes from accumulator to operand layout with two shuffles a value inside the warp.
+// The tensor core's truncating accumulation never spans more than 16 keys: P.V starts from zero every time and is folded
 // into fp32 registers with the online-softmax factor in the same multiply-add.
 //
-// Work split: the tiles of 64 keys of all (sequence, key head, row block) items form one line, cut into equal pieces,
+// Work split: the tiles of 32 keys of all (sequence, key head, row block) items form one line, cut into equal pieces,
 // one per SM — lengths differ by orders of magnitude in a batch, and the device knows them, not the host.  A piece that
 // does not hold an item's whole line leaves (max, sum, unnormalised output) in its workspace slot; the CTA that
 // arrives last at the item's counter adds the pieces in line order (nobody waits; the result does not depend on who was
 // last) and clears the counter.
 //
-// One CTA per SM: warp 8 feeds K and V tiles through separate rings; warps 0-7 each own 16 rows x a slice of a tile's
-// keys with a running softmax of their own, merged through shared memory at the end of a piece.
+// One CTA per SM: a producer warp feeds K and V tiles through a ring; eight warps each take 16 keys of a tile with
+// a running softmax of their own, merged in registers through shared memory at the end of a piece.
 #include "kv_tree.cuh"
 
 #include "errors.cuh"
@@ -38,26 +40,35 @@
 
 namespace axb {
 
-static constexpr int KT_KEYS = 64, KT_CONSUMERS = 8, KT_THREADS = (KT_CONSUMERS + 1) * 32;
-static constexpr int KT_MAX_ROWS = 64;   // query rows of an item
+static constexpr int KT_KEYS = 32, KT_CONSUMERS = 8;
+static constexpr size_t KT_SLOT_BYTES = 2 * 32 * 36 * 16;   // the largest variant's partial result
 enum { TERR_PRODUCER = 91, TERR_CONSUMER = 92 };
 
-// DKP: head dim rounded up to 32 (the tiles' columns beyond dk read as zero).  MT: 16-row tiles of an item.
-template <int DKP, int MT>
+// DKP: head dim rounded up to 32 (the tiles' columns beyond dk read as zero).  NR: query rows of a warp, in eights.
+// RG: groups of warps that share a tile's keys and differ in their query rows.
+template <int DKP, int NR, int RG>
 struct TreeCfg {
-    static constexpr int KEYS_WARP = MT == 4 ? 32 : 16;              // keys of a tile that one warp takes
-    static constexpr int SLICES = KT_KEYS / KEYS_WARP;               // warps side by side on a tile's keys
-    static constexpr int GROUPS = KT_CONSUMERS / (MT * SLICES);      // tiles in work at the same time (2 for one row tile)
-    static constexpr int PARTS = SLICES * GROUPS;                    // partial results of a row tile
-    static constexpr int NT = KEYS_WARP / 8;
-    static constexpr int TILE = KT_KEYS * DKP * 4;                   // bytes of a K or V tile
-    static constexpr int MERGE = PARTS * MT * 16 * (DKP + 4 + 2) * 4;
-    static constexpr int STAGES = (220 * 1024 - MERGE) / (2 * TILE) < 6 ? (220 * 1024 - MERGE) / (2 * TILE) : 6;
-    static constexpr int SMEM = 1024 + STAGES * 2 * TILE + MERGE;
+    static constexpr int ROWS = 8 * NR * RG;                          // query rows of an item
+    static constexpr int SLICES = KT_KEYS / 16;                       // warps side by side on a tile's keys
+    static constexpr int PARTS = KT_CONSUMERS / RG;                   // warps with the same query rows
+    static constexpr int GROUPS = PARTS / SLICES;                     // tiles in work at the same time
+    static constexpr int FRAGS = DKP / 16 * NR;                       // float4 of a lane's O^T
+    static constexpr bool SPLIT_Q = NR < 4;                           // Q lies in shared memory as hi and lo
+    static constexpr int TILE = KT_KEYS * DKP * 4;                    // bytes of a K or V tile
+    static constexpr int Q_BYTES = ROWS * DKP * 4 * (SPLIT_Q ? 2 : 1);
+    static constexpr int MERGE_BYTES = KT_CONSUMERS / 2 * 32 * (FRAGS + NR) * 16;
+    static constexpr int AREA = Q_BYTES > MERGE_BYTES ? Q_BYTES : MERGE_BYTES;   // first Q, then the merge
+    static constexpr int ROOM = (224 * 1024 - AREA) / (2 * TILE);
+    static constexpr int STAGES = ROOM < 8 ? ROOM : 8;
+    static constexpr int SMEM = 1024 + STAGES * 2 * TILE + AREA;
+    // four rows in eights and 128 columns need more than the 168 registers that nine warps leave a thread: with twelve
+    // warps the producer's four hand theirs to the consumers
+    static constexpr bool SHIFT_REGS = NR == 4 || (NR == 2 && DKP == 128);
+    static constexpr int THREADS = (KT_CONSUMERS + (SHIFT_REGS ? 4 : 1)) * 32;
 };
 
 struct TreeMaps {
-    CUtensorMap k, v;   // [B*Hkv][max_seq][dk], boxes of 32 columns x 64 rows
+    CUtensorMap k, v;   // [B*Hkv][max_seq][dk], boxes of 32 columns x 32 rows
 };
 
 struct TreeSeq {
@@ -122,14 +133,15 @@ __device__ __forceinline__ bool next_piece(const KvTreeArgs &a, TreeCursor &c, i
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// what the tensor core does not read of x, exactly
-__device__ __forceinline__ uint32_t tf32_rest(float x)
+// The lo part of x: what the tensor core, which reads the upper 19 bits of an operand, leaves of x as a hi operand; rounded
+// to the bits it will read (cut, it would keep the sign of x — a bias that the sums over columns and keys add up).
+__device__ __forceinline__ uint32_t tf32_lo(float x)
 {
-    return __float_as_uint(x - __uint_as_float(__float_as_uint(x) & 0xffffe000u));
+    return __float_as_uint(x - __uint_as_float(__float_as_uint(x) & 0xffffe000u)) + 0x1000u;
 }
 
 __device__ __forceinline__ float4 lds128(const uint8_t *p) { return *reinterpret_cast<const float4 *>(p); }
@@ -140,8 +152,8 @@ __device__ __forceinline__ uint32_t tile_at(int row, int slab, int chunk)
     return (uint32_t)(slab * (KT_KEYS * 128) + row * 128 + ((chunk ^ (row & 7)) << 4));
 }
 
-// row of an 8-key group behind key column c
-__device__ __forceinline__ int key_perm(int c) { return c & 1 ? (c - 1) ^ 5 : c; }
+// key behind row g of an 8-key group of S^T
+__device__ __forceinline__ int key_perm(int g) { return g & 1 ? g ^ 4 : g; }
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(KT_CONSUMERS * 32) : "memory"); }
 
@@ -154,97 +166,117 @@ __device__ __forceinline__ bool tree_sees(const KvTreeArgs &a, int b, int t, int
     return (__ldg(a.mask + b * a.mask_stride + (int64_t)t * a.words + (j >> 6)) >> (j & 63)) & 1;
 }
 
-template <int DKP, int MT>
+// What a lane (g = lane / 4, t = lane % 4) holds of its warp's query rows.  o[i][n]: columns 32*(i/2) + 4g + 2*(i%2) (elements
+// 0: row 8n + 2t, 1: row 8n + 2t + 1) and the column behind it (elements 2, 3).
+template <int DKP, int NR>
 struct TreeWarp {
-    using C = TreeCfg<DKP, MT>;
-    float o[DKP / 32][4][4];    // [slab][e]: rows g, g+8 x columns 32*slab + 8t + e and + 4
-    float m[2], l[2];           // running maximum (log2 domain) and this lane's part of the sum
+    float o[DKP / 16][NR][4];
+    float m[NR][2], l[NR][2];   // running maximum (log2 domain) and sum of rows 8n + 2t, 8n + 2t + 1; l of this lane's keys
 };
 
-// One tile for one warp: its 16 rows against KEYS_WARP keys.  TAIL: the tile holds rows behind the cached ones.
-template <int DKP, int MT, bool TAIL>
-__device__ __forceinline__ void tree_tile(const KvTreeArgs &a, TreeWarp<DKP, MT> &w, const uint8_t *qbase, const uint8_t *kbase, const uint8_t *vbase, int key0, const TreeSeq &s,
-                                          int b, int tok_a, int tok_b, uint32_t v_full, uint32_t v_parity, bool &ok)
+// One warp, 16 keys.  TAIL: some of them lie behind the cached rows.  toks: the token of each of the warp's query rows.
+template <int DKP, int NR, int RG, bool TAIL>
+__device__ __forceinline__ void tree_tile(const KvTreeArgs &a, TreeWarp<DKP, NR> &w, const uint8_t *qbase, const uint8_t *kbase, const uint8_t *vbase,
+                                          int key0, int row0, const TreeSeq &s, int b, const int *toks, uint32_t k_empty, uint32_t v_full,
+                                          uint32_t v_parity, bool &ok)
 {
-    using C = TreeCfg<DKP, MT>;
+    using C = TreeCfg<DKP, NR, RG>;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int slice = (threadIdx.x >> 5) / MT % C::SLICES, row0 = slice * C::KEYS_WARP;
-    float sc[C::NT][4];
+    // S^T: rows g, g+8 = keys row0 + perm(g) (+ 8), columns 2t, 2t+1 of each eight query rows; the cross products in chains of
+    // their own, which shortens the dependent chain
+    float sc[NR][4], x1[NR][4], x2[NR == 1 ? NR : 1][4];
 #pragma unroll
-    for (int i = 0; i < C::NT; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            sc[n][e] = x1[n][e] = 0.f;
+            if (NR == 1) x2[0][e] = 0.f;
+        }
     const int krow = row0 + key_perm(g);
-#pragma unroll
+#pragma unroll 2
     for (int j = 0; j < DKP / 16; ++j) {
-        const float4 qa = lds128(qbase + (2 * j) * 512), qb = lds128(qbase + (2 * j + 1) * 512);   // rows g, g+8: elements 16j + 4t .. +3
+        const float4 ka = lds128(kbase + tile_at(krow, j >> 1, 4 * (j & 1) + t)), kb = lds128(kbase + tile_at(krow + 8, j >> 1, 4 * (j & 1) + t));
         // [k step]: rows g, g+8 at k = t, then at k = t + 4
-        const float x[2][4] = { { qa.x, qb.x, qa.y, qb.y }, { qa.z, qb.z, qa.w, qb.w } };
+        const float kx[2][4] = { { ka.x, kb.x, ka.y, kb.y }, { ka.z, kb.z, ka.w, kb.w } };
         uint32_t hi[2][4], lo[2][4];
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                hi[st][e] = __float_as_uint(x[st][e]);
-                lo[st][e] = tf32_rest(x[st][e]);
+                hi[st][e] = __float_as_uint(kx[st][e]);
+                lo[st][e] = tf32_lo(kx[st][e]);
             }
 #pragma unroll
-        for (int i = 0; i < C::NT; ++i) {
-            const float4 k4 = lds128(kbase + tile_at(krow + 8 * i, j >> 1, 4 * (j & 1) + t));
-            const uint32_t h[4] = { __float_as_uint(k4.x), __float_as_uint(k4.y), __float_as_uint(k4.z), __float_as_uint(k4.w) };
-            const uint32_t r[4] = { tf32_rest(k4.x), tf32_rest(k4.y), tf32_rest(k4.z), tf32_rest(k4.w) };
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                mma_tf32(sc[i], lo[st], h[2 * st], h[2 * st + 1]);
-                mma_tf32(sc[i], hi[st], r[2 * st], r[2 * st + 1]);
-                mma_tf32(sc[i], hi[st], h[2 * st], h[2 * st + 1]);
-            }
+        for (int n = 0; n < NR; ++n) {
+            const uint8_t *qp = qbase + (n * (DKP / 16) + j) * (C::SPLIT_Q ? 1024 : 512);
+            const float4 q = lds128(qp);
+            float4 r;
+            if (C::SPLIT_Q) r = lds128(qp + 512);
+            else r = make_float4(__uint_as_float(tf32_lo(q.x)), __uint_as_float(tf32_lo(q.y)), __uint_as_float(tf32_lo(q.z)), __uint_as_float(tf32_lo(q.w)));
+            mma_tf32(x1[n], lo[0], __float_as_uint(q.x), __float_as_uint(q.y));
+            mma_tf32(sc[n], hi[0], __float_as_uint(q.x), __float_as_uint(q.y));
+            mma_tf32(NR == 1 ? x2[0] : x1[n], hi[0], __float_as_uint(r.x), __float_as_uint(r.y));
+            mma_tf32(x1[n], lo[1], __float_as_uint(q.z), __float_as_uint(q.w));
+            mma_tf32(sc[n], hi[1], __float_as_uint(q.z), __float_as_uint(q.w));
+            mma_tf32(NR == 1 ? x2[0] : x1[n], hi[1], __float_as_uint(r.z), __float_as_uint(r.w));
         }
     }
-    // scores in the log2 domain, the row maxima, the factor on what was summed before
-    float mx[2] = { -INFINITY, -INFINITY };
+    __syncwarp();
+    if (lane == 0) mbar_arrive(k_empty);
+    // scores in the log2 domain, the row maxima, the factor on what was summed before, P^T as operand B (k = t, t+4: keys 2t,
+    // 2t+1 of each eight; column g: query row 8n + g)
+    float corr[NR][2];
+    uint32_t phi[NR][4], plo[NR][4];
+    const int from = 8 * t + (g >> 1);               // lane that holds key 2t (row 2t of S^T) and query row g; key 2t+1: row (2t+1)^4
+    const int from1 = 4 * ((2 * t + 1) ^ 4) + (g >> 1);
 #pragma unroll
-    for (int i = 0; i < C::NT; ++i)
+    for (int n = 0; n < NR; ++n) {
+        float mx[2] = { -INFINITY, -INFINITY };
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float x = sc[i][e] * a.c_log2;
+            float x = (sc[n][e] + (NR == 1 ? x1[n][e] + x2[0][e] : x1[n][e])) * a.c_log2;
             if (TAIL) {
-                const int j = key0 + row0 + 8 * i + key_perm(2 * t + (e & 1)) - s.len;   // < 0: a cached row
-                if (j >= 0 && (j >= s.n || !tree_sees(a, b, e < 2 ? tok_a : tok_b, j))) x = -INFINITY;
+                const int j = key0 + krow + 8 * (e >> 1) - s.len;   // < 0: a cached row
+                if (j >= 0 && (j >= s.n || !tree_sees(a, b, toks[8 * n + 2 * t + (e & 1)], j))) x = -INFINITY;
             }
-            sc[i][e] = x;
-            mx[e >> 1] = fmaxf(mx[e >> 1], x);
+            sc[n][e] = x;
+            mx[e & 1] = fmaxf(mx[e & 1], x);
         }
-    float corr[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        const float m_new = fmaxf(w.m[r], mx[r]);
-        const float base = m_new == -INFINITY ? 0.f : m_new;   // nothing seen so far: every p below is 2^-inf = 0
-        corr[r] = ex2_approx(w.m[r] - base);
-        w.m[r] = m_new;
-        float sum = 0.f;
+        for (int r = 0; r < 2; ++r) {
 #pragma unroll
-        for (int i = 0; i < C::NT; ++i)
+            for (int o = 4; o < 32; o <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], o));
+            const float m_new = fmaxf(w.m[n][r], mx[r]);
+            const float base = m_new == -INFINITY ? 0.f : m_new;   // nothing seen so far: every p below is 2^-inf = 0
+            corr[n][r] = ex2_approx(w.m[n][r] - base);
+            w.m[n][r] = m_new;
+            sc[n][r] = ex2_approx(sc[n][r] - base);
+            sc[n][2 + r] = ex2_approx(sc[n][2 + r] - base);
+            w.l[n][r] = fmaf(w.l[n][r], corr[n][r], sc[n][r] + sc[n][2 + r]);
+        }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float p = ex2_approx(sc[i][2 * r + e] - base);
-                sc[i][2 * r + e] = p;
-                sum += p;
-            }
-        w.l[r] = w.l[r] * corr[r] + sum;
+        for (int e = 0; e < 4; ++e) {   // key 2t, 2t+1 of the first eight, then of the second
+            const int src = e & 1 ? from1 : from;
+            const float even = __shfl_sync(0xffffffffu, sc[n][e & 2], src), oddv = __shfl_sync(0xffffffffu, sc[n][(e & 2) + 1], src);
+            const float p = g & 1 ? oddv : even;
+            phi[n][e] = __float_as_uint(p);
+            plo[n][e] = tf32_lo(p);
+        }
     }
     if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(v_full, v_parity))) ok = false;
     if (!ok) return;
-    // O = O * corr + P.V, the tile's product from zero
+    // O^T = O^T * corr + V^T.P^T
     bool odd = false;   // a value behind the cached rows that is not finite
 #pragma unroll
     for (int sl = 0; sl < DKP / 32; ++sl) {
-        float acc[4][4];
+        float acc[2][NR][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < C::NT; ++i) {
-            const int ra = row0 + 8 * i + key_perm(2 * t), rb = row0 + 8 * i + key_perm(2 * t + 1);
+            for (int n = 0; n < NR; ++n) acc[h][n][0] = acc[h][n][1] = acc[h][n][2] = acc[h][n][3] = 0.f;
+#pragma unroll
+        for (int k8 = 0; k8 < 2; ++k8) {
+            const int ra = row0 + 8 * k8 + 2 * t, rb = ra + 1;
             float4 va = lds128(vbase + tile_at(ra, sl, g)), vb = lds128(vbase + tile_at(rb, sl, g));
             if (TAIL) {
                 // rows behind the last one hold anything, and rows that only some tokens see must not reach the others
@@ -257,84 +289,139 @@ __device__ __forceinline__ void tree_tile(const KvTreeArgs &a, TreeWarp<DKP, MT>
                     if (jb >= 0 && !(jb < s.n && finite_f(y[e]))) { odd = odd || jb < s.n; y[e] = 0.f; }
                 }
             }
-            const uint32_t phi[4] = { __float_as_uint(sc[i][0]), __float_as_uint(sc[i][2]), __float_as_uint(sc[i][1]), __float_as_uint(sc[i][3]) };
-            const uint32_t plo[4] = { tf32_rest(sc[i][0]), tf32_rest(sc[i][2]), tf32_rest(sc[i][1]), tf32_rest(sc[i][3]) };
-            const float *x = &va.x, *y = &vb.x;
+            // rows g: columns 4g and 4g + 2; rows g+8: 4g + 1 and 4g + 3
+            const float vx[2][4] = { { va.x, va.y, vb.x, vb.y }, { va.z, va.w, vb.z, vb.w } };
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t h0 = __float_as_uint(x[e]), h1 = __float_as_uint(y[e]);
-                mma_tf32(acc[e], plo, h0, h1);
-                mma_tf32(acc[e], phi, tf32_rest(x[e]), tf32_rest(y[e]));
-                mma_tf32(acc[e], phi, h0, h1);
+            for (int h = 0; h < 2; ++h) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    hi[e] = __float_as_uint(vx[h][e]);
+                    lo[e] = tf32_lo(vx[h][e]);
+                }
+#pragma unroll
+                for (int n = 0; n < NR; ++n) mma_tf32(acc[h][n], lo, phi[n][2 * k8], phi[n][2 * k8 + 1]);
+#pragma unroll
+                for (int n = 0; n < NR; ++n) mma_tf32(acc[h][n], hi, plo[n][2 * k8], plo[n][2 * k8 + 1]);
+#pragma unroll
+                for (int n = 0; n < NR; ++n) mma_tf32(acc[h][n], hi, phi[n][2 * k8], phi[n][2 * k8 + 1]);
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            w.o[sl][e][0] = fmaf(w.o[sl][e][0], corr[0], acc[e][0]);
-            w.o[sl][e][1] = fmaf(w.o[sl][e][1], corr[0], acc[e][1]);
-            w.o[sl][e][2] = fmaf(w.o[sl][e][2], corr[1], acc[e][2]);
-            w.o[sl][e][3] = fmaf(w.o[sl][e][3], corr[1], acc[e][3]);
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.o[2 * sl + h][n][e] = fmaf(w.o[2 * sl + h][n][e], corr[n][e & 1], acc[h][n][e]);
     }
     if (TAIL && __any_sync(0xffffffffu, odd)) {
         // rare: an infinity or a NaN among the new rows' values goes to the rows that see it, and to no others
 #pragma unroll 1
-        for (int key = 0; key < C::KEYS_WARP; ++key) {
+        for (int key = 0; key < 16; ++key) {
             const int j = key0 + row0 + key - s.len;
             if (j < 0 || j >= s.n) continue;
-            const bool see_a = tree_sees(a, b, tok_a, j), see_b = tree_sees(a, b, tok_b, j);
 #pragma unroll
-            for (int sl = 0; sl < DKP / 32; ++sl)
+            for (int sl = 0; sl < DKP / 32; ++sl) {
+                const float4 v4 = lds128(vbase + tile_at(row0 + key, sl, g));
+                const float *x = &v4.x;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float4 v4 = lds128(vbase + tile_at(row0 + key, sl, 2 * t + h));
-                    const float *x = &v4.x;
+                for (int e = 0; e < 4; ++e)
+                    if (!finite_f(x[e]))
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!finite_f(x[e])) {
-                            if (see_a) w.o[sl][e][h] += x[e];
-                            if (see_b) w.o[sl][e][2 + h] += x[e];
-                        }
-                }
+                        for (int n = 0; n < NR; ++n)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+                                if (tree_sees(a, b, toks[8 * n + 2 * t + r], j)) w.o[2 * sl + (e >> 1)][n][2 * (e & 1) + r] += x[e];
+            }
         }
     }
 }
 
-// slot of the workspace: [rows][DKP] outputs, then [rows] maxima and [rows] sums
-template <int DKP, int MT>
-__device__ __forceinline__ float *tree_slot(const KvTreeArgs &a, int slot)
+// (m, l, o) of a warp plus another part of the same rows
+template <int DKP, int NR>
+__device__ __forceinline__ void tree_add(TreeWarp<DKP, NR> &w, const float4 *frag, const float4 *ml, int stride)
 {
-    return a.slots + (size_t)slot * (MT * 16) * (DKP + 2);
+    float f0[NR][2], f1[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const float4 v = ml[n * stride];   // maxima of the two rows, then sums
+        const float m2[2] = { v.x, v.y }, l2[2] = { v.z, v.w };
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float m_new = fmaxf(w.m[n][r], m2[r]), base = m_new == -INFINITY ? 0.f : m_new;
+            f0[n][r] = ex2_approx(w.m[n][r] - base);
+            f1[n][r] = ex2_approx(m2[r] - base);
+            w.m[n][r] = m_new;
+            w.l[n][r] = w.l[n][r] * f0[n][r] + l2[r] * f1[n][r];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < DKP / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const float4 v = frag[(i * NR + n) * stride];
+            const float *x = &v.x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w.o[i][n][e] = w.o[i][n][e] * f0[n][e & 1] + x[e] * f1[n][e & 1];
+        }
 }
 
-template <int DKP, int MT>
-__global__ void __launch_bounds__(KT_THREADS, 1) kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ TreeMaps tm, int tma)
+template <int DKP, int NR>
+__device__ __forceinline__ void tree_put(const TreeWarp<DKP, NR> &w, float4 *frag, float4 *ml, int stride)
 {
-    using C = TreeCfg<DKP, MT>;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) ml[n * stride] = make_float4(w.m[n][0], w.m[n][1], w.l[n][0], w.l[n][1]);
+#pragma unroll
+    for (int i = 0; i < DKP / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) frag[(i * NR + n) * stride] = make_float4(w.o[i][n][0], w.o[i][n][1], w.o[i][n][2], w.o[i][n][3]);
+}
+
+// all parts of a row group into its part 0: halves, quarters, ...; every consumer warp takes part
+template <int DKP, int NR, int RG>
+__device__ __forceinline__ void tree_merge(TreeWarp<DKP, NR> &w, float4 *area, int rg, int part)
+{
+    using C = TreeCfg<DKP, NR, RG>;
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int half = C::PARTS / 2; half >= 1; half >>= 1) {
+        float4 *frag = area + (size_t)(rg * (C::PARTS / 2) + (part >= half ? part - half : part)) * 32 * (C::FRAGS + NR) + lane;
+        if (part >= half && part < 2 * half) tree_put<DKP, NR>(w, frag, frag + C::FRAGS * 32, 32);
+        consumers_sync();
+        if (part < half) tree_add<DKP, NR>(w, frag, frag + C::FRAGS * 32, 32);
+        consumers_sync();
+    }
+}
+
+template <int DKP, int NR, int RG>
+__global__ void __launch_bounds__(TreeCfg<DKP, NR, RG>::THREADS, 1)
+kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ TreeMaps tm, int tma)
+{
+    using C = TreeCfg<DKP, NR, RG>;
+    constexpr int ROWS = C::ROWS;
     extern __shared__ uint8_t smem_raw[];
     __shared__ alignas(8) uint64_t bars[4 * C::STAGES];
     __shared__ unsigned long long s_total;
-    __shared__ int s_b, s_last;
+    __shared__ int s_b, s_last, s_tok[ROWS];
     __shared__ long long s_off;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t *const tiles = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);   // the swizzle is a function of the address
-    float *merge = reinterpret_cast<float *>(tiles + C::STAGES * 2 * C::TILE);
+    float4 *const area = reinterpret_cast<float4 *>(tiles + C::STAGES * 2 * C::TILE);
     const uint32_t bar0 = smem_u32(bars);
     auto bar = [&](int kind, int stage) { return bar0 + 8u * (kind * C::STAGES + stage); };   // 0 K full, 1 K empty, 2 V full, 3 V empty
     auto ktile = [&](int stage) { return tiles + stage * 2 * C::TILE; };
     if (tid == 0) {
         s_total = 0;
         for (int s = 0; s < C::STAGES; ++s)
-            for (int k = 0; k < 4; ++k) mbar_init(bar(k, s), k & 1 ? MT * C::SLICES : (tma ? 1 : 32));
+            for (int k = 0; k < 4; ++k) mbar_init(bar(k, s), k & 1 ? RG * C::SLICES : (tma ? 1 : 32));
         mbar_fence_init();
     }
     __syncthreads();
 
     // the line of tiles, this CTA's part of it, and the sequence that part starts in
-    constexpr int ROWS = MT * 16;
     {
         unsigned long long sum = 0;
-        for (int b = tid; b < a.B; b += KT_THREADS) {
+        for (int b = tid; b < a.B; b += C::THREADS) {
             bool bad;
             const TreeSeq s = tree_seq(a, b, ROWS, &bad);
             sum += (unsigned long long)tree_tiles(a, s);
@@ -376,14 +463,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tree_kernel(const __grid_con
     bool ok = true;
     uint32_t it = 0;   // tiles since the start: ring stage it % STAGES, phase it / STAGES
 
-    if (warp == KT_CONSUMERS) {
+    if (warp >= KT_CONSUMERS) {
         // ---- producer
+        if (C::SHIFT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+        if (warp > KT_CONSUMERS) return;
         while (ok && next_piece(a, cur, ROWS, p)) {
             const int head = p.b * a.Hkv + p.hk;
             for (int i = 0; ok && i < p.count; ++i, ++it) {
                 const int s = it % C::STAGES, row = (p.t0 + i) * KT_KEYS;
                 const uint32_t ph = (it / C::STAGES) & 1;
-#pragma unroll
+#pragma unroll 1
                 for (int v = 0; v < 2; ++v) {
                     if (it >= C::STAGES && !__all_sync(0xffffffffu, mbar_wait_bounded(bar(2 * v + 1, s), ph ^ 1))) { ok = false; break; }
                     const uint32_t full = bar(2 * v, s), dst = smem_u32(ktile(s)) + v * C::TILE;
@@ -396,15 +485,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tree_kernel(const __grid_con
                     } else {
                         // tensors that a tensor map cannot describe: the same layout, four bytes at a time
                         const float *src = (v ? a.V : a.K) + (int64_t)head * a.max_seq * a.dk;
+#pragma unroll 1
                         for (int r = 0; r < KT_KEYS; ++r) {
                             const bool in = (int64_t)row + r < a.max_seq;
-#pragma unroll
+#pragma unroll 1
                             for (int sl = 0; sl < DKP / 32; ++sl) {
                                 const int c = 32 * sl + lane;
                                 const bool get = in && c < a.dk;
-                                const float *from = get ? src + ((int64_t)row + r) * a.dk + c : src;
+                                const float *get_from = get ? src + ((int64_t)row + r) * a.dk + c : src;
                                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + tile_at(r, sl, lane >> 2) + 4 * (lane & 3)),
-                                             "l"(from), "r"(get ? 4 : 0)
+                                             "l"(get_from), "r"(get ? 4 : 0)
                                              : "memory");
                             }
                         }
@@ -423,22 +513,30 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tree_kernel(const __grid_con
     }
 
     // ---- consumers
-    const int g = lane >> 2, t = lane & 3, rt = warp % MT, part = warp / MT, grp = part / C::SLICES;
+    if (C::SHIFT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
+    const int g = lane >> 2, t = lane & 3, rg = warp % RG, part = warp / RG, grp = part / C::SLICES, row0 = part % C::SLICES * 16;
     const int heads_per = a.H / a.Hkv;
-    TreeWarp<DKP, MT> w;
+    TreeWarp<DKP, NR> w;
+    auto clear = [&] {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            w.m[n][0] = w.m[n][1] = -INFINITY;
+            w.l[n][0] = w.l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < DKP / 16; ++i) w.o[i][n][0] = w.o[i][n][1] = w.o[i][n][2] = w.o[i][n][3] = 0.f;
+        }
+    };
     while (next_piece(a, cur, ROWS, p)) {
-        const int r0 = p.block * ROWS + rt * 16;
-        // query row r: head r / n of the group, token r % n
-        const int ra = r0 + g, rb = r0 + g + 8;
-        const int ga = ra / p.s.n, gb = rb / p.s.n, tok_a = ra < p.s.rows ? ra - ga * p.s.n : 0, tok_b = rb < p.s.rows ? rb - gb * p.s.n : 0;
-        const bool idle = r0 >= p.s.rows;
-        // the rows' Q as the lanes will read it, in the merge area: [row tile][16-column group][rows g | g + 8][lane]
+        // query row r: head r / n of the group, token r % n.  Q as the lanes will read it, in the merge area:
+        // [eight rows][16-column group][(hi, lo)][lane]
         for (int i = tid; i < ROWS * (DKP / 4); i += KT_CONSUMERS * 32) {
             const int r = i / (DKP / 4), c = i - r * (DKP / 4), row = p.block * ROWS + r;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            int tok = 0;
             if (row < p.s.rows) {
                 const int gh = row / p.s.n;
-                const float *src = a.Q + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + (row - gh * p.s.n)) * a.dk + 4 * c;
+                tok = row - gh * p.s.n;
+                const float *src = a.Q + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk + 4 * c;
                 if (tma) {   // rows are whole 16-byte pieces
                     if (4 * c < a.dk) x = __ldg(reinterpret_cast<const float4 *>(src));
                 } else {
@@ -448,15 +546,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tree_kernel(const __grid_con
                     if (4 * c + 3 < a.dk) x.w = __ldg(src + 3);
                 }
             }
-            reinterpret_cast<float4 *>(merge)[((r >> 4) * (DKP / 16) + (c >> 2)) * 64 + ((r >> 3) & 1) * 32 + (r & 7) * 4 + (c & 3)] = x;
+            if (c == 0) s_tok[r] = tok;
+            const int at = ((r >> 3) * (DKP / 16) + (c >> 2)) * (C::SPLIT_Q ? 64 : 32) + (r & 7) * 4 + (c & 3);
+            area[at] = x;
+            if (C::SPLIT_Q)
+                area[at + 32] = make_float4(__uint_as_float(tf32_lo(x.x)), __uint_as_float(tf32_lo(x.y)), __uint_as_float(tf32_lo(x.z)), __uint_as_float(tf32_lo(x.w)));
         }
-        const uint8_t *qbase = reinterpret_cast<const uint8_t *>(merge) + rt * (DKP / 16) * 1024 + lane * 16;
-        w.m[0] = w.m[1] = -INFINITY;
-        w.l[0] = w.l[1] = 0.f;
-#pragma unroll
-        for (int sl = 0; sl < DKP / 32; ++sl)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w.o[sl][e][0] = w.o[sl][e][1] = w.o[sl][e][2] = w.o[sl][e][3] = 0.f;
+        const uint8_t *qbase = reinterpret_cast<const uint8_t *>(area) + rg * NR * (DKP / 16) * (C::SPLIT_Q ? 1024 : 512) + lane * 16;
+        const int *toks = s_tok + rg * 8 * NR;
+        const bool idle = p.block * ROWS + rg * 8 * NR >= p.s.rows;
+        clear();
         consumers_sync();
 
         for (int i = 0; i < p.count; ++i, ++it) {
@@ -465,115 +564,85 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tree_kernel(const __grid_con
             const uint32_t ph = (it / C::STAGES) & 1;
             const int key0 = (p.t0 + i) * KT_KEYS;
             if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(bar(0, s), ph))) ok = false;
-            if (ok && !idle) {
-                // (the last column of a 32-bit key index: key0 <= max_seq < 2^31)
-                if (key0 + KT_KEYS > p.s.len)
-                    tree_tile<DKP, MT, true>(a, w, qbase, ktile(s), ktile(s) + C::TILE, key0, p.s, p.b, tok_a, tok_b, bar(2, s), ph, ok);
+            const bool work = ok && !idle;
+            if (work) {
+                const uint8_t *kt = ktile(s);
+                if (key0 + row0 + 16 > p.s.len)
+                    tree_tile<DKP, NR, RG, true>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, toks, bar(1, s), bar(2, s), ph, ok);
                 else
-                    tree_tile<DKP, MT, false>(a, w, qbase, ktile(s), ktile(s) + C::TILE, key0, p.s, p.b, tok_a, tok_b, bar(2, s), ph, ok);
+                    tree_tile<DKP, NR, RG, false>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, toks, bar(1, s), bar(2, s), ph, ok);
             } else if (ok) {
                 if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar(2, s), ph))) ok = false;
             }
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(bar(1, s));
+                if (!work) mbar_arrive(bar(1, s));
                 mbar_arrive(bar(3, s));
             }
         }
-
+        // the lanes' sums become the rows'
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) w.l[n][r] += __shfl_xor_sync(0xffffffffu, w.l[n][r], o);
         consumers_sync();   // Q has been read
-        // ---- merge the warps' parts: [part][row][DKP + 4] outputs, then [part][row] maxima and sums
-        float *mo = merge, *mm = merge + C::PARTS * ROWS * (DKP + 4), *ml = mm + C::PARTS * ROWS;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float sum = w.l[h];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const int row = part * ROWS + rt * 16 + g + 8 * h;
-            if (t == 0) {
-                mm[row] = w.m[h];
-                ml[row] = sum;
+        tree_merge<DKP, NR, RG>(w, area, rg, part);
+
+        bool write = p.count == p.s.tiles;
+        if (!write) {
+            // the item's pieces belong to consecutive CTAs; the first one's index names its counter.  Slots: [row group][lane order]
+            const int first = (int)(p.item_pos / per), pieces = (int)((p.item_pos + p.s.tiles - 1) / per) - first + 1;
+            constexpr int GROUP_F4 = 32 * (C::FRAGS + NR);
+            auto slot = [&](int k) { return reinterpret_cast<float4 *>(a.slots) + (size_t)k * (RG * GROUP_F4) + rg * GROUP_F4 + lane; };
+            if (part == 0) {
+                float4 *f = slot(2 * (int)blockIdx.x + (p.t0 == 0 ? 1 : 0));
+                tree_put<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
+                __threadfence();
             }
-#pragma unroll
-            for (int sl = 0; sl < DKP / 32; ++sl)
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    *reinterpret_cast<float4 *>(mo + row * (DKP + 4) + 32 * sl + 8 * t + 4 * c) =
-                        make_float4(w.o[sl][0][2 * h + c], w.o[sl][1][2 * h + c], w.o[sl][2][2 * h + c], w.o[sl][3][2 * h + c]);
-        }
-        consumers_sync();
-        const int rows_here = p.s.rows - p.block * ROWS < ROWS ? p.s.rows - p.block * ROWS : ROWS;
-        const bool whole = p.count == p.s.tiles;
-        // the item's pieces belong to consecutive CTAs; the first one's index names its counter
-        const int first = (int)(p.item_pos / per), pieces = (int)((p.item_pos + p.s.tiles - 1) / per) - first + 1;
-        float *slot = tree_slot<DKP, MT>(a, 2 * (int)blockIdx.x + (p.t0 == 0 ? 1 : 0));
-        auto store_out = [&](int r, int c, float4 y) {
-            const int row = p.block * ROWS + r, gh = row / p.s.n, tok = row - gh * p.s.n;
-            float *dst = a.out + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk + c;
-            if (tma) {
-                *reinterpret_cast<float4 *>(dst) = y;
-            } else {
-                const float *v = &y.x;
-                for (int e = 0; e < 4; ++e)
-                    if (c + e < a.dk) dst[e] = v[e];
-            }
-        };
-        for (int i = tid; i < rows_here * (DKP / 4); i += KT_CONSUMERS * 32) {
-            const int r = i / (DKP / 4), c = (i - r * (DKP / 4)) * 4;
-            float M = -INFINITY, L = 0.f;
-#pragma unroll
-            for (int k = 0; k < C::PARTS; ++k) M = fmaxf(M, mm[k * ROWS + r]);
-            const float base = M == -INFINITY ? 0.f : M;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < C::PARTS; ++k) {
-                const float f = ex2_approx(mm[k * ROWS + r] - base);
-                const float4 v = *reinterpret_cast<const float4 *>(mo + (k * ROWS + r) * (DKP + 4) + c);
-                L = fmaf(f, ml[k * ROWS + r], L);
-                y.x = fmaf(f, v.x, y.x); y.y = fmaf(f, v.y, y.y); y.z = fmaf(f, v.z, y.z); y.w = fmaf(f, v.w, y.w);
-            }
-            if (whole) {
-                if (c >= a.dk) continue;
-                const float inv = L == 0.f ? 0.f : 1.0f / L;   // nothing seen: 0
-                store_out(r, c, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
-            } else {
-                *reinterpret_cast<float4 *>(slot + r * DKP + c) = y;
-                if (c == 0) {
-                    slot[ROWS * DKP + r] = M;
-                    slot[ROWS * DKP + ROWS + r] = L;
-                }
-            }
-        }
-        if (!whole) {
-            __threadfence();
             consumers_sync();
             if (tid == 0) s_last = atomicAdd(a.counters + first, 1) == pieces - 1;
             consumers_sync();
-            if (s_last) {
+            write = s_last != 0;
+            if (write) {
                 __threadfence();
-                for (int i = tid; i < rows_here * (DKP / 4); i += KT_CONSUMERS * 32) {
-                    const int r = i / (DKP / 4), c = (i - r * (DKP / 4)) * 4;
-                    if (c >= a.dk) continue;
-                    float M = -INFINITY, L = 0.f;
-                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int k = 0; k < pieces; ++k) {
-                        const float *src = tree_slot<DKP, MT>(a, 2 * (first + k) + (k == 0 ? 1 : 0));
-                        const float mk = __ldcg(src + ROWS * DKP + r), lk = __ldcg(src + ROWS * DKP + ROWS + r);
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + r * DKP + c));
-                        const float m_new = fmaxf(M, mk), base = m_new == -INFINITY ? 0.f : m_new;
-                        const float f0 = ex2_approx(M - base), f1 = ex2_approx(mk - base);
-                        M = m_new;
-                        L = L * f0 + lk * f1;
-                        y.x = y.x * f0 + v.x * f1; y.y = y.y * f0 + v.y * f1; y.z = y.z * f0 + v.z * f1; y.w = y.w * f0 + v.w * f1;
-                    }
-                    const float inv = L == 0.f ? 0.f : 1.0f / L;
-                    store_out(r, c, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+                clear();
+#pragma unroll 1
+                for (int k = part; k < pieces; k += C::PARTS) {
+                    const float4 *f = slot(2 * (first + k) + (k == 0 ? 1 : 0));
+                    tree_add<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
                 }
+                tree_merge<DKP, NR, RG>(w, area, rg, part);
                 if (tid == 0) a.counters[first] = 0;
             }
         }
-        consumers_sync();   // the merge area is free again
+        if (write && part == 0) {
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = p.block * ROWS + (rg * NR + n) * 8 + 2 * t + r;
+                    if (row >= p.s.rows) continue;
+                    const int gh = row / p.s.n, tok = row - gh * p.s.n;
+                    float *dst = a.out + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk;
+                    const float inv = w.l[n][r] == 0.f ? 0.f : 1.0f / w.l[n][r];   // nothing seen: 0
+#pragma unroll
+                    for (int sl = 0; sl < DKP / 32; ++sl) {
+                        const int c = 32 * sl + 4 * g;
+                        const float4 y = make_float4(w.o[2 * sl][n][r] * inv, w.o[2 * sl][n][2 + r] * inv, w.o[2 * sl + 1][n][r] * inv,
+                                                     w.o[2 * sl + 1][n][2 + r] * inv);
+                        if (tma) {
+                            if (c < a.dk) *reinterpret_cast<float4 *>(dst + c) = y;
+                        } else {
+                            const float *v = &y.x;
+                            for (int e = 0; e < 4; ++e)
+                                if (c + e < a.dk) dst[c + e] = v[e];
+                        }
+                    }
+                }
+        }
+        consumers_sync();   // the merge area and s_tok are free again
     }
     if (!ok && lane == 0 && a.err) atomicCAS(a.err, 0, (int)TERR_CONSUMER);
 }
@@ -636,31 +705,31 @@ static inline bool kt_aligned16(const void *p) { return (reinterpret_cast<uintpt
 
 size_t kv_tree_workspace_bytes(int sm_count)
 {
-    return (size_t)sm_count * 2 * KT_MAX_ROWS * (128 + 2) * sizeof(float);
+    return (size_t)sm_count * 2 * KT_SLOT_BYTES;
 }
 
-template <int DKP, int MT>
+template <int DKP, int NR, int RG>
 static int launch_tree(const KvTreeArgs &a, const TreeMaps &tm, int tma, int sm_count, cudaStream_t st)
 {
-    using C = TreeCfg<DKP, MT>;
-    static_assert(C::STAGES >= 2 && C::SMEM <= 227 * 1024, "shared memory");
-    static_assert(MT * 16 <= KT_MAX_ROWS && DKP <= 128, "workspace slots");
+    using C = TreeCfg<DKP, NR, RG>;
+    static_assert(C::STAGES >= 2 && C::SMEM <= 227 * 1024 - 2048, "shared memory");
+    static_assert((size_t)RG * 32 * (C::FRAGS + NR) * 16 <= KT_SLOT_BYTES, "workspace slots");
     static PerDeviceOnce once;
     if (once.first()) {
-        cudaError_t e = cudaFuncSetAttribute(kv_tree_kernel<DKP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(kv_tree_kernel<DKP, NR, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return (int)e;
     }
-    kv_tree_kernel<DKP, MT><<<sm_count, KT_THREADS, C::SMEM, st>>>(a, tm, tma);
+    kv_tree_kernel<DKP, NR, RG><<<sm_count, C::THREADS, C::SMEM, st>>>(a, tm, tma);
     return (int)cudaGetLastError();
 }
 
-template <int MT>
-static int launch_tree_mt(const KvTreeArgs &a, const TreeMaps &tm, int tma, int sm_count, cudaStream_t st)
+template <int NR, int RG>
+static int launch_tree_rows(const KvTreeArgs &a, const TreeMaps &tm, int tma, int sm_count, cudaStream_t st)
 {
-    if (a.dk <= 32) return launch_tree<32, MT>(a, tm, tma, sm_count, st);
-    if (a.dk <= 64) return launch_tree<64, MT>(a, tm, tma, sm_count, st);
-    if (a.dk <= 96) return launch_tree<96, MT>(a, tm, tma, sm_count, st);
-    return launch_tree<128, MT>(a, tm, tma, sm_count, st);
+    if (a.dk <= 32) return launch_tree<32, NR, RG>(a, tm, tma, sm_count, st);
+    if (a.dk <= 64) return launch_tree<64, NR, RG>(a, tm, tma, sm_count, st);
+    if (a.dk <= 96) return launch_tree<96, NR, RG>(a, tm, tma, sm_count, st);
+    return launch_tree<128, NR, RG>(a, tm, tma, sm_count, st);
 }
 
 int launch_kv_cache_attend_tree(const KvTreeArgs &a, int sm_count, cudaStream_t st)
@@ -673,9 +742,10 @@ int launch_kv_cache_attend_tree(const KvTreeArgs &a, int sm_count, cudaStream_t 
         if (e) return e;
     }
     const int64_t rows = (int64_t)(a.H / a.Hkv) * a.T;   // of a key head, if every token is there
-    if (rows <= 16) return launch_tree_mt<1>(a, tm, tma, sm_count, st);
-    if (rows <= 32) return launch_tree_mt<2>(a, tm, tma, sm_count, st);
-    return launch_tree_mt<4>(a, tm, tma, sm_count, st);
+    if (rows <= 8) return launch_tree_rows<1, 1>(a, tm, tma, sm_count, st);
+    if (rows <= 16) return launch_tree_rows<2, 1>(a, tm, tma, sm_count, st);
+    if (rows <= 32) return launch_tree_rows<4, 1>(a, tm, tma, sm_count, st);
+    return launch_tree_rows<4, 2>(a, tm, tma, sm_count, st);
 }
 
 int launch_kv_cache_compact(float *K, float *V, const int32_t *keep, const int32_t *n_keep, const int32_t *lens, int32_t *lens_out,
