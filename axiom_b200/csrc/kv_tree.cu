@@ -26,7 +26,7 @@
 // arrives last at the item's counter adds the pieces in line order (nobody waits; the result does not depend on who was
 // last) and clears the counter.
 //
-// One CTA per SM: a producer warp feeds K and V tiles through a ring; eight warps each take 16 keys of a tile with
+// One CTA per SM: two producer warps feed K and V tiles through a ring; eight warps each take 16 keys of a tile with
 // a running softmax of their own, merged in registers through shared memory at the end of a piece.
 #include "kv_tree.cuh"
 
@@ -61,10 +61,10 @@ struct TreeCfg {
     static constexpr int ROOM = (224 * 1024 - AREA) / (2 * TILE);
     static constexpr int STAGES = ROOM < 8 ? ROOM : 8;
     static constexpr int SMEM = 1024 + STAGES * 2 * TILE + AREA;
-    // four rows in eights and 128 columns need more than the 168 registers that nine warps leave a thread: with twelve
+    // four rows in eights and 128 columns need more than the 168 registers that ten warps leave a thread: with twelve
     // warps the producer's four hand theirs to the consumers
     static constexpr bool SHIFT_REGS = NR == 4 || (NR == 2 && DKP == 128);
-    static constexpr int THREADS = (KT_CONSUMERS + (SHIFT_REGS ? 4 : 1)) * 32;
+    static constexpr int THREADS = (KT_CONSUMERS + (SHIFT_REGS ? 4 : 2)) * 32;
 };
 
 struct TreeMaps {
@@ -400,20 +400,25 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
     using C = TreeCfg<DKP, NR, RG>;
     constexpr int ROWS = C::ROWS;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ alignas(8) uint64_t bars[4 * C::STAGES];
+    __shared__ alignas(8) uint64_t bars[6 * C::STAGES];
     __shared__ unsigned long long s_total;
     __shared__ int s_b, s_last, s_tok[ROWS];
+    __shared__ volatile int s_gave_up;   // a consumer's wait ran out: its arrivals no longer mean free stages
     __shared__ long long s_off;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t *const tiles = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);   // the swizzle is a function of the address
     float4 *const area = reinterpret_cast<float4 *>(tiles + C::STAGES * 2 * C::TILE);
     const uint32_t bar0 = smem_u32(bars);
-    auto bar = [&](int kind, int stage) { return bar0 + 8u * (kind * C::STAGES + stage); };   // 0 K full, 1 K empty, 2 V full, 3 V empty
+    // Barriers of a stage: K empty, V empty, and two "full" ones each for K and V, which its uses take in turn.  Successive uses
+    // of a stage may belong to different groups of warps, and loads may land out of order: with one barrier a group could
+    // ask for use u while use u - 1 is still in flight and take the completion of use u - 2, which has the parity it waits for.
+    auto empty_bar = [&](int v, int stage) { return bar0 + 8u * (v * C::STAGES + stage); };
+    auto full_bar = [&](int v, int stage, uint32_t use) { return bar0 + 8u * ((2 + 2 * v + (use & 1)) * C::STAGES + stage); };
     auto ktile = [&](int stage) { return tiles + stage * 2 * C::TILE; };
     if (tid == 0) {
         s_total = 0;
-        for (int s = 0; s < C::STAGES; ++s)
-            for (int k = 0; k < 4; ++k) mbar_init(bar(k, s), k & 1 ? RG * C::SLICES : (tma ? 1 : 32));
+        s_gave_up = 0;
+        for (int i = 0; i < 6 * C::STAGES; ++i) mbar_init(bar0 + 8u * i, i < 2 * C::STAGES ? RG * C::SLICES : (tma ? 1 : 32));
         mbar_fence_init();
     }
     __syncthreads();
@@ -461,53 +466,54 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
     cur.off = s_off;
     TreePiece p;
     bool ok = true;
-    uint32_t it = 0;   // tiles since the start: ring stage it % STAGES, phase it / STAGES
+    uint32_t it = 0;   // tiles since the start: ring stage it % STAGES, its use number it / STAGES
 
     if (warp >= KT_CONSUMERS) {
-        // ---- producer
+        // ---- producers: warp 8 the K tiles, warp 9 the V tiles (one issuing thread turns a 16 KB tile around in some 700
+        // cycles, which HBM's share of an SM would just about saturate)
         if (C::SHIFT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
-        if (warp > KT_CONSUMERS) return;
+        if (warp > KT_CONSUMERS + 1) return;
+        const int v = warp - KT_CONSUMERS;
+        const float *const cache = v ? a.V : a.K;
         while (ok && next_piece(a, cur, ROWS, p)) {
             const int head = p.b * a.Hkv + p.hk;
             for (int i = 0; ok && i < p.count; ++i, ++it) {
                 const int s = it % C::STAGES, row = (p.t0 + i) * KT_KEYS;
-                const uint32_t ph = (it / C::STAGES) & 1;
-#pragma unroll 1
-                for (int v = 0; v < 2; ++v) {
-                    if (it >= C::STAGES && !__all_sync(0xffffffffu, mbar_wait_bounded(bar(2 * v + 1, s), ph ^ 1))) { ok = false; break; }
-                    const uint32_t full = bar(2 * v, s), dst = smem_u32(ktile(s)) + v * C::TILE;
-                    if (tma) {
-                        if (lane == 0) {
-                            mbar_arrive_expect_tx(full, C::TILE);
+                const uint32_t use = it / C::STAGES;
+                if (use && !__all_sync(0xffffffffu, mbar_wait_bounded(empty_bar(v, s), (use - 1) & 1))) { ok = false; break; }
+                if (s_gave_up) { ok = false; break; }
+                const uint32_t full = full_bar(v, s, use), dst = smem_u32(ktile(s)) + v * C::TILE;
+                if (tma) {
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(full, C::TILE);
 #pragma unroll
-                            for (int sl = 0; sl < DKP / 32; ++sl) tma_load_3d(dst + sl * (KT_KEYS * 128), v ? &tm.v : &tm.k, full, 32 * sl, row, head);
-                        }
-                    } else {
-                        // tensors that a tensor map cannot describe: the same layout, four bytes at a time
-                        const float *src = (v ? a.V : a.K) + (int64_t)head * a.max_seq * a.dk;
-#pragma unroll 1
-                        for (int r = 0; r < KT_KEYS; ++r) {
-                            const bool in = (int64_t)row + r < a.max_seq;
-#pragma unroll 1
-                            for (int sl = 0; sl < DKP / 32; ++sl) {
-                                const int c = 32 * sl + lane;
-                                const bool get = in && c < a.dk;
-                                const float *get_from = get ? src + ((int64_t)row + r) * a.dk + c : src;
-                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + tile_at(r, sl, lane >> 2) + 4 * (lane & 3)),
-                                             "l"(get_from), "r"(get ? 4 : 0)
-                                             : "memory");
-                            }
-                        }
-                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full) : "memory");
+                        for (int sl = 0; sl < DKP / 32; ++sl) tma_load_3d(dst + sl * (KT_KEYS * 128), v ? &tm.v : &tm.k, full, 32 * sl, row, head);
                     }
+                } else {
+                    // tensors that a tensor map cannot describe: the same layout, four bytes at a time
+                    const float *src = cache + (int64_t)head * a.max_seq * a.dk;
+#pragma unroll 1
+                    for (int r = 0; r < KT_KEYS; ++r) {
+                        const bool in = (int64_t)row + r < a.max_seq;
+#pragma unroll 1
+                        for (int sl = 0; sl < DKP / 32; ++sl) {
+                            const int c = 32 * sl + lane;
+                            const bool get = in && c < a.dk;
+                            const float *get_from = get ? src + ((int64_t)row + r) * a.dk + c : src;
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + tile_at(r, sl, lane >> 2) + 4 * (lane & 3)),
+                                         "l"(get_from), "r"(get ? 4 : 0)
+                                         : "memory");
+                        }
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full) : "memory");
                 }
             }
         }
         if (!ok) {
             if (lane == 0 && a.err) atomicCAS(a.err, 0, (int)TERR_PRODUCER);
             // copies in flight land before the CTA's memory goes away
-            for (int s = 0; s < C::STAGES; ++s)
-                for (int k = 0; k <= 2; k += 2) mbar_wait_bounded(bar(k, s), ((it >= (uint32_t)s ? it - s : 0) / C::STAGES) & 1);
+            for (uint32_t i = it > C::STAGES ? it - C::STAGES : 0; i < it; ++i)
+                mbar_wait_bounded(full_bar(v, i % C::STAGES, i / C::STAGES), (i / C::STAGES >> 1) & 1);
         }
         return;
     }
@@ -561,23 +567,27 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
         for (int i = 0; i < p.count; ++i, ++it) {
             if (C::GROUPS > 1 && (int)(it % C::GROUPS) != grp) continue;
             const int s = it % C::STAGES;
-            const uint32_t ph = (it / C::STAGES) & 1;
+            const uint32_t use = it / C::STAGES, ph = (use >> 1) & 1;
             const int key0 = (p.t0 + i) * KT_KEYS;
-            if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(bar(0, s), ph))) ok = false;
+            if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(full_bar(0, s, use), ph))) ok = false;
             const bool work = ok && !idle;
             if (work) {
                 const uint8_t *kt = ktile(s);
                 if (key0 + row0 + 16 > p.s.len)
-                    tree_tile<DKP, NR, RG, true>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, toks, bar(1, s), bar(2, s), ph, ok);
+                    tree_tile<DKP, NR, RG, true>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, toks, empty_bar(0, s), full_bar(1, s, use), ph, ok);
                 else
-                    tree_tile<DKP, NR, RG, false>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, toks, bar(1, s), bar(2, s), ph, ok);
+                    tree_tile<DKP, NR, RG, false>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, toks, empty_bar(0, s), full_bar(1, s, use), ph, ok);
             } else if (ok) {
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar(2, s), ph))) ok = false;
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(full_bar(1, s, use), ph))) ok = false;
+            }
+            if (!ok) {
+                s_gave_up = 1;
+                __threadfence_block();
             }
             __syncwarp();
             if (lane == 0) {
-                if (!work) mbar_arrive(bar(1, s));
-                mbar_arrive(bar(3, s));
+                if (!work) mbar_arrive(empty_bar(0, s));
+                mbar_arrive(empty_bar(1, s));
             }
         }
         // the lanes' sums become the rows'
