@@ -1410,7 +1410,7 @@ inline bool overlaps(const void *p, int64_t n, const void *q, int64_t m)   // n,
 
 // counters first (zero between calls), then room for either call's partial results
 constexpr size_t kAttnCounters = 4096;
-static_assert(sizeof(int) * 1024 <= kAttnCounters, "a counter per SM");
+static_assert(sizeof(int) * 3 * 256 <= kAttnCounters, "three counters per SM");
 
 size_t attn_workspace_bytes()
 {

@@ -21,7 +21,8 @@
 // into fp32 registers with the online-softmax factor in the same multiply-add.
 //
 // Work split: the tiles of 32 keys of all (sequence, key head, row block) items form one line, cut into equal pieces,
-// one per SM — lengths differ by orders of magnitude in a batch, and the device knows them, not the host.  A piece that
+// one per SM (kv_tree_line.cuh) — lengths differ by orders of magnitude in a batch, and the device knows them, not the
+// host.  A piece that
 // does not hold an item's whole line leaves (max, sum, unnormalised output) in its workspace slot; the CTA that
 // arrives last at the item's counter adds the pieces in line order (nobody waits; the result does not depend on who was
 // last) and clears the counter.
@@ -32,8 +33,8 @@
 
 #include "errors.cuh"
 #include "gemm_tc.cuh"
+#include "kv_tree_line.cuh"
 #include "ptx.cuh"
-#include "rope.cuh"
 
 #include <cuda.h>
 #include <math.h>
@@ -41,17 +42,14 @@
 namespace axb {
 
 static constexpr int KT_KEYS = 32, KT_CONSUMERS = 8;
-static constexpr size_t KT_SLOT_BYTES = 2 * 32 * 36 * 16;   // the largest variant's partial result
 enum { TERR_PRODUCER = 91, TERR_CONSUMER = 92 };
 
-// DKP: head dim rounded up to 32 (the tiles' columns beyond dk read as zero).  NR: query rows of a warp, in eights.
-// RG: groups of warps that share a tile's keys and differ in their query rows.
-template <int DKP, int NR, int RG>
+// DKP: head dim rounded up to 32 (the tiles' columns beyond dk read as zero).  NR: query rows of an item, in eights.
+template <int DKP, int NR>
 struct TreeCfg {
-    static constexpr int ROWS = 8 * NR * RG;                          // query rows of an item
+    static constexpr int ROWS = 8 * NR;                          // query rows of an item
     static constexpr int SLICES = KT_KEYS / 16;                       // warps side by side on a tile's keys
-    static constexpr int PARTS = KT_CONSUMERS / RG;                   // warps with the same query rows
-    static constexpr int GROUPS = PARTS / SLICES;                     // tiles in work at the same time
+    static constexpr int GROUPS = KT_CONSUMERS / SLICES;              // tiles in work at the same time
     static constexpr int FRAGS = DKP / 16 * NR;                       // float4 of a lane's O^T
     static constexpr bool SPLIT_Q = NR < 4;                           // Q lies in shared memory as hi and lo
     static constexpr int TILE = KT_KEYS * DKP * 4;                    // bytes of a K or V tile
@@ -70,65 +68,6 @@ struct TreeCfg {
 struct TreeMaps {
     CUtensorMap k, v;   // [B*Hkv][max_seq][dk], boxes of 32 columns x 32 rows
 };
-
-struct TreeSeq {
-    int len, n, rows, blocks, tiles;   // cached rows, new tokens, query rows of a key head, row blocks, key tiles
-};
-
-__device__ __forceinline__ TreeSeq tree_seq(const KvTreeArgs &a, int b, int block_rows, bool *bad = nullptr)
-{
-    TreeSeq s;
-    s.len = __ldg(a.lens + b);
-    s.n = a.n_new ? __ldg(a.n_new + b) : a.T;
-    const bool off = s.len < 0 || s.n < 0 || s.n > a.T || (int64_t)s.len + s.n > a.max_seq;
-    if (bad) *bad = off;
-    if (off) s.len = s.n = 0;   // refused whole: its output rows are left alone
-    s.rows = s.n * (a.H / a.Hkv);
-    s.blocks = (s.rows + block_rows - 1) / block_rows;
-    s.tiles = s.n ? (int)(((int64_t)s.len + s.n + KT_KEYS - 1) / KT_KEYS) : 0;
-    return s;
-}
-
-__device__ __forceinline__ int64_t tree_tiles(const KvTreeArgs &a, const TreeSeq &s) { return (int64_t)a.Hkv * s.blocks * s.tiles; }
-
-// a CTA's place in the line of tiles
-struct TreeCursor {
-    int b;
-    int64_t off;        // tile inside sequence b's part of the line
-    int64_t pos, end;   // tile inside the whole line
-};
-
-// one piece: consecutive tiles of one item
-struct TreePiece {
-    TreeSeq s;
-    int b, hk, block, t0, count;
-    int64_t item_pos;   // where the item's line starts
-};
-
-__device__ __forceinline__ bool next_piece(const KvTreeArgs &a, TreeCursor &c, int block_rows, TreePiece &p)
-{
-    while (c.pos < c.end) {
-        p.s = tree_seq(a, c.b, block_rows);
-        const int64_t total = tree_tiles(a, p.s);
-        if (c.off >= total) {
-            c.off -= total;
-            ++c.b;
-            continue;
-        }
-        const int64_t item = c.off / p.s.tiles;
-        p.b = c.b;
-        p.t0 = (int)(c.off - item * p.s.tiles);
-        p.hk = (int)(item / p.s.blocks);
-        p.block = (int)(item - (int64_t)p.hk * p.s.blocks);
-        const int64_t left = c.end - c.pos;
-        p.count = p.s.tiles - p.t0 < left ? p.s.tiles - p.t0 : (int)left;
-        p.item_pos = c.pos - p.t0;
-        c.off += p.count;
-        c.pos += p.count;
-        return true;
-    }
-    return false;
-}
 
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -157,15 +96,6 @@ __device__ __forceinline__ int key_perm(int g) { return g & 1 ? g ^ 4 : g; }
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(KT_CONSUMERS * 32) : "memory"); }
 
-__device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
-
-// whether token t sees new token j
-__device__ __forceinline__ bool tree_sees(const KvTreeArgs &a, int b, int t, int j)
-{
-    if (!a.mask) return j <= t;
-    return (__ldg(a.mask + b * a.mask_stride + (int64_t)t * a.words + (j >> 6)) >> (j & 63)) & 1;
-}
-
 // What a lane (g = lane / 4, t = lane % 4) holds of its warp's query rows.  o[i][n]: columns 32*(i/2) + 4g + 2*(i%2) (elements
 // 0: row 8n + 2t, 1: row 8n + 2t + 1) and the column behind it (elements 2, 3).
 template <int DKP, int NR>
@@ -175,12 +105,12 @@ struct TreeWarp {
 };
 
 // One warp, 16 keys.  TAIL: some of them lie behind the cached rows.  toks: the token of each of the warp's query rows.
-template <int DKP, int NR, int RG, bool TAIL>
+template <int DKP, int NR, bool TAIL>
 __device__ __forceinline__ void tree_tile(const KvTreeArgs &a, TreeWarp<DKP, NR> &w, const uint8_t *qbase, const uint8_t *kbase, const uint8_t *vbase,
                                           int key0, int row0, const TreeSeq &s, int b, const int *toks, uint32_t k_empty, uint32_t v_full,
                                           uint32_t v_parity, bool &ok)
 {
-    using C = TreeCfg<DKP, NR, RG>;
+    using C = TreeCfg<DKP, NR>;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // S^T: rows g, g+8 = keys row0 + perm(g) (+ 8), columns 2t, 2t+1 of each eight query rows; the cross products in chains of
     // their own, which shortens the dependent chain
@@ -223,15 +153,11 @@ __device__ __forceinline__ void tree_tile(const KvTreeArgs &a, TreeWarp<DKP, NR>
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(k_empty);
-    // scores in the log2 domain, the row maxima, the factor on what was summed before, P^T as operand B (k = t, t+4: keys 2t,
-    // 2t+1 of each eight; column g: query row 8n + g)
-    float corr[NR][2];
-    uint32_t phi[NR][4], plo[NR][4];
-    const int from = 8 * t + (g >> 1);               // lane that holds key 2t (row 2t of S^T) and query row g; key 2t+1: row (2t+1)^4
-    const int from1 = 4 * ((2 * t + 1) ^ 4) + (g >> 1);
+    // Scores in the log2 domain.  The reference that is taken off in the exponent need not be the maximum: while no score
+    // is more than 2^8 above it (one vote), it stays and nothing summed before needs a factor.
+    bool above = false;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        float mx[2] = { -INFINITY, -INFINITY };
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float x = (sc[n][e] + (NR == 1 ? x1[n][e] + x2[0][e] : x1[n][e])) * a.c_log2;
@@ -240,16 +166,33 @@ __device__ __forceinline__ void tree_tile(const KvTreeArgs &a, TreeWarp<DKP, NR>
                 if (j >= 0 && (j >= s.n || !tree_sees(a, b, toks[8 * n + 2 * t + (e & 1)], j))) x = -INFINITY;
             }
             sc[n][e] = x;
-            mx[e & 1] = fmaxf(mx[e & 1], x);
+            above = above || x > w.m[n][e & 1] + 8.f;
         }
+    float corr[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) corr[n][0] = corr[n][1] = 1.f;
+    if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float top = fmaxf(sc[n][r], sc[n][2 + r]);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float m_new = fmaxf(w.m[n][r], top);
+                corr[n][r] = ex2_approx(w.m[n][r] - (m_new == -INFINITY ? 0.f : m_new));
+                w.m[n][r] = m_new;
+            }
+    }
+    // P^T as operand B (k = t, t+4: keys 2t, 2t+1 of each eight; column g: query row 8n + g)
+    uint32_t phi[NR][4], plo[NR][4];
+    const int from = 8 * t + (g >> 1);               // lane that holds key 2t (row 2t of S^T) and query row g; key 2t+1: row (2t+1)^4
+    const int from1 = 4 * ((2 * t + 1) ^ 4) + (g >> 1);
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], o));
-            const float m_new = fmaxf(w.m[n][r], mx[r]);
-            const float base = m_new == -INFINITY ? 0.f : m_new;   // nothing seen so far: every p below is 2^-inf = 0
-            corr[n][r] = ex2_approx(w.m[n][r] - base);
-            w.m[n][r] = m_new;
+            const float base = w.m[n][r] == -INFINITY ? 0.f : w.m[n][r];   // nothing seen so far: p = 2^-inf = 0
             sc[n][r] = ex2_approx(sc[n][r] - base);
             sc[n][2 + r] = ex2_approx(sc[n][2 + r] - base);
             w.l[n][r] = fmaf(w.l[n][r], corr[n][r], sc[n][r] + sc[n][2 + r]);
@@ -377,15 +320,15 @@ __device__ __forceinline__ void tree_put(const TreeWarp<DKP, NR> &w, float4 *fra
         for (int n = 0; n < NR; ++n) frag[(i * NR + n) * stride] = make_float4(w.o[i][n][0], w.o[i][n][1], w.o[i][n][2], w.o[i][n][3]);
 }
 
-// all parts of a row group into its part 0: halves, quarters, ...; every consumer warp takes part
-template <int DKP, int NR, int RG>
-__device__ __forceinline__ void tree_merge(TreeWarp<DKP, NR> &w, float4 *area, int rg, int part)
+// all warps' parts into warp 0's: halves, quarters, ...; every consumer warp takes part
+template <int DKP, int NR>
+__device__ __forceinline__ void tree_merge(TreeWarp<DKP, NR> &w, float4 *area, int part)
 {
-    using C = TreeCfg<DKP, NR, RG>;
+    using C = TreeCfg<DKP, NR>;
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
-    for (int half = C::PARTS / 2; half >= 1; half >>= 1) {
-        float4 *frag = area + (size_t)(rg * (C::PARTS / 2) + (part >= half ? part - half : part)) * 32 * (C::FRAGS + NR) + lane;
+    for (int half = KT_CONSUMERS / 2; half >= 1; half >>= 1) {
+        float4 *frag = area + (size_t)(part >= half ? part - half : part) * 32 * (C::FRAGS + NR) + lane;
         if (part >= half && part < 2 * half) tree_put<DKP, NR>(w, frag, frag + C::FRAGS * 32, 32);
         consumers_sync();
         if (part < half) tree_add<DKP, NR>(w, frag, frag + C::FRAGS * 32, 32);
@@ -393,18 +336,17 @@ __device__ __forceinline__ void tree_merge(TreeWarp<DKP, NR> &w, float4 *area, i
     }
 }
 
-template <int DKP, int NR, int RG>
-__global__ void __launch_bounds__(TreeCfg<DKP, NR, RG>::THREADS, 1)
+template <int DKP, int NR>
+__global__ void __launch_bounds__(TreeCfg<DKP, NR>::THREADS, 1)
 kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ TreeMaps tm, int tma)
 {
-    using C = TreeCfg<DKP, NR, RG>;
+    using C = TreeCfg<DKP, NR>;
     constexpr int ROWS = C::ROWS;
     extern __shared__ uint8_t smem_raw[];
     __shared__ alignas(8) uint64_t bars[6 * C::STAGES];
-    __shared__ unsigned long long s_total;
-    __shared__ int s_b, s_last, s_tok[ROWS];
+    __shared__ unsigned long long s_line[3];
+    __shared__ int s_last, s_tok[ROWS];
     __shared__ volatile int s_gave_up;   // a consumer's wait ran out: its arrivals no longer mean free stages
-    __shared__ long long s_off;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t *const tiles = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);   // the swizzle is a function of the address
     float4 *const area = reinterpret_cast<float4 *>(tiles + C::STAGES * 2 * C::TILE);
@@ -416,54 +358,13 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
     auto full_bar = [&](int v, int stage, uint32_t use) { return bar0 + 8u * ((2 + 2 * v + (use & 1)) * C::STAGES + stage); };
     auto ktile = [&](int stage) { return tiles + stage * 2 * C::TILE; };
     if (tid == 0) {
-        s_total = 0;
         s_gave_up = 0;
-        for (int i = 0; i < 6 * C::STAGES; ++i) mbar_init(bar0 + 8u * i, i < 2 * C::STAGES ? RG * C::SLICES : (tma ? 1 : 32));
+        for (int i = 0; i < 6 * C::STAGES; ++i) mbar_init(bar0 + 8u * i, i < 2 * C::STAGES ? C::SLICES : (tma ? 1 : 32));
         mbar_fence_init();
     }
-    __syncthreads();
-
-    // the line of tiles, this CTA's part of it, and the sequence that part starts in
-    {
-        unsigned long long sum = 0;
-        for (int b = tid; b < a.B; b += C::THREADS) {
-            bool bad;
-            const TreeSeq s = tree_seq(a, b, ROWS, &bad);
-            sum += (unsigned long long)tree_tiles(a, s);
-            if (bad && blockIdx.x == 0 && a.err) atomicCAS(a.err, 0, (int)AXB_DEVERR_ROWS);
-        }
-        if (sum) atomicAdd(&s_total, sum);
-        __syncthreads();
-    }
-    const int64_t total = (int64_t)s_total, per = (total + gridDim.x - 1) / gridDim.x;
+    constexpr TreeLine line = { ROWS, KT_KEYS };
     TreeCursor cur;
-    cur.pos = per * blockIdx.x;
-    cur.end = cur.pos + per < total ? cur.pos + per : total;
-    if (cur.pos >= cur.end) return;
-    if (warp == 0) {
-        int64_t before = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 32) {
-            const int64_t mine = b0 + lane < a.B ? tree_tiles(a, tree_seq(a, b0 + lane, ROWS)) : 0;
-            int64_t upto = mine;
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += v;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, before + upto > cur.pos);
-            if (past) {
-                const int k = __ffs(past) - 1;
-                if (lane == k) {
-                    s_b = b0 + k;
-                    s_off = cur.pos - (before + upto - mine);
-                }
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, upto, 31);
-        }
-    }
-    __syncthreads();
-    cur.b = s_b;
-    cur.off = s_off;
+    if (!tree_start(a, line, s_line, cur)) return;   // (its barriers make the initialised ones above visible)
     TreePiece p;
     bool ok = true;
     uint32_t it = 0;   // tiles since the start: ring stage it % STAGES, its use number it / STAGES
@@ -471,11 +372,11 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
     if (warp >= KT_CONSUMERS) {
         // ---- producers: warp 8 the K tiles, warp 9 the V tiles (one issuing thread turns a 16 KB tile around in some 700
         // cycles, which HBM's share of an SM would just about saturate)
-        if (C::SHIFT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+        if (C::SHIFT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp > KT_CONSUMERS + 1) return;
         const int v = warp - KT_CONSUMERS;
         const float *const cache = v ? a.V : a.K;
-        while (ok && next_piece(a, cur, ROWS, p)) {
+        while (ok && next_piece(a, line, cur, p)) {
             const int head = p.b * a.Hkv + p.hk;
             for (int i = 0; ok && i < p.count; ++i, ++it) {
                 const int s = it % C::STAGES, row = (p.t0 + i) * KT_KEYS;
@@ -519,8 +420,8 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
     }
 
     // ---- consumers
-    if (C::SHIFT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
-    const int g = lane >> 2, t = lane & 3, rg = warp % RG, part = warp / RG, grp = part / C::SLICES, row0 = part % C::SLICES * 16;
+    if (C::SHIFT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int g = lane >> 2, t = lane & 3, part = warp, grp = part / C::SLICES, row0 = part % C::SLICES * 16;
     const int heads_per = a.H / a.Hkv;
     TreeWarp<DKP, NR> w;
     auto clear = [&] {
@@ -532,7 +433,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
             for (int i = 0; i < DKP / 16; ++i) w.o[i][n][0] = w.o[i][n][1] = w.o[i][n][2] = w.o[i][n][3] = 0.f;
         }
     };
-    while (next_piece(a, cur, ROWS, p)) {
+    while (next_piece(a, line, cur, p)) {
         // query row r: head r / n of the group, token r % n.  Q as the lanes will read it, in the merge area:
         // [eight rows][16-column group][(hi, lo)][lane]
         for (int i = tid; i < ROWS * (DKP / 4); i += KT_CONSUMERS * 32) {
@@ -558,9 +459,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
             if (C::SPLIT_Q)
                 area[at + 32] = make_float4(__uint_as_float(tf32_lo(x.x)), __uint_as_float(tf32_lo(x.y)), __uint_as_float(tf32_lo(x.z)), __uint_as_float(tf32_lo(x.w)));
         }
-        const uint8_t *qbase = reinterpret_cast<const uint8_t *>(area) + rg * NR * (DKP / 16) * (C::SPLIT_Q ? 1024 : 512) + lane * 16;
-        const int *toks = s_tok + rg * 8 * NR;
-        const bool idle = p.block * ROWS + rg * 8 * NR >= p.s.rows;
+        const uint8_t *qbase = reinterpret_cast<const uint8_t *>(area) + lane * 16;
         clear();
         consumers_sync();
 
@@ -570,15 +469,13 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
             const uint32_t use = it / C::STAGES, ph = (use >> 1) & 1;
             const int key0 = (p.t0 + i) * KT_KEYS;
             if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(full_bar(0, s, use), ph))) ok = false;
-            const bool work = ok && !idle;
+            const bool work = ok;
             if (work) {
                 const uint8_t *kt = ktile(s);
                 if (key0 + row0 + 16 > p.s.len)
-                    tree_tile<DKP, NR, RG, true>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, toks, empty_bar(0, s), full_bar(1, s, use), ph, ok);
+                    tree_tile<DKP, NR, true>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, s_tok, empty_bar(0, s), full_bar(1, s, use), ph, ok);
                 else
-                    tree_tile<DKP, NR, RG, false>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, toks, empty_bar(0, s), full_bar(1, s, use), ph, ok);
-            } else if (ok) {
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(full_bar(1, s, use), ph))) ok = false;
+                    tree_tile<DKP, NR, false>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, s_tok, empty_bar(0, s), full_bar(1, s, use), ph, ok);
             }
             if (!ok) {
                 s_gave_up = 1;
@@ -598,16 +495,15 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) w.l[n][r] += __shfl_xor_sync(0xffffffffu, w.l[n][r], o);
         consumers_sync();   // Q has been read
-        tree_merge<DKP, NR, RG>(w, area, rg, part);
+        tree_merge<DKP, NR>(w, area, part);
 
         bool write = p.count == p.s.tiles;
         if (!write) {
-            // the item's pieces belong to consecutive CTAs; the first one's index names its counter.  Slots: [row group][lane order]
-            const int first = (int)(p.item_pos / per), pieces = (int)((p.item_pos + p.s.tiles - 1) / per) - first + 1;
-            constexpr int GROUP_F4 = 32 * (C::FRAGS + NR);
-            auto slot = [&](int k) { return reinterpret_cast<float4 *>(a.slots) + (size_t)k * (RG * GROUP_F4) + rg * GROUP_F4 + lane; };
+            // the item's first CTA names its counter
+            const int first = p.first, pieces = p.pieces;
+            auto slot = [&](int k) { return reinterpret_cast<float4 *>(a.slots) + (size_t)k * (32 * (C::FRAGS + NR)) + lane; };
             if (part == 0) {
-                float4 *f = slot(2 * (int)blockIdx.x + (p.t0 == 0 ? 1 : 0));
+                float4 *f = slot(tree_slot(blockIdx.x, p.t0 == 0));
                 tree_put<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
                 __threadfence();
             }
@@ -619,11 +515,11 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
                 __threadfence();
                 clear();
 #pragma unroll 1
-                for (int k = part; k < pieces; k += C::PARTS) {
-                    const float4 *f = slot(2 * (first + k) + (k == 0 ? 1 : 0));
+                for (int k = part; k < pieces; k += KT_CONSUMERS) {
+                    const float4 *f = slot(tree_slot(first + k, k == 0));
                     tree_add<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
                 }
-                tree_merge<DKP, NR, RG>(w, area, rg, part);
+                tree_merge<DKP, NR>(w, area, part);
                 if (tid == 0) a.counters[first] = 0;
             }
         }
@@ -632,7 +528,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
             for (int n = 0; n < NR; ++n)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const int row = p.block * ROWS + (rg * NR + n) * 8 + 2 * t + r;
+                    const int row = p.block * ROWS + n * 8 + 2 * t + r;
                     if (row >= p.s.rows) continue;
                     const int gh = row / p.s.n, tok = row - gh * p.s.n;
                     float *dst = a.out + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk;
@@ -718,44 +614,44 @@ size_t kv_tree_workspace_bytes(int sm_count)
     return (size_t)sm_count * 2 * KT_SLOT_BYTES;
 }
 
-template <int DKP, int NR, int RG>
+template <int DKP, int NR>
 static int launch_tree(const KvTreeArgs &a, const TreeMaps &tm, int tma, int sm_count, cudaStream_t st)
 {
-    using C = TreeCfg<DKP, NR, RG>;
+    using C = TreeCfg<DKP, NR>;
     static_assert(C::STAGES >= 2 && C::SMEM <= 227 * 1024 - 2048, "shared memory");
-    static_assert((size_t)RG * 32 * (C::FRAGS + NR) * 16 <= KT_SLOT_BYTES, "workspace slots");
+    static_assert((size_t)32 * (C::FRAGS + NR) * 16 <= KT_SLOT_BYTES, "workspace slots");
     static PerDeviceOnce once;
     if (once.first()) {
-        cudaError_t e = cudaFuncSetAttribute(kv_tree_kernel<DKP, NR, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(kv_tree_kernel<DKP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return (int)e;
     }
-    kv_tree_kernel<DKP, NR, RG><<<sm_count, C::THREADS, C::SMEM, st>>>(a, tm, tma);
+    kv_tree_kernel<DKP, NR><<<sm_count, C::THREADS, C::SMEM, st>>>(a, tm, tma);
     return (int)cudaGetLastError();
 }
 
-template <int NR, int RG>
+template <int NR>
 static int launch_tree_rows(const KvTreeArgs &a, const TreeMaps &tm, int tma, int sm_count, cudaStream_t st)
 {
-    if (a.dk <= 32) return launch_tree<32, NR, RG>(a, tm, tma, sm_count, st);
-    if (a.dk <= 64) return launch_tree<64, NR, RG>(a, tm, tma, sm_count, st);
-    if (a.dk <= 96) return launch_tree<96, NR, RG>(a, tm, tma, sm_count, st);
-    return launch_tree<128, NR, RG>(a, tm, tma, sm_count, st);
+    if (a.dk <= 32) return launch_tree<32, NR>(a, tm, tma, sm_count, st);
+    if (a.dk <= 64) return launch_tree<64, NR>(a, tm, tma, sm_count, st);
+    if (a.dk <= 96) return launch_tree<96, NR>(a, tm, tma, sm_count, st);
+    return launch_tree<128, NR>(a, tm, tma, sm_count, st);
 }
 
 int launch_kv_cache_attend_tree(const KvTreeArgs &a, int sm_count, cudaStream_t st)
 {
     const int tma = a.dk % 4 == 0 && kt_aligned16(a.K) && kt_aligned16(a.V) && kt_aligned16(a.Q) && kt_aligned16(a.out);
+    const int64_t rows = (int64_t)(a.H / a.Hkv) * a.T;   // of a key head, if every token is there
+    if (tma && rows > KT_TC_ROWS) return launch_kv_tree_tc(a, sm_count, st);
     TreeMaps tm = {};
     if (tma) {
         int e = encode_f32_batched_tmap(&tm.k, a.K, (int64_t)a.B * a.Hkv, a.max_seq, a.dk, a.dk, KT_KEYS, false);
         if (!e) e = encode_f32_batched_tmap(&tm.v, a.V, (int64_t)a.B * a.Hkv, a.max_seq, a.dk, a.dk, KT_KEYS, false);
         if (e) return e;
     }
-    const int64_t rows = (int64_t)(a.H / a.Hkv) * a.T;   // of a key head, if every token is there
-    if (rows <= 8) return launch_tree_rows<1, 1>(a, tm, tma, sm_count, st);
-    if (rows <= 16) return launch_tree_rows<2, 1>(a, tm, tma, sm_count, st);
-    if (rows <= 32) return launch_tree_rows<4, 1>(a, tm, tma, sm_count, st);
-    return launch_tree_rows<4, 2>(a, tm, tma, sm_count, st);
+    if (rows <= 8) return launch_tree_rows<1>(a, tm, tma, sm_count, st);
+    if (rows <= 16) return launch_tree_rows<2>(a, tm, tma, sm_count, st);
+    return launch_tree_rows<4>(a, tm, tma, sm_count, st);
 }
 
 int launch_kv_cache_compact(float *K, float *V, const int32_t *keep, const int32_t *n_keep, const int32_t *lens, int32_t *lens_out,

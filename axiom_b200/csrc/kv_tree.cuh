@@ -13,7 +13,7 @@ struct KvTreeArgs {
     const uint64_t *mask;        // [B or 1][T][words] bit j of token t: t attends to new token j; nullptr: j <= t
     const int32_t *lens, *n_new; // [B]; n_new nullptr: T for every sequence
     float *out;                  // [B*H, T, dk]
-    int *counters;               // one per SM, zero on entry and on exit
+    int *counters;               // three per SM, zero on entry and on exit
     float *slots;                // kv_tree_workspace_bytes(): partial results, two slots per SM
     int64_t max_seq, mask_stride;
     int *err;
@@ -21,7 +21,11 @@ struct KvTreeArgs {
     int B, H, Hkv, T, dk, words;
 };
 
+constexpr size_t KT_SLOT_BYTES = 128 * (128 + 2) * sizeof(float);   // the largest variant's partial result
 size_t kv_tree_workspace_bytes(int sm_count);
+// query rows of a key head from which on the tensor-memory kernel (kv_tree_tc.cu) takes over; it wants 16-byte pieces
+constexpr int KT_TC_ROWS = 32;
+int launch_kv_tree_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st);
 int launch_kv_cache_attend_tree(const KvTreeArgs &a, int sm_count, cudaStream_t st);
 
 // rows lens[b] + keep[b][i] -> lens[b] + i for i < n_keep[b] in both caches; lens_out[b] = lens[b] + n_keep[b] (or nullptr)

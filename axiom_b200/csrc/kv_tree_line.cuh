@@ -1,0 +1,134 @@
+// kv_tree_line.cuh — how the kernels of kv_cache_attend_tree divide a ragged batch between their CTAs, on the device.
+// The key tiles of all (sequence, key head, row block) items form one line, cut into equal stretches, one a CTA; the
+// CTAs that share an item are consecutive and each holds a tile of it.
+#pragma once
+#include "../../include/axiom_b200.h"
+#include "kv_tree.cuh"
+
+namespace axb {
+
+// query rows of an item, keys of a tile
+struct TreeLine {
+    int block_rows, tile_keys;
+};
+
+struct TreeSeq {
+    int len, n, rows, blocks, tiles;   // cached rows, new tokens, query rows of a key head, row blocks, key tiles
+};
+
+__device__ __forceinline__ TreeSeq tree_seq(const KvTreeArgs &a, const TreeLine &ln, int b, bool *bad = nullptr)
+{
+    TreeSeq s;
+    s.len = __ldg(a.lens + b);
+    s.n = a.n_new ? __ldg(a.n_new + b) : a.T;
+    const bool off = s.len < 0 || s.n < 0 || s.n > a.T || (int64_t)s.len + s.n > a.max_seq;
+    if (bad) *bad = off;
+    if (off) s.len = s.n = 0;   // refused whole: its output rows are left alone
+    s.rows = s.n * (a.H / a.Hkv);
+    s.blocks = (s.rows + ln.block_rows - 1) / ln.block_rows;
+    s.tiles = s.n ? (int)(((int64_t)s.len + s.n + ln.tile_keys - 1) / ln.tile_keys) : 0;
+    return s;
+}
+
+__device__ __forceinline__ int64_t tree_tiles(const KvTreeArgs &a, const TreeSeq &s) { return (int64_t)a.Hkv * s.blocks * s.tiles; }
+
+struct TreeCursor {
+    int b;
+    int64_t base;      // where sequence b's part of the line begins
+    int64_t pos, end;  // what is left of this CTA's stretch
+    int64_t per;       // a stretch
+};
+
+// one piece: consecutive tiles of one item
+struct TreePiece {
+    TreeSeq s;
+    int b, hk, block, t0, count;
+    int first, pieces;   // the CTA that holds the item's first tile, and how many CTAs hold some
+};
+
+// Every thread of the CTA; shared: 3 words.  False: nothing for this CTA (for all its threads).
+__device__ __forceinline__ bool tree_start(const KvTreeArgs &a, const TreeLine &ln, unsigned long long *shared, TreeCursor &c)
+{
+    if (threadIdx.x == 0) shared[0] = 0;
+    __syncthreads();
+    unsigned long long sum = 0;
+    for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
+        bool bad;
+        const TreeSeq s = tree_seq(a, ln, b, &bad);
+        sum += (unsigned long long)tree_tiles(a, s);
+        if (bad && blockIdx.x == 0 && a.err) atomicCAS(a.err, 0, (int)AXB_DEVERR_ROWS);
+    }
+    if (sum) atomicAdd(shared, sum);
+    __syncthreads();
+    const int64_t total = (int64_t)shared[0];
+    c.per = (total + gridDim.x - 1) / gridDim.x;
+    c.pos = c.per * blockIdx.x;
+    c.end = c.pos + c.per < total ? c.pos + c.per : total;
+    if (c.pos >= c.end) return false;
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        int64_t before = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 32) {
+            const int64_t mine = b0 + lane < a.B ? tree_tiles(a, tree_seq(a, ln, b0 + lane)) : 0;
+            int64_t upto = mine;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, before + upto > c.pos);
+            if (past) {
+                const int k = __ffs(past) - 1;
+                if (lane == k) {
+                    shared[1] = (unsigned long long)(b0 + k);
+                    shared[2] = (unsigned long long)(before + upto - mine);
+                }
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+    __syncthreads();
+    c.b = (int)shared[1];
+    c.base = (int64_t)shared[2];
+    return true;
+}
+
+__device__ __forceinline__ bool next_piece(const KvTreeArgs &a, const TreeLine &ln, TreeCursor &c, TreePiece &p)
+{
+    while (c.pos < c.end) {
+        p.s = tree_seq(a, ln, c.b);
+        const int64_t total = tree_tiles(a, p.s);
+        if (c.pos >= c.base + total) {
+            c.base += total;
+            ++c.b;
+            continue;
+        }
+        const int64_t item = (c.pos - c.base) / p.s.tiles, item_pos = c.base + item * p.s.tiles;
+        p.b = c.b;
+        p.t0 = (int)(c.pos - item_pos);
+        p.hk = (int)(item / p.s.blocks);
+        p.block = (int)(item - (int64_t)p.hk * p.s.blocks);
+        const int64_t left = c.end - c.pos;
+        p.count = p.s.tiles - p.t0 < left ? p.s.tiles - p.t0 : (int)left;
+        p.first = (int)(item_pos / c.per);
+        p.pieces = (int)((item_pos + p.s.tiles - 1) / c.per) - p.first + 1;
+        c.pos += p.count;
+        return true;
+    }
+    return false;
+}
+
+// A CTA holds at most one piece that continues an item (its first) and one that begins an item it does not finish (its
+// last): two workspace slots a CTA are enough.
+__device__ __forceinline__ int tree_slot(int cta, bool begins) { return 2 * cta + (begins ? 1 : 0); }
+
+// whether token t sees new token j
+__device__ __forceinline__ bool tree_sees(const KvTreeArgs &a, int b, int t, int j)
+{
+    if (!a.mask) return j <= t;
+    return (__ldg(a.mask + b * a.mask_stride + (int64_t)t * a.words + (j >> 6)) >> (j & 63)) & 1;
+}
+
+__device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+}  // namespace axb

@@ -1,0 +1,613 @@
+// kv_tree_tc.cu — kv_cache_attend_tree when many query rows share a key head (wide trees, grouped heads, chunks of a
+// prompt): the same result as kv_tree.cu on tcgen05, 128 query rows of a key head at a time, head dim <= 128.
+//     S = Q.K^T, O = P.V as three tf32 products each over hi/lo parts; the value as it lies is the hi operand (the tensor
+//     core reads its tf32 part), the remainder rounded to tf32 the lo operand.
+// The work line of kv_tree_line.cuh, cut into one stretch per CTA, replaces the grid over query tiles; key blocks of 128
+// (head dim <= 64) or 64 keys.  Twenty warps:
+//   0-7   softmax: two threads per query row, half the block's columns each (they swap maxima through shared memory).  P hi is
+//         written over the scores in tensor memory, P lo beside them: both are the A operand of P.V as they lie.  The
+//         exponent's reference stays until a score passes it by 2^8; every block's P.V starts from zero and is folded into
+//         fp32 registers, so the tensor core's truncating accumulation never spans more than a block.
+//   8-11  Q of a piece (gathered rows -> swizzled shared memory, lo part there or, for head dims above 64, in tensor
+//         memory), then the lo part of every K block;   12-15  the lo part of every V block, and what must not reach the
+//         product: rows behind the last token, and infinities or NaN in new rows (those are added row by row).
+//   16, 17  TMA of K and V (the operand whose chain is the longer one has two raw buffers: V for head dims up to 64, K above);
+//   18, 19  one thread each issues the score and the P.V products.
+// Shared memory is full either way (224 KB): Q 64 KB, five K / V tiles of 32 KB.  A block costs the same for one row or 128; up to
+// 32 rows the warp-level kernel is the faster one.
+#include "errors.cuh"
+#include "gemm_tc.cuh"
+#include "kv_tree_line.cuh"
+#include "ptx.cuh"
+
+#include <cuda.h>
+#include <math.h>
+
+namespace axb {
+
+static constexpr int TT_ROWS = 128, TT_THREADS = 640;
+enum { CERR_LOAD = 94, CERR_CONVERT = 95, CERR_MMA = 96, CERR_SOFTMAX = 97 };
+
+template <int NSLAB>
+struct TreeTc {
+    static constexpr bool WIDE = NSLAB > 2;
+    static constexpr int DKP = 32 * NSLAB;
+    static constexpr int KB = WIDE ? 64 : 128;                 // keys of a block
+    static constexpr int QSLAB = TT_ROWS * 128, SLAB = KB * 128;   // bytes of 32 columns
+    static constexpr int QPLANE = NSLAB * QSLAB, PLANE = NSLAB * SLAB;
+    static constexpr int KS = WIDE ? 2 : 1, VS = WIDE ? 1 : 2; // raw buffers
+    static constexpr int OB = WIDE ? 1 : 2;                    // accumulators of P.V
+    // tensor memory columns
+    static constexpr int T_S = 0, T_PLO = 2 * KB, T_O = 3 * KB, T_QLO = T_O + OB * DKP;
+    static constexpr int COLS = 512;
+    static_assert(T_QLO + (WIDE ? DKP : 0) <= COLS, "tensor memory");
+    static constexpr int HEADER = 3072;   // barriers, words, then the softmax threads' maxima
+    static constexpr int Q_AT = HEADER, K_AT = Q_AT + QPLANE * (WIDE ? 1 : 2), KLO_AT = K_AT + KS * PLANE, V_AT = KLO_AT + PLANE,
+                         VLO_AT = V_AT + VS * PLANE, SMEM = VLO_AT + PLANE;
+    static_assert(SMEM <= 227 * 1024, "shared memory");   // all of it: the kernel has no static shared memory
+};
+
+enum {
+    TB_Q_FULL, TB_Q_EMPTY, TB_K_RAW, TB_K_FULL = TB_K_RAW + 2, TB_K_EMPTY, TB_V_RAW = TB_K_EMPTY + 2, TB_V_FULL = TB_V_RAW + 2, TB_V_EMPTY,
+    TB_S_FULL = TB_V_EMPTY + 2, TB_P_FULL = TB_S_FULL + 2, TB_PLO_FULL = TB_P_FULL + 2, TB_KLO_EMPTY, TB_VLO_EMPTY, TB_O_FULL, TB_O_EMPTY = TB_O_FULL + 2, TB_DRAIN = TB_O_EMPTY + 2,
+    TB_COUNT = TB_DRAIN + 2
+};
+
+struct TreeTcMaps {
+    CUtensorMap k, v;   // [B*Hkv][max_seq][dk], boxes of 32 columns x KB rows (v: 32-byte swizzle atoms)
+};
+
+__device__ __forceinline__ uint32_t lo_bits(uint32_t x)
+{
+    return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u)) + 0x1000u;
+}
+
+// the three products of a block's scores / outputs, issued by one thread.  B: block parity.  Everything that an instruction
+// names is a constant offset from the bases, so that it takes no moves into the registers that tcgen05.mma reads (with
+// addresses formed at run time an instruction cost the issuing thread 110 cycles where the pipe takes 48 to 64).
+template <int NSLAB, int B>
+__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, uint32_t idesc, uint32_t klo_empty)
+{
+    using C = TreeTc<NSLAB>;
+    const uint64_t dk = smem_desc_kmajor(0, 128);
+    auto desc = [&](uint32_t at) { return dk | (uint64_t)(((base + at) & 0x3FFFFu) >> 4); };
+    constexpr uint32_t khi = C::K_AT + (B % C::KS) * C::PLANE;
+#pragma unroll
+    for (int pr = 0; pr < 3; ++pr) {   // hi.lo, whose lo tile the next block waits for, lo.hi, hi.hi
+        const uint32_t kk = pr == 0 ? C::KLO_AT : khi, qq = C::Q_AT + (pr == 1 && !C::WIDE ? C::QPLANE : 0);
+#pragma unroll
+        for (int ks = 0; ks < 4 * NSLAB; ++ks) {   // (columns from dk on are zero)
+            const uint64_t bd = desc(kk + (ks >> 2) * C::SLAB + (ks & 3) * 32);
+            if (C::WIDE && pr == 1) tc_mma_ts_tf32(tmem + C::T_S + B * C::KB, tmem + C::T_QLO + ks * 8, bd, idesc, 1);
+            else tc_mma<KIND_TF32>(tmem + C::T_S + B * C::KB, desc(qq + (ks >> 2) * C::QSLAB + (ks & 3) * 32), bd, idesc, pr | ks);
+        }
+        if (pr == 0) tc_commit(klo_empty);
+    }
+}
+
+// part 0: hi.lo and hi.hi; part 1: lo.hi, whose operand comes last
+template <int NSLAB, int B, int PART>
+__device__ __forceinline__ void issue_outputs(uint32_t base, uint32_t tmem, uint32_t idesc, uint32_t vlo_empty)
+{
+    using C = TreeTc<NSLAB>;
+    const uint64_t dm = smem_desc_mnmajor_sw128_32b(0, C::SLAB, 512);
+    auto desc = [&](uint32_t at) { return dm | (uint64_t)(((base + at) & 0x3FFFFu) >> 4); };
+    constexpr uint32_t vhi = C::V_AT + (B % C::VS) * C::PLANE;
+    const uint32_t d = tmem + C::T_O + (B % C::OB) * C::DKP;
+    if (PART == 0) {
+#pragma unroll
+        for (int ks = 0; ks < C::KB / 8; ++ks) tc_mma_ts_tf32(d, tmem + C::T_S + B * C::KB + ks * 8, desc(C::VLO_AT + ks * 1024), idesc, ks);
+        tc_commit(vlo_empty);
+#pragma unroll
+        for (int ks = 0; ks < C::KB / 8; ++ks) tc_mma_ts_tf32(d, tmem + C::T_S + B * C::KB + ks * 8, desc(vhi + ks * 1024), idesc, 1);
+    } else {
+#pragma unroll
+        for (int ks = 0; ks < C::KB / 8; ++ks) tc_mma_ts_tf32(d, tmem + C::T_PLO + ks * 8, desc(vhi + ks * 1024), idesc, 1);
+    }
+}
+
+// which of the 32 keys from new-token index `base` (negative: cached rows) token t sees
+__device__ __forceinline__ uint32_t seen_bits(const KvTreeArgs &a, int b, int t, int n, int base)
+{
+    if (base <= -32) return 0xFFFFFFFFu;
+    const int j0 = base > 0 ? base : 0, skip = j0 - base;   // skip cached rows come first
+    uint32_t bits = 0;
+    if (j0 < n) {
+        if (!a.mask) {
+            const int last = t < n - 1 ? t : n - 1;
+            bits = last - j0 >= 31 ? 0xFFFFFFFFu : last < j0 ? 0u : (2u << (last - j0)) - 1u;
+        } else {
+            const uint64_t *m = a.mask + b * a.mask_stride + (int64_t)t * a.words + (j0 >> 6);
+            const int sh = j0 & 63;
+            uint64_t w = __ldg(m) >> sh;
+            if (sh && (j0 >> 6) + 1 < a.words) w |= __ldg(m + 1) << (64 - sh);
+            bits = (uint32_t)w;
+            if (n - j0 < 32) bits &= (1u << (n - j0)) - 1u;
+        }
+    }
+    return skip ? (bits << skip) | ((1u << skip) - 1u) : bits;
+}
+
+template <int NSLAB>
+__global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ TreeTcMaps tm)
+{
+    using C = TreeTc<NSLAB>;
+    constexpr int KB = C::KB, OH = C::DKP / 2;   // OH: output columns of a softmax thread
+    extern __shared__ __align__(1024) uint8_t sm[];
+    const uint32_t base = smem_u32(sm);
+    auto bar = [&](int i) -> uint32_t { return base + 8u * (uint32_t)i; };
+    unsigned long long *s_line = reinterpret_cast<unsigned long long *>(sm + 512);
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(sm + 544);
+    volatile int *words = reinterpret_cast<volatile int *>(sm + 560);
+    volatile int &s_gave_up = words[0], &s_last = words[1], *s_odd = words + 2;   // s_odd: block it + 1 holds non-finite new values
+    float (*s_max)[2][TT_ROWS] = reinterpret_cast<float (*)[2][TT_ROWS]>(sm + 1024);   // [block parity][half][row]
+    if (base & 1023) {   // the swizzles are functions of the address (it starts at a multiple of 1 KB; refused, should it ever not)
+        if (threadIdx.x == 0 && a.err) atomicCAS(a.err, 0, (int)CERR_LOAD);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    static_assert(8 * TB_COUNT <= 512, "barriers");
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < TB_COUNT; ++i) mbar_init(bar(i), 1);
+        mbar_init(bar(TB_Q_FULL), 128);
+        mbar_init(bar(TB_K_FULL), 128);
+        mbar_init(bar(TB_V_FULL), 128);
+        mbar_init(bar(TB_PLO_FULL), 256);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(TB_P_FULL + i), 256);
+            mbar_init(bar(TB_O_EMPTY + i), 256);
+        }
+        mbar_fence_init();
+        s_gave_up = 0;
+        for (int i = 0; i < 4; ++i) s_odd[i] = 0;
+    }
+    constexpr TreeLine line = { TT_ROWS, KB };
+    TreeCursor cur;
+    if (!tree_start(a, line, s_line, cur)) return;
+    if (warp == 19) {
+        tmem_alloc(base + 544, C::COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+
+    // a wait that ran out anywhere stops every role: nobody loads or multiplies on arrivals that no longer mean anything
+    auto wait = [&](int i, uint32_t parity) -> bool { return mbar_wait_bounded(bar(i), parity) && !s_gave_up; };
+    auto wait_all = [&](int i, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, wait(i, parity) ? 1 : 0) != 0;
+    };
+    auto give_up = [&](int code) {
+        s_gave_up = 1;
+        if (a.err) atomicCAS(a.err, 0, code);
+    };
+    TreePiece p;
+    uint32_t it = 0;      // key blocks since the start
+    uint32_t np = 0;      // pieces since the start
+    const int heads_per = a.H / a.Hkv;
+    bool ok = true;
+
+    // registers: 640 threads x 96 at launch = 256 x 144 (softmax) + 384 x 64
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp < 18 && lane == 0) {
+            // -------------------------------------------------------- loads
+            const bool v = warp == 17;
+            const int stages = v ? C::VS : C::KS, b_raw = v ? TB_V_RAW : TB_K_RAW, b_empty = v ? TB_V_EMPTY : TB_K_EMPTY;
+            const void *map = v ? &tm.v : &tm.k;
+            tma_prefetch_desc(map);
+            while (ok && next_piece(a, line, cur, p)) {
+                const int head = p.b * a.Hkv + p.hk;
+                for (int i = 0; i < p.count; ++i, ++it) {
+                    const uint32_t s = it % stages, use = it / stages;
+                    if (use && !wait(b_empty + s, (use - 1) & 1)) { ok = false; break; }
+                    if (s_gave_up) { ok = false; break; }
+                    const int row = (p.t0 + i) * KB;
+                    const uint32_t dst = base + (v ? C::V_AT : C::K_AT) + s * C::PLANE;
+                    mbar_arrive_expect_tx(bar(b_raw + s), C::PLANE);
+#pragma unroll
+                    for (int sl = 0; sl < NSLAB; ++sl) tma_load_3d(dst + sl * C::SLAB, map, bar(b_raw + s), 32 * sl, row, head);
+                    if (i + stages < p.count) {   // the block that waits for a buffer: into L2 meanwhile
+#pragma unroll
+                        for (int sl = 0; sl < NSLAB; ++sl) tma_prefetch_3d(map, 32 * sl, row + stages * KB, head);
+                    }
+                }
+            }
+            if (!ok) {
+                give_up(CERR_LOAD);
+                for (uint32_t i = it > (uint32_t)stages ? it - stages : 0; i < it; ++i) mbar_wait_bounded(bar(b_raw + i % stages), (i / stages) & 1);
+            }
+        } else if (warp == 18 && lane == 0) {
+            // ----------------------------------------------------- scores
+            const uint32_t idesc = make_idesc<KIND_TF32>(TT_ROWS, KB);
+            while (ok && next_piece(a, line, cur, p)) {
+                if (!wait(TB_Q_FULL, np & 1)) { ok = false; break; }
+                ++np;
+                for (int i = 0; i < p.count; ++i, ++it) {
+                    const uint32_t b = it & 1;
+                    // score buffer b held P hi of block it - 2, the A operand of that block's product
+                    if (it >= 2 && !wait(TB_O_FULL + b, ((it - 2) >> 1) & 1)) { ok = false; break; }
+                    if (!wait(TB_K_FULL, it & 1)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    if (b) issue_scores<NSLAB, 1>(base, tmem, idesc, bar(TB_KLO_EMPTY));
+                    else issue_scores<NSLAB, 0>(base, tmem, idesc, bar(TB_KLO_EMPTY));
+                    tc_commit(bar(TB_S_FULL + b));
+                    tc_commit(bar(TB_K_EMPTY + it % C::KS));
+                    if (i == p.count - 1) tc_commit(bar(TB_Q_EMPTY));
+                }
+            }
+        } else if (warp == 19 && lane == 0) {
+            // ----------------------------------------------------- outputs
+            const uint32_t idesc = make_idesc<KIND_TF32>(TT_ROWS, (a.dk + 15) / 16 * 16) | (1u << 16);   // B is MN-major
+            while (ok && next_piece(a, line, cur, p)) {
+                for (int i = 0; i < p.count; ++i, ++it) {
+                    const uint32_t b = it & 1;
+                    if (!wait(TB_P_FULL + b, (it >> 1) & 1)) { ok = false; break; }
+                    if (!wait(TB_V_FULL, it & 1)) { ok = false; break; }
+                    if (it >= C::OB && !wait(TB_O_EMPTY + it % C::OB, (it / C::OB - 1) & 1)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    if (b) issue_outputs<NSLAB, 1, 0>(base, tmem, idesc, bar(TB_VLO_EMPTY));
+                    else issue_outputs<NSLAB, 0, 0>(base, tmem, idesc, bar(TB_VLO_EMPTY));
+                    if (!wait(TB_PLO_FULL, it & 1)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    if (b) issue_outputs<NSLAB, 1, 1>(base, tmem, idesc, 0);
+                    else issue_outputs<NSLAB, 0, 1>(base, tmem, idesc, 0);
+                    tc_commit(bar(TB_O_FULL + b));
+                    tc_commit(bar(TB_V_EMPTY + it % C::VS));
+                }
+            }
+        }
+        if (!ok && warp >= 18) {
+            give_up(CERR_MMA);
+            tc_commit(bar(TB_DRAIN + warp - 18));   // products in flight end before the tensor memory goes
+            mbar_wait_bounded(bar(TB_DRAIN + warp - 18), 0);
+        }
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        // ---------------------------------------------------------- lo parts
+        const bool v = warp >= 12;
+        const int ct = (threadIdx.x - 256) & 127;
+        const int stages = v ? C::VS : C::KS, b_raw = v ? TB_V_RAW : TB_K_RAW, b_full = v ? TB_V_FULL : TB_K_FULL;
+        while (ok && next_piece(a, line, cur, p)) {
+            if (!v) {
+                // the piece's query rows: row r of the key head is head r / n, token r % n
+#pragma unroll 1
+                for (int i0 = ct; i0 < TT_ROWS * (C::DKP / 4); i0 += 8 * 128) {   // (a multiple of 8 x 128 pieces)
+                    float4 x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {   // the loads of a batch in flight together
+                        const int i = i0 + e * 128, r = i / (C::DKP / 4), c = i - r * (C::DKP / 4), row = p.block * TT_ROWS + r;
+                        x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (row < p.s.rows && 4 * c < a.dk) {
+                            const int gh = row / p.s.n, tok = row - gh * p.s.n;
+                            x[e] = __ldg(reinterpret_cast<const float4 *>(a.Q + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk) + c);
+                        }
+                    }
+                    if (i0 == ct && np && !wait_all(TB_Q_EMPTY, (np - 1) & 1)) { ok = false; break; }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int i = i0 + e * 128, r = i / (C::DKP / 4), c = i - r * (C::DKP / 4);
+                        uint8_t *dst = sm + C::Q_AT + (c >> 3) * C::QSLAB + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                        *reinterpret_cast<float4 *>(dst) = x[e];
+                        if (!C::WIDE)
+                            *reinterpret_cast<uint4 *>(dst + C::QPLANE) = make_uint4(lo_bits(__float_as_uint(x[e].x)), lo_bits(__float_as_uint(x[e].y)),
+                                                                                     lo_bits(__float_as_uint(x[e].z)), lo_bits(__float_as_uint(x[e].w)));
+                    }
+                }
+                if (!ok) break;
+                if (C::WIDE) {
+                    asm volatile("bar.sync 6, 128;" ::: "memory");
+                    // thread = row: lane of tensor memory
+                    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::T_QLO;
+#pragma unroll 1
+                    for (int sl = 0; sl < NSLAB; ++sl) {
+                        uint32_t r32[32];
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const uint4 x = *reinterpret_cast<const uint4 *>(sm + C::Q_AT + sl * C::QSLAB + ct * 128 + ((c ^ (ct & 7)) << 4));
+                            r32[4 * c] = lo_bits(x.x); r32[4 * c + 1] = lo_bits(x.y); r32[4 * c + 2] = lo_bits(x.z); r32[4 * c + 3] = lo_bits(x.w);
+                        }
+                        tmem_st_32x32(at + 32 * sl, r32);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before_sync();
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(bar(TB_Q_FULL));
+                ++np;
+            }
+            for (int i = 0; i < p.count; ++i, ++it) {
+                const uint32_t s = it % stages, use = it / stages;
+                if (!wait_all(b_raw + s, use & 1)) { ok = false; break; }
+                // the lo tile is single: the product of the block before that reads it (the first of the three) must be done
+                if (it && !wait_all(v ? TB_VLO_EMPTY : TB_KLO_EMPTY, (it - 1) & 1)) { ok = false; break; }
+                const int key0 = (p.t0 + i) * KB;
+                bool odd = false;
+                if (v && key0 + KB > p.s.len) {
+                    // rows behind the last one hold anything, and rows that only some tokens see must not reach the others through
+                    // 0 * inf: such values leave the product
+#pragma unroll 1
+                    for (int c = ct; c < C::PLANE / 16; c += 128) {
+                        const int j = key0 + (c >> 3) % KB - p.s.len;   // rows are 128 bytes whatever the swizzle
+                        if (j < 0) continue;
+                        uint4 *at = reinterpret_cast<uint4 *>(sm + C::V_AT + s * C::PLANE) + c;
+                        uint4 x = *at;
+                        uint32_t *w = &x.x;
+                        bool change = false;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (j >= p.s.n || !finite_f(__uint_as_float(w[e]))) {
+                                odd = odd || j < p.s.n;
+                                change = true;
+                                w[e] = 0;
+                            }
+                        if (change) *at = x;
+                    }
+                }
+                const uint4 *src = reinterpret_cast<const uint4 *>(sm + (v ? C::V_AT : C::K_AT) + s * C::PLANE) + ct;
+                uint4 *lo = reinterpret_cast<uint4 *>(sm + (v ? C::VLO_AT : C::KLO_AT)) + ct;
+                constexpr int PART = C::PLANE / 16 % (8 * 128) ? 4 : 8;
+                static_assert(C::PLANE / 16 % (PART * 128) == 0, "whole batches");
+#pragma unroll 1
+                for (int c = 0; c < C::PLANE / 16; c += PART * 128) {   // (a thread meets the chunks it changed above)
+                    uint4 x[PART];
+#pragma unroll
+                    for (int e = 0; e < PART; ++e) x[e] = src[c + e * 128];
+#pragma unroll
+                    for (int e = 0; e < PART; ++e) lo[c + e * 128] = make_uint4(lo_bits(x[e].x), lo_bits(x[e].y), lo_bits(x[e].z), lo_bits(x[e].w));
+                }
+                // (the word's last reader folded block it - 4: the product of block it - 1, which has begun, had to wait for the
+                // accumulator of block it - 2 or it - 3)
+                if (odd) s_odd[it & 3] = (int)it + 1;
+                fence_proxy_async_smem();
+                mbar_arrive(bar(b_full));
+            }
+        }
+        if (!ok && lane == 0) give_up(CERR_CONVERT);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+        // ---------------------------------------------------------- softmax
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane;   // row = lane of tensor memory
+        const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };   // the two warps of 32 rows
+        auto all_sync = [&] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        float o[OH], m, l;
+        while (next_piece(a, line, cur, p)) {
+            const int r = p.block * TT_ROWS + row, gh = r / p.s.n, tok = r < p.s.rows ? r - gh * p.s.n : 0;
+            const bool mine = r < p.s.rows;
+            m = -INFINITY;
+            l = 0.f;
+#pragma unroll
+            for (int c = 0; c < OH; ++c) o[c] = 0.f;
+            // o = (o + O of block jt) * f, jt the block before `it`
+            auto fold = [&](uint32_t jt, int key0, float f) {
+                tc_fence_after_sync();
+                const bool odd = s_odd[jt & 3] == (int)jt + 1;
+#pragma unroll
+                for (int h = 0; h < OH / 16; ++h) {
+                    uint32_t x[16];
+                    tmem_ld_32x32_x16(lane_base + C::T_O + (jt % C::OB) * C::DKP + half * OH + 16 * h, x);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) o[16 * h + c] += __uint_as_float(x[c]);
+                }
+                tc_fence_before_sync();
+                mbar_arrive(bar(TB_O_EMPTY + jt % C::OB));
+                if (odd && mine) {
+                    // rare: an infinity or a NaN among the new rows' values goes to the rows that see it, and to no others
+#pragma unroll 1
+                    for (int key = key0; key < key0 + KB; ++key) {
+                        const int j = key - p.s.len;
+                        if (j < 0 || j >= p.s.n || !tree_sees(a, p.b, tok, j)) continue;
+                        const float *src = a.V + (((int64_t)p.b * a.Hkv + p.hk) * a.max_seq + key) * a.dk + half * OH;
+#pragma unroll
+                        for (int c = 0; c < OH; ++c)
+                            if (half * OH + c < a.dk) {
+                                const float x = __ldg(src + c);
+                                if (!finite_f(x)) o[c] += x;
+                            }
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < OH; ++c) o[c] *= f;
+            };
+            for (int i = 0; i < p.count; ++i, ++it) {
+                const uint32_t b = it & 1;
+                const int key0 = (p.t0 + i) * KB;
+                const uint32_t s_addr = lane_base + C::T_S + b * KB + half * (KB / 2), lo_addr = lane_base + C::T_PLO + half * (KB / 2);
+                const int first = key0 + half * (KB / 2) - p.s.len;   // new-token index of this thread's first column
+                const bool tail = first + KB / 2 > 0;
+                if (ok && !wait_all(TB_S_FULL + b, (it >> 1) & 1)) ok = false;
+                float mx = -INFINITY;
+                if (ok) {
+                    tc_fence_after_sync();
+                    float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+#pragma unroll 1
+                    for (int c0 = 0; c0 < KB / 2; c0 += 32) {
+                        uint32_t x[32];
+                        tmem_ld_32x32(s_addr + c0, x);
+                        tmem_ld_wait();
+                        const uint32_t see = tail ? seen_bits(a, p.b, tok, p.s.n, first + c0) : 0xFFFFFFFFu;
+                        if (see == 0xFFFFFFFFu) {
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(x[c]) * a.c_log2);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 32; ++c)
+                                if (see >> c & 1) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(x[c]) * a.c_log2);
+                        }
+                    }
+                    mx = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                }
+                s_max[b][half][row] = mx;
+                pair_sync();
+                if (!ok) continue;
+                mx = fmaxf(mx, s_max[b][half ^ 1][row]);
+                float corr = 1.f;
+                if (mx > m + 8.f) {
+                    corr = ex2_approx(m - mx);   // 0 the first time
+                    m = mx;
+                }
+                const float neg = m == -INFINITY ? 0.f : -m;
+                float sum[4] = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll 1
+                for (int c0 = 0; c0 < KB / 2; c0 += 32) {
+                    uint32_t x[32];
+                    tmem_ld_32x32(s_addr + c0, x);
+                    tmem_ld_wait();
+                    const uint32_t see = tail ? seen_bits(a, p.b, tok, p.s.n, first + c0) : 0xFFFFFFFFu;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        float e = ex2_approx(fmaf(__uint_as_float(x[c]), a.c_log2, neg));
+                        if (!(see >> c & 1)) e = 0.f;
+                        sum[c & 3] += e;
+                        x[c] = __float_as_uint(e);
+                    }
+                    tmem_st_32x32(s_addr + c0, x);
+                }
+                tmem_st_wait();
+                l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                tc_fence_before_sync();
+                mbar_arrive(bar(TB_P_FULL + b));   // P hi: two of the three products can start
+                // P lo is a single buffer: the product of the block before must have read it
+                if (i > 0) {
+                    if (!wait_all(TB_O_FULL + (b ^ 1), ((it - 1) >> 1) & 1)) { ok = false; continue; }
+                    if (C::OB == 1) fold(it - 1, key0 - KB, corr);   // the single accumulator has to be free for this block's product
+                }
+#pragma unroll 1
+                for (int c0 = 0; c0 < KB / 2; c0 += 32) {
+                    uint32_t x[32];
+                    tmem_ld_32x32(s_addr + c0, x);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) x[c] = lo_bits(x[c]);
+                    tmem_st_32x32(lo_addr + c0, x);
+                }
+                tmem_st_wait();
+                tc_fence_before_sync();
+                mbar_arrive(bar(TB_PLO_FULL));
+                if (i > 0 && C::OB == 2) fold(it - 1, key0 - KB, corr);
+            }
+            if (ok) {
+                if (wait_all(TB_O_FULL + ((it - 1) & 1), ((it - 1) >> 1) & 1)) fold(it - 1, (p.t0 + p.count - 1) * KB, 1.f);
+                else ok = false;
+            }
+            s_max[(it - 1) & 1][half][row] = l;   // (the last block's maxima have been read: its product had to wait for that)
+            pair_sync();
+            l += s_max[(it - 1) & 1][half ^ 1][row];
+
+            // pieces of a shared item: [16-byte column][row] outputs, then [row] (maximum, sum).  Up to GROUP pieces are added by
+            // the CTA that arrives last; more in groups first, whose sums take the place of the group's first piece.
+            constexpr int GROUP = 12;
+            auto slot = [&](int cta) {
+                return reinterpret_cast<float4 *>(a.slots) + (size_t)tree_slot(cta, cta == p.first) * (KT_SLOT_BYTES / 16);
+            };
+            auto put = [&](float4 *s) {
+#pragma unroll
+                for (int c = 0; c < OH / 4; ++c)
+                    s[(half * (OH / 4) + c) * TT_ROWS + row] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                if (half == 0) reinterpret_cast<float2 *>(s + C::DKP / 4 * TT_ROWS)[row] = make_float2(m, l);
+            };
+            auto arrive_last = [&](int *counter, int of) -> bool {
+                __threadfence();
+                all_sync();
+                if (threadIdx.x == 0) {
+                    s_last = atomicAdd(counter, 1) == of - 1;
+                    if (s_last) *counter = 0;
+                }
+                all_sync();
+                const bool last = s_last != 0;
+                __threadfence();
+                return last;
+            };
+            auto add_up = [&](int from, int to, int step) {   // pieces first + from, first + from + step, ... in line order
+                m = -INFINITY;
+                l = 0.f;
+#pragma unroll
+                for (int c = 0; c < OH; ++c) o[c] = 0.f;
+#pragma unroll 1
+                for (int k = from; k < to; k += step) {
+                    const float4 *s = slot(p.first + k);
+                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(s + C::DKP / 4 * TT_ROWS) + row);
+                    const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
+                    const float f0 = ex2_approx(m - ref), f1 = ex2_approx(ml.x - ref);
+                    m = m_new;
+                    l = l * f0 + ml.y * f1;
+#pragma unroll
+                    for (int c = 0; c < OH / 4; ++c) {
+                        const float4 x = __ldcg(s + (half * (OH / 4) + c) * TT_ROWS + row);
+                        o[4 * c] = o[4 * c] * f0 + x.x * f1;
+                        o[4 * c + 1] = o[4 * c + 1] * f0 + x.y * f1;
+                        o[4 * c + 2] = o[4 * c + 2] * f0 + x.z * f1;
+                        o[4 * c + 3] = o[4 * c + 3] * f0 + x.w * f1;
+                    }
+                }
+            };
+            bool write = p.pieces == 1;
+            if (!write) {
+                const int k = (int)blockIdx.x - p.first;
+                put(slot(blockIdx.x));
+                if (p.pieces <= GROUP) {
+                    write = arrive_last(a.counters + p.first, p.pieces);
+                    if (write) add_up(0, p.pieces, 1);
+                } else {
+                    // counters: [items by first CTA][first groups by first CTA][other groups by their first CTA]
+                    const int g0 = k / GROUP * GROUP, in_group = p.pieces - g0 < GROUP ? p.pieces - g0 : GROUP;
+                    if (arrive_last(a.counters + (g0 ? 2 : 1) * gridDim.x + p.first + g0, in_group)) {
+                        add_up(g0, g0 + in_group, 1);
+                        put(slot(p.first + g0));   // (each thread wrote over what it alone had read)
+                        write = arrive_last(a.counters + p.first, (p.pieces + GROUP - 1) / GROUP);
+                        if (write) add_up(0, p.pieces, GROUP);
+                    }
+                }
+            }
+            if (write && mine) {
+                float *dst = a.out + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk + half * OH;
+                const float inv = l == 0.f ? 0.f : 1.0f / l;   // nothing seen: 0
+#pragma unroll
+                for (int c = 0; c < OH; c += 4)
+                    if (half * OH + c < a.dk)
+                        *reinterpret_cast<float4 *>(dst + c) = make_float4(o[c] * inv, o[c + 1] * inv, o[c + 2] * inv, o[c + 3] * inv);
+            }
+        }
+        if (!ok && lane == 0) give_up(CERR_SOFTMAX);
+    }
+
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 19) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, C::COLS);
+    }
+}
+
+// ---------------------------------------------------------------------- host
+
+template <int NSLAB>
+static int launch_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st)
+{
+    using C = TreeTc<NSLAB>;
+    static PerDeviceOnce once;
+    if (once.first()) {
+        cudaError_t e = cudaFuncSetAttribute(kv_tree_tc_kernel<NSLAB>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return (int)e;
+    }
+    TreeTcMaps tm;
+    int e = encode_f32_batched_tmap(&tm.k, a.K, (int64_t)a.B * a.Hkv, a.max_seq, a.dk, a.dk, C::KB, false);
+    if (!e) e = encode_f32_batched_tmap(&tm.v, a.V, (int64_t)a.B * a.Hkv, a.max_seq, a.dk, a.dk, C::KB, true);
+    if (e) return e;
+    kv_tree_tc_kernel<NSLAB><<<sm_count, TT_THREADS, C::SMEM, st>>>(a, tm);
+    return (int)cudaGetLastError();
+}
+
+int launch_kv_tree_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st)
+{
+    if (a.dk <= 32) return launch_tc<1>(a, sm_count, st);
+    if (a.dk <= 64) return launch_tc<2>(a, sm_count, st);
+    if (a.dk <= 96) return launch_tc<3>(a, sm_count, st);
+    return launch_tc<4>(a, sm_count, st);
+}
+
+}  // namespace axb

@@ -92,6 +92,17 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity)
     }
 }
 
+// The same bounded by a number of polls instead of the timer, with a short sleep between them (about a second in all).
+__device__ __forceinline__ bool mbar_poll_bounded(uint32_t bar, uint32_t parity)
+{
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 24); ++i) {
+        if (mbar_test_wait(bar, parity)) return true;
+        __nanosleep(40);
+    }
+    return false;
+}
+
 // Whole-warp wait for warps that wait long (epilogue warps wait a whole K loop): only lane 0
 // polls, with a sleep between polls, so the waiters do not compete with the MMA-issuing
 // thread for the barrier unit; the outcome is broadcast to the warp.
@@ -228,6 +239,17 @@ __device__ __forceinline__ void tmem_ld_32x32_x8(uint32_t taddr, uint32_t (&r)[8
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
+// The same for 16 consecutive columns.
+__device__ __forceinline__ void tmem_ld_32x32_x16(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr)
                  : "memory");
 }

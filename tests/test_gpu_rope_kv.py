@@ -318,6 +318,17 @@ ATTEND = [
     (40, 2, 2, 1, 64, list(range(0, 400, 10)), True, "tree"),
     (1, 4, 2, 1, 128, [40000], False, "tree"),
     (7, 3, 16, 8, 64, [5000, 0, 1, 2, 3, 64, 4000], True, None),
+    # more than 32 query rows to a key head: 128-row blocks
+    (2, 1, 64, 1, 64, [300, 1000], False, None),
+    (2, 3, 12, 1, 32, [0, 129], True, "tree"),
+    (3, 33, 2, 2, 128, [63, 64, 0], True, "tree"),
+    (1, 40, 2, 1, 64, [30000], False, "tree"),           # one item over every CTA
+    (1, 40, 1, 1, 128, [12000], False, "shared"),
+    (1, 300, 2, 1, 96, [200], False, None),
+    (1, 200, 6, 2, 64, [0], False, None),
+    (5, 17, 8, 4, 100, [1, 500, 0, 77, 128], True, "tree"),
+    (3, 64, 4, 2, 128, [4000, 10, 900], True, "shared"),
+    (1, 513, 1, 1, 64, [100], False, None),
 ]
 
 
@@ -342,7 +353,8 @@ def run_attend(engine, s, **more):
 
 def check_attend(s, got, magnitudes=None):
     want, smag, vmag = ref.attend_tree(s["K"], s["V"], s["Q"], s["out"], s["lens"], s["scale"], s["n_new"], s["mask"])
-    assert float((got.double() - want).abs().max()) <= ref.attend_bound(smag, vmag, s["Q"].shape[-1])
+    err, bound = float((got.double() - want).abs().max()), ref.attend_bound(smag, vmag, s["Q"].shape[-1])
+    assert err <= bound
     B, T = s["lens"].numel(), s["Q"].shape[1]
     if s["n_new"] is not None:         # rows behind the last token keep their bits
         behind = (torch.arange(T, device="cuda")[None, :] >= s["n_new"][:, None])[:, None, :, None].expand(B, s["Q"].shape[0] // B, T, s["Q"].shape[2])
@@ -385,8 +397,9 @@ def test_rows_that_see_nothing_are_zero(engine, lens):
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), torch.finfo(torch.float32).max])
-@pytest.mark.parametrize("case", [(2, 6, 4, 2, 64, [59, 130], False, "tree"), (2, 40, 4, 2, 128, [59, 130], True, "tree"), (1, 20, 2, 1, 50, [3], False, "tree")],
-                         ids=["few", "many", "scalar"])
+@pytest.mark.parametrize("case", [(2, 6, 4, 2, 64, [59, 130], False, "tree"), (2, 40, 4, 2, 128, [59, 130], True, "tree"), (1, 20, 2, 1, 50, [3], False, "tree"),
+                                  (2, 40, 4, 2, 64, [59, 130], True, "tree"), (1, 140, 2, 2, 96, [200], False, "tree")],
+                         ids=["few", "many", "scalar", "many64", "blocks"])
 def test_values_in_unseen_rows_reach_nobody(engine, case, bad):
     """Anything in cache rows behind the last token and in new rows that a token does not see leaves its result alone, bit for
     bit; a token that does see such a row becomes non-finite (or huge) in the columns concerned."""
