@@ -8,9 +8,9 @@
 //         written over the scores in tensor memory, P lo beside them: both are the A operand of P.V as they lie.  The
 //         exponent's reference stays until a score passes it by 2^8; every block's P.V starts from zero and is folded into
 //         fp32 registers, so the tensor core's truncating accumulation never spans more than a block.
-//   8-11  Q of a piece (gathered rows -> swizzled shared memory, lo part there or, for head dims above 64, in tensor
-//         memory), then the lo part of every K block;   12-15  the lo part of every V block, and what must not reach the
-//         product: rows behind the last token, and infinities or NaN in new rows (those are added row by row).
+//   8-15  Q of a piece (gathered rows -> swizzled shared memory, lo part there or, for head dims above 64, in tensor
+//         memory), the lo parts of the K and V blocks, and what must not reach the V product: rows behind the last token,
+//         and infinities or NaN in new rows (those are added row by row);
 //   16, 17  TMA of K and V (the operand whose chain is the longer one has two raw buffers: V for head dims up to 64, K above);
 //   18, 19  one thread each issues the score and the P.V products.
 // Shared memory is full either way (224 KB): Q 64 KB, five K / V tiles of 32 KB.  A block costs the same for one row or 128; up to
@@ -136,23 +136,24 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     extern __shared__ __align__(1024) uint8_t sm[];
     const uint32_t base = smem_u32(sm);
     auto bar = [&](int i) -> uint32_t { return base + 8u * (uint32_t)i; };
-    unsigned long long *s_line = reinterpret_cast<unsigned long long *>(sm + 512);
-    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(sm + 544);
-    volatile int *words = reinterpret_cast<volatile int *>(sm + 560);
+    unsigned long long *s_line = reinterpret_cast<unsigned long long *>(sm + 256);
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(sm + 288);
+    volatile int *words = reinterpret_cast<volatile int *>(sm + 304);
     volatile int &s_gave_up = words[0], &s_last = words[1], *s_odd = words + 2;   // s_odd: block it + 1 holds non-finite new values
+    int *s_row = reinterpret_cast<int *>(sm + 512);   // [TT_ROWS]
     float (*s_max)[2][TT_ROWS] = reinterpret_cast<float (*)[2][TT_ROWS]>(sm + 1024);   // [block parity][half][row]
     if (base & 1023) {   // the swizzles are functions of the address (it starts at a multiple of 1 KB; refused, should it ever not)
         if (threadIdx.x == 0 && a.err) atomicCAS(a.err, 0, (int)CERR_LOAD);
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    static_assert(8 * TB_COUNT <= 512, "barriers");
+    static_assert(8 * TB_COUNT <= 256, "barriers");
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < TB_COUNT; ++i) mbar_init(bar(i), 1);
-        mbar_init(bar(TB_Q_FULL), 128);
-        mbar_init(bar(TB_K_FULL), 128);
-        mbar_init(bar(TB_V_FULL), 128);
+        mbar_init(bar(TB_Q_FULL), 256);
+        mbar_init(bar(TB_K_FULL), 256);
+        mbar_init(bar(TB_V_FULL), 256);
         mbar_init(bar(TB_PLO_FULL), 256);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(TB_P_FULL + i), 256);
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;
     if (warp == 19) {
-        tmem_alloc(base + 544, C::COLS);
+        tmem_alloc(base + 288, C::COLS);
         tmem_relinquish();
     }
     tc_fence_before_sync();
@@ -266,40 +267,80 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
         }
     } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        // ---------------------------------------------------------- lo parts
-        const bool v = warp >= 12;
-        const int ct = (threadIdx.x - 256) & 127;
-        const int stages = v ? C::VS : C::KS, b_raw = v ? TB_V_RAW : TB_K_RAW, b_full = v ? TB_V_FULL : TB_K_FULL;
-        while (ok && next_piece(a, line, cur, p)) {
-            if (!v) {
-                // the piece's query rows: row r of the key head is head r / n, token r % n
+        // ------------------------------------------------- Q, and the lo parts of K and V
+        const int ct = threadIdx.x - 256;   // 0..255
+        auto conv_sync = [] { asm volatile("bar.sync 6, 256;" ::: "memory"); };
+        auto split = [&](const uint4 *src, uint4 *lo) {
+            constexpr int PART = C::PLANE / 16 % (4 * 256) ? 2 : 4;
+            static_assert(C::PLANE / 16 % (PART * 256) == 0, "whole batches");
 #pragma unroll 1
-                for (int i0 = ct; i0 < TT_ROWS * (C::DKP / 4); i0 += 8 * 128) {   // (a multiple of 8 x 128 pieces)
-                    float4 x[8];
+            for (int c = ct; c < C::PLANE / 16; c += PART * 256) {
+                uint4 x[PART];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {   // the loads of a batch in flight together
-                        const int i = i0 + e * 128, r = i / (C::DKP / 4), c = i - r * (C::DKP / 4), row = p.block * TT_ROWS + r;
-                        x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (row < p.s.rows && 4 * c < a.dk) {
-                            const int gh = row / p.s.n, tok = row - gh * p.s.n;
-                            x[e] = __ldg(reinterpret_cast<const float4 *>(a.Q + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk) + c);
+                for (int e = 0; e < PART; ++e) x[e] = src[c + e * 256];
+#pragma unroll
+                for (int e = 0; e < PART; ++e) lo[c + e * 256] = make_uint4(lo_bits(x[e].x), lo_bits(x[e].y), lo_bits(x[e].z), lo_bits(x[e].w));
+            }
+        };
+        // the lo tiles are single: the product of the block before that reads them (the first of its three) must be done
+        auto ready = [&](int i, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_test_wait(bar(i), parity) ? 1 : 0) != 0; };
+        auto do_k = [&](uint32_t jt) {
+            split(reinterpret_cast<const uint4 *>(sm + C::K_AT + (jt % C::KS) * C::PLANE), reinterpret_cast<uint4 *>(sm + C::KLO_AT));
+            fence_proxy_async_smem();
+            mbar_arrive(bar(TB_K_FULL));
+        };
+        auto do_v = [&](uint32_t jt, int key0) {
+            uint4 *tile = reinterpret_cast<uint4 *>(sm + C::V_AT + (jt % C::VS) * C::PLANE);
+            bool odd = false;
+            if (key0 + KB > p.s.len) {
+                // rows behind the last one hold anything, and rows that only some tokens see must not reach the others through
+                // 0 * inf: such values leave the product
+#pragma unroll 1
+                for (int c = ct; c < C::PLANE / 16; c += 256) {
+                    const int j = key0 + (c >> 3) % KB - p.s.len;   // rows are 128 bytes whatever the swizzle
+                    if (j < 0) continue;
+                    uint4 x = tile[c];
+                    uint32_t *w = &x.x;
+                    bool change = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (j >= p.s.n || !finite_f(__uint_as_float(w[e]))) {
+                            odd = odd || j < p.s.n;
+                            change = true;
+                            w[e] = 0;
                         }
-                    }
-                    if (i0 == ct && np && !wait_all(TB_Q_EMPTY, (np - 1) & 1)) { ok = false; break; }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int i = i0 + e * 128, r = i / (C::DKP / 4), c = i - r * (C::DKP / 4);
-                        uint8_t *dst = sm + C::Q_AT + (c >> 3) * C::QSLAB + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                        *reinterpret_cast<float4 *>(dst) = x[e];
-                        if (!C::WIDE)
-                            *reinterpret_cast<uint4 *>(dst + C::QPLANE) = make_uint4(lo_bits(__float_as_uint(x[e].x)), lo_bits(__float_as_uint(x[e].y)),
-                                                                                     lo_bits(__float_as_uint(x[e].z)), lo_bits(__float_as_uint(x[e].w)));
-                    }
+                    if (change) tile[c] = x;
                 }
-                if (!ok) break;
-                if (C::WIDE) {
-                    asm volatile("bar.sync 6, 128;" ::: "memory");
-                    // thread = row: lane of tensor memory
+            }
+            split(tile, reinterpret_cast<uint4 *>(sm + C::VLO_AT));   // (a thread meets the pieces it changed)
+            // (the word's last reader folded block jt - 4: the product of block jt - 1, which has begun, had to wait for the
+            // accumulator of block jt - 2 or jt - 3)
+            if (odd) s_odd[jt & 3] = (int)jt + 1;
+            fence_proxy_async_smem();
+            mbar_arrive(bar(TB_V_FULL));
+        };
+        while (ok && next_piece(a, line, cur, p)) {
+            if (np && !wait_all(TB_Q_EMPTY, (np - 1) & 1)) { ok = false; break; }
+            ++np;
+            // the piece's query rows: row r of the key head is head r / n, token r % n.  s_row: rows of Q from the key head's first
+            if (ct < TT_ROWS) {
+                const int r = p.block * TT_ROWS + ct, gh = r / p.s.n;
+                s_row[ct] = r < p.s.rows ? gh * a.T + (r - gh * p.s.n) : -1;
+            }
+            conv_sync();
+            const float *q0 = a.Q + ((int64_t)p.b * a.H + p.hk * heads_per) * a.T * a.dk;
+#pragma unroll 4
+            for (int i = ct; i < TT_ROWS * (C::DKP / 4); i += 256) {
+                const int r = i / (C::DKP / 4), c = i - r * (C::DKP / 4), row = s_row[r];
+                const bool get = row >= 0 && 4 * c < a.dk;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + C::Q_AT + (c >> 3) * C::QSLAB + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                             "l"(get ? q0 + (int64_t)row * a.dk + 4 * c : a.Q), "r"(get ? 16 : 0)
+                             : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (C::WIDE) {
+                conv_sync();
+                if (ct < TT_ROWS) {   // thread = row: lane of tensor memory
                     const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::T_QLO;
 #pragma unroll 1
                     for (int sl = 0; sl < NSLAB; ++sl) {
@@ -314,56 +355,35 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
                     tmem_st_wait();
                     tc_fence_before_sync();
                 }
-                fence_proxy_async_smem();
-                mbar_arrive(bar(TB_Q_FULL));
-                ++np;
-            }
-            for (int i = 0; i < p.count; ++i, ++it) {
-                const uint32_t s = it % stages, use = it / stages;
-                if (!wait_all(b_raw + s, use & 1)) { ok = false; break; }
-                // the lo tile is single: the product of the block before that reads it (the first of the three) must be done
-                if (it && !wait_all(v ? TB_VLO_EMPTY : TB_KLO_EMPTY, (it - 1) & 1)) { ok = false; break; }
-                const int key0 = (p.t0 + i) * KB;
-                bool odd = false;
-                if (v && key0 + KB > p.s.len) {
-                    // rows behind the last one hold anything, and rows that only some tokens see must not reach the others through
-                    // 0 * inf: such values leave the product
-#pragma unroll 1
-                    for (int c = ct; c < C::PLANE / 16; c += 128) {
-                        const int j = key0 + (c >> 3) % KB - p.s.len;   // rows are 128 bytes whatever the swizzle
-                        if (j < 0) continue;
-                        uint4 *at = reinterpret_cast<uint4 *>(sm + C::V_AT + s * C::PLANE) + c;
-                        uint4 x = *at;
-                        uint32_t *w = &x.x;
-                        bool change = false;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (j >= p.s.n || !finite_f(__uint_as_float(w[e]))) {
-                                odd = odd || j < p.s.n;
-                                change = true;
-                                w[e] = 0;
-                            }
-                        if (change) *at = x;
-                    }
+            } else {
+#pragma unroll 4
+                for (int i = ct; i < TT_ROWS * (C::DKP / 4); i += 256) {   // (the pieces this thread brought)
+                    const int r = i / (C::DKP / 4), c = i - r * (C::DKP / 4);
+                    uint8_t *at = sm + C::Q_AT + (c >> 3) * C::QSLAB + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    const uint4 x = *reinterpret_cast<const uint4 *>(at);
+                    *reinterpret_cast<uint4 *>(at + C::QPLANE) = make_uint4(lo_bits(x.x), lo_bits(x.y), lo_bits(x.z), lo_bits(x.w));
                 }
-                const uint4 *src = reinterpret_cast<const uint4 *>(sm + (v ? C::V_AT : C::K_AT) + s * C::PLANE) + ct;
-                uint4 *lo = reinterpret_cast<uint4 *>(sm + (v ? C::VLO_AT : C::KLO_AT)) + ct;
-                constexpr int PART = C::PLANE / 16 % (8 * 128) ? 4 : 8;
-                static_assert(C::PLANE / 16 % (PART * 128) == 0, "whole batches");
-#pragma unroll 1
-                for (int c = 0; c < C::PLANE / 16; c += PART * 128) {   // (a thread meets the chunks it changed above)
-                    uint4 x[PART];
-#pragma unroll
-                    for (int e = 0; e < PART; ++e) x[e] = src[c + e * 128];
-#pragma unroll
-                    for (int e = 0; e < PART; ++e) lo[c + e * 128] = make_uint4(lo_bits(x[e].x), lo_bits(x[e].y), lo_bits(x[e].z), lo_bits(x[e].w));
-                }
-                // (the word's last reader folded block it - 4: the product of block it - 1, which has begun, had to wait for the
-                // accumulator of block it - 2 or it - 3)
-                if (odd) s_odd[it & 3] = (int)it + 1;
-                fence_proxy_async_smem();
-                mbar_arrive(bar(b_full));
             }
+            fence_proxy_async_smem();
+            mbar_arrive(bar(TB_Q_FULL));
+            // K and V blocks in whichever order they can be taken (every warp for itself: its part of a tile is its own)
+            uint32_t kt = it, vt = it;
+            const uint32_t end = it + p.count;
+            for (uint32_t idle = 0; ok && (kt < end || vt < end);) {
+                if (kt < end && ready(TB_K_RAW + kt % C::KS, (kt / C::KS) & 1) && (!kt || ready(TB_KLO_EMPTY, (kt - 1) & 1))) {
+                    do_k(kt++);
+                    idle = 0;
+                } else if (vt < end && ready(TB_V_RAW + vt % C::VS, (vt / C::VS) & 1) && (!vt || ready(TB_VLO_EMPTY, (vt - 1) & 1))) {
+                    do_v(vt, (p.t0 + (int)(vt - it)) * KB);
+                    ++vt;
+                    idle = 0;
+                } else {
+                    __nanosleep(20);
+                    ok = ++idle < (1u << 24) && !s_gave_up;
+                    ok = __all_sync(0xffffffffu, ok);
+                }
+            }
+            it = end;
         }
         if (!ok && lane == 0) give_up(CERR_CONVERT);
     } else {
