@@ -28,7 +28,8 @@
 // last) and clears the counter.
 //
 // One CTA per SM: two producer warps feed K and V tiles through a ring; eight warps each take 16 keys of a tile with
-// a running softmax of their own, merged in registers through shared memory at the end of a piece.
+// a running softmax of their own, added up at the end of a piece — up to 8 rows (16 of narrower heads) by a merger warp
+// while the eight are at the next piece, which a scout warp has prepared.
 #include "kv_tree.cuh"
 
 #include "errors.cuh"
@@ -51,18 +52,26 @@ struct TreeCfg {
     static constexpr int SLICES = KT_KEYS / 16;                       // warps side by side on a tile's keys
     static constexpr int GROUPS = KT_CONSUMERS / SLICES;              // tiles in work at the same time
     static constexpr int FRAGS = DKP / 16 * NR;                       // float4 of a lane's O^T
+    // Decode and small trees (ASYNC): a scout warp prepares the next piece (its place in the batch, its Q) and a merger warp
+    // adds up and writes the finished one while the consumers go on; otherwise the consumers do both themselves, between
+    // barriers (each costs a piece some 7,000 cycles, in which the ring stands still).
+    static constexpr bool ASYNC = NR == 1 || (NR == 2 && DKP <= 96);
     static constexpr bool SPLIT_Q = NR < 4;                           // Q lies in shared memory as hi and lo
     static constexpr int TILE = KT_KEYS * DKP * 4;                    // bytes of a K or V tile
     static constexpr int Q_BYTES = ROWS * DKP * 4 * (SPLIT_Q ? 2 : 1);
-    static constexpr int MERGE_BYTES = KT_CONSUMERS / 2 * 32 * (FRAGS + NR) * 16;
-    static constexpr int AREA = Q_BYTES > MERGE_BYTES ? Q_BYTES : MERGE_BYTES;   // first Q, then the merge
-    static constexpr int ROOM = (224 * 1024 - AREA) / (2 * TILE);
-    static constexpr int STAGES = ROOM < 8 ? ROOM : 8;
+    static constexpr int PART_BYTES = 32 * (FRAGS + NR) * 16;         // a warp's partial result
+    static constexpr int MERGE_BYTES = KT_CONSUMERS / (ASYNC ? 1 : 2) * PART_BYTES;
+    static constexpr int AREA = ASYNC ? 2 * Q_BYTES + MERGE_BYTES : Q_BYTES > MERGE_BYTES ? Q_BYTES : MERGE_BYTES;   // else first Q, then the merge
+    // A stage always belongs to the same group of warps: a barrier's phases are then waited for in order by the same threads.
+    // (Four stages carry HBM's rate, six were slower: 90 against 95 us for 537 MB.)
+    static constexpr int ROOM = (224 * 1024 - AREA) / (2 * TILE) / GROUPS * GROUPS;
+    static constexpr int STAGES = ROOM < 2 * GROUPS && ROOM > 0 ? ROOM : TILE <= 8192 ? 2 * GROUPS : GROUPS;
+    static_assert(STAGES % GROUPS == 0 && STAGES <= ROOM, "ring");
     static constexpr int SMEM = 1024 + STAGES * 2 * TILE + AREA;
-    // four rows in eights and 128 columns need more than the 168 registers that ten warps leave a thread: with twelve
-    // warps the producer's four hand theirs to the consumers
-    static constexpr bool SHIFT_REGS = NR == 4 || (NR == 2 && DKP == 128);
-    static constexpr int THREADS = (KT_CONSUMERS + (SHIFT_REGS ? 4 : 2)) * 32;
+    // four rows in eights and 128 columns need more than the 168 registers that twelve warps leave a thread: the four
+    // others hand theirs to the consumers
+    static constexpr bool SHIFT_REGS = !ASYNC;
+    static constexpr int THREADS = (KT_CONSUMERS + 4) * 32;
 };
 
 struct TreeMaps {
@@ -343,37 +352,200 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
     using C = TreeCfg<DKP, NR>;
     constexpr int ROWS = C::ROWS;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ alignas(8) uint64_t bars[6 * C::STAGES];
-    __shared__ unsigned long long s_line[3];
-    __shared__ int s_last, s_tok[ROWS];
+    __shared__ alignas(8) uint64_t bars[4 * C::STAGES + 6];
+    __shared__ TreePiece s_piece[2];
+    __shared__ int s_line[3], s_last, s_toks[2][ROWS];
     __shared__ volatile int s_gave_up;   // a consumer's wait ran out: its arrivals no longer mean free stages
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t *const tiles = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);   // the swizzle is a function of the address
     float4 *const area = reinterpret_cast<float4 *>(tiles + C::STAGES * 2 * C::TILE);
     const uint32_t bar0 = smem_u32(bars);
-    // Barriers of a stage: K empty, V empty, and two "full" ones each for K and V, which its uses take in turn.  Successive uses
-    // of a stage may belong to different groups of warps, and loads may land out of order: with one barrier a group could
-    // ask for use u while use u - 1 is still in flight and take the completion of use u - 2, which has the parity it waits for.
     auto empty_bar = [&](int v, int stage) { return bar0 + 8u * (v * C::STAGES + stage); };
-    auto full_bar = [&](int v, int stage, uint32_t use) { return bar0 + 8u * ((2 + 2 * v + (use & 1)) * C::STAGES + stage); };
+    auto full_bar = [&](int v, int stage) { return bar0 + 8u * ((2 + v) * C::STAGES + stage); };
+    // pieces (ASYNC): prepared, done with; partial results: all there, taken
+    const uint32_t piece_full = bar0 + 8u * (4 * C::STAGES), piece_empty = piece_full + 16, merge_full = piece_full + 32, merge_empty = piece_full + 40;
     auto ktile = [&](int stage) { return tiles + stage * 2 * C::TILE; };
     if (tid == 0) {
         s_gave_up = 0;
-        for (int i = 0; i < 6 * C::STAGES; ++i) mbar_init(bar0 + 8u * i, i < 2 * C::STAGES ? C::SLICES : (tma ? 1 : 32));
+        for (int i = 0; i < 4 * C::STAGES; ++i) mbar_init(bar0 + 8u * i, i < 2 * C::STAGES ? C::SLICES : (tma ? 1 : 32));
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(piece_full + 8 * i, 1);
+            mbar_init(piece_empty + 8 * i, KT_CONSUMERS + 1);
+        }
+        mbar_init(merge_full, KT_CONSUMERS);
+        mbar_init(merge_empty, 1);
         mbar_fence_init();
     }
-    constexpr TreeLine line = { ROWS, KT_KEYS };
+    constexpr TreeLine line = { ROWS, KT_KEYS, C::GROUPS };
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;   // (its barriers make the initialised ones above visible)
     TreePiece p;
     bool ok = true;
     uint32_t it = 0;   // tiles since the start: ring stage it % STAGES, its use number it / STAGES
 
+    const int heads_per = a.H / a.Hkv;
+    // Query row r of a key head: head r / n, token r % n.  A piece's Q as the lanes will read it, [eight rows][16-column group]
+    // [(hi, lo)][lane], and the rows' tokens, by `threads` threads.
+    auto stage_q = [&](const TreePiece &pc, float4 *to, int *toks, int thread, int threads) {
+#pragma unroll 4
+        for (int i = thread; i < ROWS * (DKP / 4); i += threads) {
+            const int r = i / (DKP / 4), c = i - r * (DKP / 4), row = pc.block * ROWS + r;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            int tok = 0;
+            if (row < pc.s.rows) {
+                const int gh = row / pc.s.n;
+                tok = row - gh * pc.s.n;
+                const float *src = a.Q + (((int64_t)pc.b * a.H + pc.hk * heads_per + gh) * a.T + tok) * a.dk + 4 * c;
+                if (tma) {   // rows are whole 16-byte pieces
+                    if (4 * c < a.dk) x = __ldg(reinterpret_cast<const float4 *>(src));
+                } else {
+                    if (4 * c < a.dk) x.x = __ldg(src);
+                    if (4 * c + 1 < a.dk) x.y = __ldg(src + 1);
+                    if (4 * c + 2 < a.dk) x.z = __ldg(src + 2);
+                    if (4 * c + 3 < a.dk) x.w = __ldg(src + 3);
+                }
+            }
+            if (c == 0) toks[r] = tok;
+            const int at = ((r >> 3) * (DKP / 16) + (c >> 2)) * (C::SPLIT_Q ? 64 : 32) + (r & 7) * 4 + (c & 3);
+            to[at] = x;
+            if (C::SPLIT_Q)
+                to[at + 32] = make_float4(__uint_as_float(tf32_lo(x.x)), __uint_as_float(tf32_lo(x.y)), __uint_as_float(tf32_lo(x.z)), __uint_as_float(tf32_lo(x.w)));
+        }
+    };
+    TreeWarp<DKP, NR> w;
+    auto clear = [&] {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            w.m[n][0] = w.m[n][1] = -INFINITY;
+            w.l[n][0] = w.l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < DKP / 16; ++i) w.o[i][n][0] = w.o[i][n][1] = w.o[i][n][2] = w.o[i][n][3] = 0.f;
+        }
+    };
+    // the workspace slots of an item's pieces, in lane order
+    auto slot = [&](int k) { return reinterpret_cast<float4 *>(a.slots) + (size_t)k * (C::PART_BYTES / 16) + lane; };
+    // a piece's tiles, by one consumer warp
+    auto consume = [&](const TreePiece &pc, const float4 *q, const int *toks) {
+        const uint8_t *qbase = reinterpret_cast<const uint8_t *>(q) + lane * 16;
+        const int grp = warp / C::SLICES, row0 = warp % C::SLICES * 16;
+        for (int i = 0; i < pc.count; ++i, ++it) {
+            if (C::GROUPS > 1 && (int)(it % C::GROUPS) != grp) continue;
+            const int s = it % C::STAGES;
+            const uint32_t ph = (it / C::STAGES) & 1;
+            const int key0 = (pc.t0 + i) * KT_KEYS;
+            if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(full_bar(0, s), ph))) ok = false;
+            const bool work = ok;
+            if (work) {
+                const uint8_t *kt = ktile(s);
+                if (key0 + row0 + 16 > pc.s.len)
+                    tree_tile<DKP, NR, true>(a, w, qbase, kt, kt + C::TILE, key0, row0, pc.s, pc.b, toks, empty_bar(0, s), full_bar(1, s), ph, ok);
+                else
+                    tree_tile<DKP, NR, false>(a, w, qbase, kt, kt + C::TILE, key0, row0, pc.s, pc.b, toks, empty_bar(0, s), full_bar(1, s), ph, ok);
+            }
+            if (!ok) {
+                s_gave_up = 1;
+                __threadfence_block();
+            }
+            __syncwarp();
+            if (lane == 0) {
+                if (!work) mbar_arrive(empty_bar(0, s));
+                mbar_arrive(empty_bar(1, s));
+            }
+        }
+        // the lanes' sums become the rows'
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) w.l[n][r] += __shfl_xor_sync(0xffffffffu, w.l[n][r], o);
+    };
+    // an item's result, by the warp that holds it
+    auto write_out = [&](const TreePiece &pc) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = pc.block * ROWS + n * 8 + 2 * t + r;
+                if (row >= pc.s.rows) continue;
+                const int gh = row / pc.s.n, tok = row - gh * pc.s.n;
+                float *dst = a.out + (((int64_t)pc.b * a.H + pc.hk * heads_per + gh) * a.T + tok) * a.dk;
+                const float inv = w.l[n][r] == 0.f ? 0.f : 1.0f / w.l[n][r];   // nothing seen: 0
+#pragma unroll
+                for (int sl = 0; sl < DKP / 32; ++sl) {
+                    const int c = 32 * sl + 4 * g;
+                    const float4 y = make_float4(w.o[2 * sl][n][r] * inv, w.o[2 * sl][n][2 + r] * inv, w.o[2 * sl + 1][n][r] * inv,
+                                                 w.o[2 * sl + 1][n][2 + r] * inv);
+                    if (tma) {
+                        if (c < a.dk) *reinterpret_cast<float4 *>(dst + c) = y;
+                    } else {
+                        const float *v = &y.x;
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < a.dk) dst[c + e] = v[e];
+                    }
+                }
+            }
+    };
+
     if (warp >= KT_CONSUMERS) {
         // ---- producers: warp 8 the K tiles, warp 9 the V tiles (one issuing thread turns a 16 KB tile around in some 700
         // cycles, which HBM's share of an SM would just about saturate)
         if (C::SHIFT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp > KT_CONSUMERS + 1) return;
+        if (!C::ASYNC && warp > KT_CONSUMERS + 1) return;
+        if (C::ASYNC && warp == KT_CONSUMERS + 2) {
+            // ---- scout
+            for (uint32_t k = 0;; ++k) {
+                const bool more = next_piece(a, line, cur, p);
+                if (k >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(piece_empty + 8 * (k & 1), (k / 2 - 1) & 1))) return;
+                if (!more) p.count = 0;
+                if (lane == 0) s_piece[k & 1] = p;
+                if (more) stage_q(p, area + (k & 1) * (C::Q_BYTES / 16), s_toks[k & 1], lane, 32);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(piece_full + 8 * (k & 1));
+                if (!more) return;
+            }
+        }
+        if (C::ASYNC && warp == KT_CONSUMERS + 3) {
+            // ---- merger
+            float4 *const parts = area + 2 * (C::Q_BYTES / 16) + lane;
+            for (uint32_t k = 0;; ++k) {
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(piece_full + 8 * (k & 1), (k / 2) & 1))) return;
+                p = s_piece[k & 1];
+                if (p.count == 0) return;
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(merge_full, k & 1))) return;
+                clear();
+#pragma unroll 1
+                for (int i = 0; i < KT_CONSUMERS; ++i) tree_add<DKP, NR>(w, parts + i * (C::PART_BYTES / 16), parts + i * (C::PART_BYTES / 16) + C::FRAGS * 32, 32);
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(merge_empty);
+                    mbar_arrive(piece_empty + 8 * (k & 1));
+                }
+                bool write = p.pieces == 1;
+                if (!write) {
+                    // the item's first CTA names its counter
+                    float4 *f = slot(tree_slot(blockIdx.x, p.t0 == 0));
+                    tree_put<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
+                    __threadfence();
+                    __syncwarp();
+                    int last = 0;
+                    if (lane == 0) last = atomicAdd(a.counters + p.first, 1) == p.pieces - 1;
+                    write = __shfl_sync(0xffffffffu, last, 0) != 0;
+                    if (write) {
+                        __threadfence();
+                        clear();
+#pragma unroll 3
+                        for (int i = 0; i < p.pieces; ++i) {   // (several pieces' loads in flight: a lone warp's time is their latency)
+                            const float4 *s = slot(tree_slot(p.first + i, i == 0));
+                            tree_add<DKP, NR>(w, s, s + C::FRAGS * 32, 32);
+                        }
+                        if (lane == 0) a.counters[p.first] = 0;
+                    }
+                }
+                if (write) write_out(p);
+            }
+        }
         const int v = warp - KT_CONSUMERS;
         const float *const cache = v ? a.V : a.K;
         while (ok && next_piece(a, line, cur, p)) {
@@ -383,7 +555,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
                 const uint32_t use = it / C::STAGES;
                 if (use && !__all_sync(0xffffffffu, mbar_wait_bounded(empty_bar(v, s), (use - 1) & 1))) { ok = false; break; }
                 if (s_gave_up) { ok = false; break; }
-                const uint32_t full = full_bar(v, s, use), dst = smem_u32(ktile(s)) + v * C::TILE;
+                const uint32_t full = full_bar(v, s), dst = smem_u32(ktile(s)) + v * C::TILE;
                 if (tma) {
                     if (lane == 0) {
                         mbar_arrive_expect_tx(full, C::TILE);
@@ -413,142 +585,63 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
         if (!ok) {
             if (lane == 0 && a.err) atomicCAS(a.err, 0, (int)TERR_PRODUCER);
             // copies in flight land before the CTA's memory goes away
-            for (uint32_t i = it > C::STAGES ? it - C::STAGES : 0; i < it; ++i)
-                mbar_wait_bounded(full_bar(v, i % C::STAGES, i / C::STAGES), (i / C::STAGES >> 1) & 1);
+            for (uint32_t i = it > C::STAGES ? it - C::STAGES : 0; i < it; ++i) mbar_wait_bounded(full_bar(v, i % C::STAGES), (i / C::STAGES) & 1);
         }
         return;
     }
 
     // ---- consumers
     if (C::SHIFT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-    const int g = lane >> 2, t = lane & 3, part = warp, grp = part / C::SLICES, row0 = part % C::SLICES * 16;
-    const int heads_per = a.H / a.Hkv;
-    TreeWarp<DKP, NR> w;
-    auto clear = [&] {
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-            w.m[n][0] = w.m[n][1] = -INFINITY;
-            w.l[n][0] = w.l[n][1] = 0.f;
-#pragma unroll
-            for (int i = 0; i < DKP / 16; ++i) w.o[i][n][0] = w.o[i][n][1] = w.o[i][n][2] = w.o[i][n][3] = 0.f;
-        }
-    };
-    while (next_piece(a, line, cur, p)) {
-        // query row r: head r / n of the group, token r % n.  Q as the lanes will read it, in the merge area:
-        // [eight rows][16-column group][(hi, lo)][lane]
-        for (int i = tid; i < ROWS * (DKP / 4); i += KT_CONSUMERS * 32) {
-            const int r = i / (DKP / 4), c = i - r * (DKP / 4), row = p.block * ROWS + r;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            int tok = 0;
-            if (row < p.s.rows) {
-                const int gh = row / p.s.n;
-                tok = row - gh * p.s.n;
-                const float *src = a.Q + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk + 4 * c;
-                if (tma) {   // rows are whole 16-byte pieces
-                    if (4 * c < a.dk) x = __ldg(reinterpret_cast<const float4 *>(src));
-                } else {
-                    if (4 * c < a.dk) x.x = __ldg(src);
-                    if (4 * c + 1 < a.dk) x.y = __ldg(src + 1);
-                    if (4 * c + 2 < a.dk) x.z = __ldg(src + 2);
-                    if (4 * c + 3 < a.dk) x.w = __ldg(src + 3);
-                }
-            }
-            if (c == 0) s_tok[r] = tok;
-            const int at = ((r >> 3) * (DKP / 16) + (c >> 2)) * (C::SPLIT_Q ? 64 : 32) + (r & 7) * 4 + (c & 3);
-            area[at] = x;
-            if (C::SPLIT_Q)
-                area[at + 32] = make_float4(__uint_as_float(tf32_lo(x.x)), __uint_as_float(tf32_lo(x.y)), __uint_as_float(tf32_lo(x.z)), __uint_as_float(tf32_lo(x.w)));
-        }
-        const uint8_t *qbase = reinterpret_cast<const uint8_t *>(area) + lane * 16;
-        clear();
-        consumers_sync();
-
-        for (int i = 0; i < p.count; ++i, ++it) {
-            if (C::GROUPS > 1 && (int)(it % C::GROUPS) != grp) continue;
-            const int s = it % C::STAGES;
-            const uint32_t use = it / C::STAGES, ph = (use >> 1) & 1;
-            const int key0 = (p.t0 + i) * KT_KEYS;
-            if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(full_bar(0, s, use), ph))) ok = false;
-            const bool work = ok;
-            if (work) {
-                const uint8_t *kt = ktile(s);
-                if (key0 + row0 + 16 > p.s.len)
-                    tree_tile<DKP, NR, true>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, s_tok, empty_bar(0, s), full_bar(1, s, use), ph, ok);
-                else
-                    tree_tile<DKP, NR, false>(a, w, qbase, kt, kt + C::TILE, key0, row0, p.s, p.b, s_tok, empty_bar(0, s), full_bar(1, s, use), ph, ok);
-            }
-            if (!ok) {
-                s_gave_up = 1;
-                __threadfence_block();
-            }
+    if (C::ASYNC) {
+        float4 *const mine = area + 2 * (C::Q_BYTES / 16) + warp * (C::PART_BYTES / 16) + lane;
+        for (uint32_t k = 0;; ++k) {
+            if (!ok || !__all_sync(0xffffffffu, mbar_wait_bounded(piece_full + 8 * (k & 1), (k / 2) & 1))) { ok = false; break; }
+            p = s_piece[k & 1];
+            if (p.count == 0) break;
+            clear();
+            consume(p, area + (k & 1) * (C::Q_BYTES / 16), s_toks[k & 1]);
+            if (!ok || (k && !__all_sync(0xffffffffu, mbar_wait_bounded(merge_empty, (k - 1) & 1)))) { ok = false; break; }
+            tree_put<DKP, NR>(w, mine, mine + C::FRAGS * 32, 32);
             __syncwarp();
             if (lane == 0) {
-                if (!work) mbar_arrive(empty_bar(0, s));
-                mbar_arrive(empty_bar(1, s));
+                mbar_arrive(merge_full);
+                mbar_arrive(piece_empty + 8 * (k & 1));
             }
         }
-        // the lanes' sums become the rows'
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) w.l[n][r] += __shfl_xor_sync(0xffffffffu, w.l[n][r], o);
-        consumers_sync();   // Q has been read
-        tree_merge<DKP, NR>(w, area, part);
-
-        bool write = p.count == p.s.tiles;
-        if (!write) {
-            // the item's first CTA names its counter
-            const int first = p.first, pieces = p.pieces;
-            auto slot = [&](int k) { return reinterpret_cast<float4 *>(a.slots) + (size_t)k * (32 * (C::FRAGS + NR)) + lane; };
-            if (part == 0) {
-                float4 *f = slot(tree_slot(blockIdx.x, p.t0 == 0));
-                tree_put<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
-                __threadfence();
-            }
+    } else {
+        while (next_piece(a, line, cur, p)) {
+            stage_q(p, area, s_toks[0], tid, KT_CONSUMERS * 32);
+            clear();
             consumers_sync();
-            if (tid == 0) s_last = atomicAdd(a.counters + first, 1) == pieces - 1;
-            consumers_sync();
-            write = s_last != 0;
-            if (write) {
-                __threadfence();
-                clear();
+            consume(p, area, s_toks[0]);
+            consumers_sync();   // Q has been read
+            tree_merge<DKP, NR>(w, area, warp);
+            bool write = p.pieces == 1;
+            if (!write) {
+                if (warp == 0) {
+                    float4 *f = slot(tree_slot(blockIdx.x, p.t0 == 0));
+                    tree_put<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
+                    __threadfence();
+                }
+                consumers_sync();
+                if (tid == 0) s_last = atomicAdd(a.counters + p.first, 1) == p.pieces - 1;
+                consumers_sync();
+                write = s_last != 0;
+                if (write) {
+                    __threadfence();
+                    clear();
 #pragma unroll 1
-                for (int k = part; k < pieces; k += KT_CONSUMERS) {
-                    const float4 *f = slot(tree_slot(first + k, k == 0));
-                    tree_add<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
-                }
-                tree_merge<DKP, NR>(w, area, part);
-                if (tid == 0) a.counters[first] = 0;
-            }
-        }
-        if (write && part == 0) {
-#pragma unroll
-            for (int n = 0; n < NR; ++n)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int row = p.block * ROWS + n * 8 + 2 * t + r;
-                    if (row >= p.s.rows) continue;
-                    const int gh = row / p.s.n, tok = row - gh * p.s.n;
-                    float *dst = a.out + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk;
-                    const float inv = w.l[n][r] == 0.f ? 0.f : 1.0f / w.l[n][r];   // nothing seen: 0
-#pragma unroll
-                    for (int sl = 0; sl < DKP / 32; ++sl) {
-                        const int c = 32 * sl + 4 * g;
-                        const float4 y = make_float4(w.o[2 * sl][n][r] * inv, w.o[2 * sl][n][2 + r] * inv, w.o[2 * sl + 1][n][r] * inv,
-                                                     w.o[2 * sl + 1][n][2 + r] * inv);
-                        if (tma) {
-                            if (c < a.dk) *reinterpret_cast<float4 *>(dst + c) = y;
-                        } else {
-                            const float *v = &y.x;
-                            for (int e = 0; e < 4; ++e)
-                                if (c + e < a.dk) dst[c + e] = v[e];
-                        }
+                    for (int k = warp; k < p.pieces; k += KT_CONSUMERS) {
+                        const float4 *f = slot(tree_slot(p.first + k, k == 0));
+                        tree_add<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
                     }
+                    tree_merge<DKP, NR>(w, area, warp);
+                    if (tid == 0) a.counters[p.first] = 0;
                 }
+            }
+            if (write && warp == 0) write_out(p);
+            consumers_sync();   // the merge area and the tokens are free again
         }
-        consumers_sync();   // the merge area and s_tok are free again
     }
     if (!ok && lane == 0 && a.err) atomicCAS(a.err, 0, (int)TERR_CONSUMER);
 }
@@ -618,8 +711,8 @@ template <int DKP, int NR>
 static int launch_tree(const KvTreeArgs &a, const TreeMaps &tm, int tma, int sm_count, cudaStream_t st)
 {
     using C = TreeCfg<DKP, NR>;
-    static_assert(C::STAGES >= 2 && C::SMEM <= 227 * 1024 - 2048, "shared memory");
-    static_assert((size_t)32 * (C::FRAGS + NR) * 16 <= KT_SLOT_BYTES, "workspace slots");
+    static_assert(C::SMEM <= 227 * 1024 - 2048, "shared memory");
+    static_assert((size_t)C::PART_BYTES <= KT_SLOT_BYTES, "workspace slots");
     static PerDeviceOnce once;
     if (once.first()) {
         cudaError_t e = cudaFuncSetAttribute(kv_tree_kernel<DKP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);

@@ -7,9 +7,10 @@
 
 namespace axb {
 
-// query rows of an item, keys of a tile
+// query rows of an item, keys of a tile, tiles that a CTA works on side by side (a shorter stretch takes as long, and an item
+// cut into fewer pieces is added up sooner)
 struct TreeLine {
-    int block_rows, tile_keys;
+    int block_rows, tile_keys, min_stretch;
 };
 
 struct TreeSeq {
@@ -21,22 +22,23 @@ __device__ __forceinline__ TreeSeq tree_seq(const KvTreeArgs &a, const TreeLine 
     TreeSeq s;
     s.len = __ldg(a.lens + b);
     s.n = a.n_new ? __ldg(a.n_new + b) : a.T;
-    const bool off = s.len < 0 || s.n < 0 || s.n > a.T || (int64_t)s.len + s.n > a.max_seq;
+    const bool off = s.len < 0 || s.n < 0 || s.n > a.T || (int64_t)s.len + s.n > a.max_seq;   // (max_seq <= 2^30)
     if (bad) *bad = off;
     if (off) s.len = s.n = 0;   // refused whole: its output rows are left alone
     s.rows = s.n * (a.H / a.Hkv);
     s.blocks = (s.rows + ln.block_rows - 1) / ln.block_rows;
-    s.tiles = s.n ? (int)(((int64_t)s.len + s.n + ln.tile_keys - 1) / ln.tile_keys) : 0;
+    s.tiles = s.n ? (s.len + s.n + ln.tile_keys - 1) / ln.tile_keys : 0;
     return s;
 }
 
-__device__ __forceinline__ int64_t tree_tiles(const KvTreeArgs &a, const TreeSeq &s) { return (int64_t)a.Hkv * s.blocks * s.tiles; }
+// (the launcher refuses batches whose line could pass 2^31 tiles)
+__device__ __forceinline__ int tree_tiles(const KvTreeArgs &a, const TreeSeq &s) { return a.Hkv * s.blocks * s.tiles; }
 
 struct TreeCursor {
     int b;
-    int64_t base;      // where sequence b's part of the line begins
-    int64_t pos, end;  // what is left of this CTA's stretch
-    int64_t per;       // a stretch
+    int base;      // where sequence b's part of the line begins
+    int pos, end;  // what is left of this CTA's stretch
+    int per;       // a stretch
 };
 
 // one piece: consecutive tiles of one item
@@ -47,71 +49,84 @@ struct TreePiece {
 };
 
 // Every thread of the CTA; shared: 3 words.  False: nothing for this CTA (for all its threads).
-__device__ __forceinline__ bool tree_start(const KvTreeArgs &a, const TreeLine &ln, unsigned long long *shared, TreeCursor &c)
+__device__ __forceinline__ bool tree_start(const KvTreeArgs &a, const TreeLine &ln, int *shared, TreeCursor &c)
 {
-    if (threadIdx.x == 0) shared[0] = 0;
-    __syncthreads();
-    unsigned long long sum = 0;
-    for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
+    const int lane = threadIdx.x & 31;
+    auto tiles_of = [&](int b) -> int {
+        if (b >= a.B) return 0;
         bool bad;
         const TreeSeq s = tree_seq(a, ln, b, &bad);
-        sum += (unsigned long long)tree_tiles(a, s);
         if (bad && blockIdx.x == 0 && a.err) atomicCAS(a.err, 0, (int)AXB_DEVERR_ROWS);
+        return tree_tiles(a, s);
+    };
+    int mine = 0;
+    if (a.B > 32) {
+        if (threadIdx.x == 0) shared[0] = 0;
+        __syncthreads();
+        int sum = 0;
+        for (int b = threadIdx.x; b < a.B; b += blockDim.x) sum += tiles_of(b);
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0 && sum) atomicAdd(shared, sum);
+        __syncthreads();
     }
-    if (sum) atomicAdd(shared, sum);
-    __syncthreads();
-    const int64_t total = (int64_t)shared[0];
-    c.per = (total + gridDim.x - 1) / gridDim.x;
-    c.pos = c.per * blockIdx.x;
-    c.end = c.pos + c.per < total ? c.pos + c.per : total;
-    if (c.pos >= c.end) return false;
     if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        int64_t before = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 32) {
-            const int64_t mine = b0 + lane < a.B ? tree_tiles(a, tree_seq(a, ln, b0 + lane)) : 0;
-            int64_t upto = mine;
+        // one warp finds the total (of up to 32 sequences) and the sequence in which the stretch begins
+        int total = shared[0];
+        if (a.B <= 32) {
+            mine = tiles_of(lane);
+            total = __reduce_add_sync(0xffffffffu, mine);
+        }
+        const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, ln.min_stretch), pos = min(per * (int)blockIdx.x, total);
+        int before = 0;
+        for (int b0 = 0; pos < total && b0 < a.B; b0 += 32) {
+            if (a.B > 32) mine = tiles_of(b0 + lane);
+            int upto = mine;
             for (int o = 1; o < 32; o <<= 1) {
-                const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += v;
             }
-            const unsigned past = __ballot_sync(0xffffffffu, before + upto > c.pos);
+            const unsigned past = __ballot_sync(0xffffffffu, before + upto > pos);
             if (past) {
                 const int k = __ffs(past) - 1;
                 if (lane == k) {
-                    shared[1] = (unsigned long long)(b0 + k);
-                    shared[2] = (unsigned long long)(before + upto - mine);
+                    shared[1] = b0 + k;
+                    shared[2] = before + upto - mine;
                 }
                 break;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
+        __syncwarp();
+        if (lane == 0) shared[0] = total;
     }
     __syncthreads();
-    c.b = (int)shared[1];
-    c.base = (int64_t)shared[2];
-    return true;
+    const int total = shared[0];
+    c.per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, ln.min_stretch);
+    c.pos = min(c.per * (int)blockIdx.x, total);
+    c.end = min(c.pos + c.per, total);
+    c.b = shared[1];
+    c.base = shared[2];
+    return c.pos < c.end;
 }
 
 __device__ __forceinline__ bool next_piece(const KvTreeArgs &a, const TreeLine &ln, TreeCursor &c, TreePiece &p)
 {
     while (c.pos < c.end) {
         p.s = tree_seq(a, ln, c.b);
-        const int64_t total = tree_tiles(a, p.s);
-        if (c.pos >= c.base + total) {
+        const int total = tree_tiles(a, p.s);
+        if (c.pos - c.base >= total) {
             c.base += total;
             ++c.b;
             continue;
         }
-        const int64_t item = (c.pos - c.base) / p.s.tiles, item_pos = c.base + item * p.s.tiles;
+        const int item = (c.pos - c.base) / p.s.tiles, item_pos = c.base + item * p.s.tiles;
         p.b = c.b;
-        p.t0 = (int)(c.pos - item_pos);
-        p.hk = (int)(item / p.s.blocks);
-        p.block = (int)(item - (int64_t)p.hk * p.s.blocks);
-        const int64_t left = c.end - c.pos;
-        p.count = p.s.tiles - p.t0 < left ? p.s.tiles - p.t0 : (int)left;
-        p.first = (int)(item_pos / c.per);
-        p.pieces = (int)((item_pos + p.s.tiles - 1) / c.per) - p.first + 1;
+        p.t0 = c.pos - item_pos;
+        p.hk = item / p.s.blocks;
+        p.block = item - p.hk * p.s.blocks;
+        p.count = min(p.s.tiles - p.t0, c.end - c.pos);
+        p.first = item_pos / c.per;
+        p.pieces = (item_pos + p.s.tiles - 1) / c.per - p.first + 1;
         c.pos += p.count;
         return true;
     }

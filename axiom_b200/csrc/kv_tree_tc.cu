@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     extern __shared__ __align__(1024) uint8_t sm[];
     const uint32_t base = smem_u32(sm);
     auto bar = [&](int i) -> uint32_t { return base + 8u * (uint32_t)i; };
-    unsigned long long *s_line = reinterpret_cast<unsigned long long *>(sm + 256);
+    int *s_line = reinterpret_cast<int *>(sm + 256);
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(sm + 288);
     volatile int *words = reinterpret_cast<volatile int *>(sm + 304);
     volatile int &s_gave_up = words[0], &s_last = words[1], *s_odd = words + 2;   // s_odd: block it + 1 holds non-finite new values
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
         s_gave_up = 0;
         for (int i = 0; i < 4; ++i) s_odd[i] = 0;
     }
-    constexpr TreeLine line = { TT_ROWS, KB };
+    constexpr TreeLine line = { TT_ROWS, KB, 1 };
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;
     if (warp == 19) {
