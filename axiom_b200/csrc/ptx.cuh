@@ -92,17 +92,6 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity)
     }
 }
 
-// The same bounded by a number of polls instead of the timer, with a short sleep between them (about a second in all).
-__device__ __forceinline__ bool mbar_poll_bounded(uint32_t bar, uint32_t parity)
-{
-#pragma unroll 1
-    for (uint32_t i = 0; i < (1u << 24); ++i) {
-        if (mbar_test_wait(bar, parity)) return true;
-        __nanosleep(40);
-    }
-    return false;
-}
-
 // Whole-warp wait for warps that wait long (epilogue warps wait a whole K loop): only lane 0
 // polls, with a sleep between polls, so the waiters do not compete with the MMA-issuing
 // thread for the barrier unit; the outcome is broadcast to the warp.

@@ -9,27 +9,35 @@
 // of a cache — like the layout pass (head_layout.cu), whose place this takes: one read and one write of every element
 // (the backward reads x too where there is a norm).  HBM-bound.
 //
-// A CTA takes a few tokens.  Their angles are formed once, for all heads: p * f in turns in 64 bits (a position of
-// 10^6 times a frequency of 1 has lost five of fp32's seven digits), the whole turns dropped, and the remainder's sine
-// and cosine in fp32.  A group of lanes owns a head row; a lane owns two 16-byte pieces of it that hold both partners of
-// its pairs (piece c and c + pairs/4 of the half-split layout; the interleaved pairs lie inside a piece), so the rotation
-// needs no exchange and the norm one shuffle tree.  Head dims and rotated parts that do not cut into 16-byte pieces,
-// and unaligned tensors, take the same kernel with single floats in the place of the pieces.
+// The tokens lie on a line, each of them a number of steps long: a warp step takes as many head rows, all q, all k or all v,
+// as fit its lanes.  Every warp gets a stretch of the line of the same length to within a step, and the next step's rows are
+// on their way while it works on this one's; where a warp meets a token it forms that token's angles, each pair's once by one
+// lane, for all its heads: p * f in turns in 64 bits (a position of 10^6 times a frequency of 1 has lost five of fp32's
+// seven digits), the whole turns dropped, and the remainder's sine and cosine in fp32.  No barrier of the CTA is met: with
+// CTAs that took four tokens at a time (angles behind a barrier, no row ahead) the backward of 8192 tokens of 16 + 2*8 heads
+// of 128 (369 MB) took 113 us, so 70; the forward of 16384 tokens of 32 + 2*8 heads (805 MB) 143 and 135.  The backward's
+// instructions, not its bytes, set its time: rows of one kind a step, instead of q, k and v rows side by side with selects,
+// made 78 us 70.
+//
+// A group of lanes owns a head row (any number of lanes up to 32: a head of 80 takes 10, three rows a warp); a lane owns two
+// 16-byte pieces of it that hold both partners of its pairs (piece c and c + pairs/4 of the half-split layout; the
+// interleaved pairs lie inside a piece), so the rotation needs no exchange and the norm one shuffle tree.  Head dims and
+// rotated parts that do not cut into 16-byte pieces, and unaligned tensors, take the same kernel with single floats in the
+// place of the pieces.
 #include "rope.cuh"
 
 #include <math.h>
 
 namespace axb {
 
-static constexpr int RP_THREADS = 256;
+static constexpr int RP_THREADS = 128, RP_WARPS = RP_THREADS / 32, RP_FWD_CTAS = 8, RP_BWD_CTAS = 5;
 static constexpr double RP_INV_2PI = 0.15915494309189533577;
 
 // which pieces (VEC floats each) of a head row unit u of a lane covers, and whether they form rotated pairs
 template <int VEC>
 struct RopeUnit {
     int v0, v1;      // piece indices, -1: none
-    int p0, p1;      // first pair of the rotation of piece 0 (half split: of both pieces; -1: not rotated)
-    bool half;
+    int p0, p1;      // first pair of the rotation of piece 0 (of both, unless whole pairs lie in a piece; -1: not rotated)
 };
 
 template <int VEC, bool INTER>
@@ -37,7 +45,6 @@ __device__ __forceinline__ RopeUnit<VEC> rope_unit(int u, int dk, int pairs)
 {
     const int nv = dk / VEC;
     RopeUnit<VEC> r;
-    r.half = false;
     if (INTER && VEC == 4) {
         const int h = (nv + 1) / 2, rv = pairs / 2;   // rotated pieces: two pairs each
         r.v0 = u < h ? u : -1;
@@ -52,7 +59,6 @@ __device__ __forceinline__ RopeUnit<VEC> rope_unit(int u, int dk, int pairs)
         r.v1 = INTER ? 2 * u + 1 : u + pu;
         r.p0 = u * VEC;
         r.p1 = -1;
-        r.half = true;
     } else {
         const int t = u - pu, tail = nv - 2 * pu, tu = (tail + 1) / 2;
         r.v0 = t < tu ? 2 * pu + t : -1;
@@ -67,18 +73,16 @@ struct Piece {
     float x[VEC];
 };
 
+// (16-byte pieces: a lane without a second piece reads its first again, and its caller leaves it out of the sums)
 template <int VEC>
-__device__ __forceinline__ Piece<VEC> load_piece(const float *row, int v)
+__device__ __forceinline__ Piece<VEC> load_piece(const float *row, int v, int else_v)
 {
     Piece<VEC> p;
-    if (v < 0) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) p.x[i] = 0.f;
-    } else if (VEC == 4) {
-        const float4 t = *reinterpret_cast<const float4 *>(row + 4 * v);
+    if (VEC == 4) {
+        const float4 t = *reinterpret_cast<const float4 *>(row + 4 * (v < 0 ? else_v : v));
         p.x[0] = t.x; p.x[1 % VEC] = t.y; p.x[2 % VEC] = t.z; p.x[3 % VEC] = t.w;
     } else {
-        p.x[0] = row[v];
+        p.x[0] = v < 0 ? 0.f : row[v];
     }
     return p;
 }
@@ -91,192 +95,320 @@ __device__ __forceinline__ void store_piece(float *row, int v, const Piece<VEC> 
     else row[v] = p.x[0];
 }
 
-// rotates a lane's two pieces by the angles whose cosines and sines (times the amplitude) lie at cs, sn; BACK turns the
-// other way (the transpose)
-template <int VEC, bool BACK>
+// rotates a lane's two pieces by its angles (cosines and sines times the amplitude); BACK turns the other way (the transpose)
+template <int VEC, bool INTER, bool BACK>
 __device__ __forceinline__ void rotate_unit(const RopeUnit<VEC> &u, const float *cs, const float *sn, Piece<VEC> &a, Piece<VEC> &b)
 {
-    if (u.half) {
+    if (!(INTER && VEC == 4)) {
+        if (u.p0 < 0) return;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const float c = cs[u.p0 + i], s = BACK ? -sn[u.p0 + i] : sn[u.p0 + i];
+            const float c = cs[i], s = BACK ? -sn[i] : sn[i];
             const float x = a.x[i], y = b.x[i];
             a.x[i] = x * c - y * s;
             b.x[i] = y * c + x * s;
         }
         return;
     }
+    auto turn = [&](Piece<VEC> &p, int at) {
 #pragma unroll
-    for (int i = 0; i + 1 < VEC; i += 2) {
-        if (u.p0 >= 0) {
-            const float c = cs[u.p0 + i / 2], s = BACK ? -sn[u.p0 + i / 2] : sn[u.p0 + i / 2];
-            const float x = a.x[i], y = a.x[(i + 1) % VEC];
-            a.x[i] = x * c - y * s;
-            a.x[(i + 1) % VEC] = y * c + x * s;
+        for (int i = 0; i < VEC; i += 2) {
+            const float c = cs[(at + i / 2) % VEC], s = BACK ? -sn[(at + i / 2) % VEC] : sn[(at + i / 2) % VEC];
+            const float x = p.x[i], y = p.x[(i + 1) % VEC];
+            p.x[i] = x * c - y * s;
+            p.x[(i + 1) % VEC] = y * c + x * s;
         }
-        if (u.p1 >= 0) {
-            const float c = cs[u.p1 + i / 2], s = BACK ? -sn[u.p1 + i / 2] : sn[u.p1 + i / 2];
-            const float x = b.x[i], y = b.x[(i + 1) % VEC];
-            b.x[i] = x * c - y * s;
-            b.x[(i + 1) % VEC] = y * c + x * s;
-        }
-    }
+    };
+    if (u.p0 >= 0) turn(a, 0);
+    if (u.p1 >= 0) turn(b, 2);
 }
 
-__device__ __forceinline__ float lanes_sum(float v, int width)
+// the sums of N numbers over a row's `width` lanes, in each of them (li: the lane's place in the row; lanes past the last
+// row get what nobody uses)
+template <int N>
+__device__ __forceinline__ void lanes_sum(float *v, int li, int width)
 {
-    for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    if ((width & (width - 1)) == 0) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            if (o < width) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+            }
+        return;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const float t = __shfl_down_sync(0xffffffffu, v[n], o);
+            if (li + o < width) v[n] += t;
+        }
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = __shfl_sync(0xffffffffu, v[n], (int)(threadIdx.x & 31) - li);
 }
 
 struct RopePlan {
-    int lpr;        // lanes per head row (power of two)
-    int tok_cta;    // tokens a CTA takes at a time
-    int heads_cta;  // head rows (of H + 2*Hkv) of a token that one CTA takes
+    int lpr, rpw;   // lanes of a head row, head rows a warp takes at a time
+    int sq, sk;     // steps of a token's q heads and of its k or v heads (a step's rows are of one kind: the code of a step
+    int steps;      // is then the same for the whole warp); steps of a token: sq + 2*sk
+    int blocks;
 };
 
-// Places and angles of a CTA's tokens, in shared memory.  q_row / kv_row: the row index of head 0 (-1: not written).
-struct RopeTokens {
-    float *cs, *sn;            // [tok_cta][pairs]
-    int64_t *q_row, *kv_row;   // [tok_cta]
+// A token: number s of sequence b (b < 0: not wanted), its row among the sequence's keys, its position.
+struct RopeToken {
+    int tok, b, s, kv, p;
 };
 
-__device__ __forceinline__ RopeTokens rope_tokens(void *smem, const RopePlan &p, int pairs)
+__device__ __forceinline__ RopeToken rope_token(const RopeArgs &a, int tok)
 {
-    RopeTokens t;
-    t.q_row = reinterpret_cast<int64_t *>(smem);
-    t.kv_row = t.q_row + p.tok_cta;
-    t.cs = reinterpret_cast<float *>(t.kv_row + p.tok_cta);
-    t.sn = t.cs + (size_t)p.tok_cta * pairs;
+    RopeToken t;
+    t.tok = tok;
+    t.b = tok / a.T;
+    t.s = t.kv = tok - t.b * a.T;
+    bool valid = true;
+    if (a.lens) {
+        const int len = a.lens[t.b], n = a.n_new ? a.n_new[t.b] : a.T;
+        // a sequence that does not fit its rows is refused whole: nothing of it is read or written
+        const bool bad = len < 0 || n < 0 || n > a.T || (int64_t)len + n > a.kv_rows;
+        if (bad && a.err && (threadIdx.x & 31) == 0) atomicCAS(a.err, 0, (int)AXB_DEVERR_ROWS);
+        valid = !bad && t.s < n;
+        if (valid) t.kv += len;
+    }
+    t.p = !valid ? 0 : a.pos ? a.pos[tok] : t.kv;
+    if (!valid) t.b = -1;
     return t;
 }
 
-__device__ __forceinline__ void rope_place(const RopeArgs &a, const RopeTokens &t, int64_t tok0, int ntok, int64_t seq_rows)
+// A warp's stretch of the work line (all tokens in order, each `steps` long), and its place in it.
+struct RopeCursor {
+    int left;   // steps from here to the stretch's end
+    int step;   // of the token
+    RopeToken t;
+};
+
+__device__ __forceinline__ void rope_seek(RopeCursor &c, const RopeArgs &a, const RopePlan &p)
 {
-    for (int i = threadIdx.x; i < ntok; i += RP_THREADS) {
-        const int64_t tok = tok0 + i;
-        const int b = (int)(tok / a.T), s = (int)(tok - (int64_t)b * a.T);
-        int64_t first = 0;
-        bool valid = true;
-        if (a.lens) {
-            const int len = a.lens[b], n = a.n_new ? a.n_new[b] : a.T;
-            // a sequence that does not fit its rows is refused whole: nothing of it is read or written
-            const bool bad = len < 0 || n < 0 || n > a.T || (int64_t)len + n > a.kv_rows;
-            if (bad && a.err) atomicCAS(a.err, 0, (int)AXB_DEVERR_ROWS);
-            valid = !bad && s < n;
-            first = len;
-        }
-        t.q_row[i] = valid ? (int64_t)b * a.H * a.T + s : -1;
-        t.kv_row[i] = valid ? (int64_t)b * a.Hkv * seq_rows + first + s : -1;
-    }
-    for (int i = threadIdx.x; i < ntok * a.pairs; i += RP_THREADS) {
-        const int k = i / a.pairs;
-        const int64_t tok = tok0 + k;
-        const int b = (int)(tok / a.T);
-        const int p = a.pos ? a.pos[tok] : (int)(tok - (int64_t)b * a.T) + (a.lens ? a.lens[b] : 0);
-        const double turns = (double)p * (a.freq[i - k * a.pairs] * RP_INV_2PI);
-        float s, c;
-        sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-        t.cs[i] = c * a.amplitude;
-        t.sn[i] = s * a.amplitude;
+    while (c.left > 0 && c.t.b < 0) {   // the rest of a token that is not wanted
+        c.left -= p.steps - c.step;
+        c.step = 0;
+        if (c.left > 0) c.t = rope_token(a, c.t.tok + 1);
     }
 }
 
+__device__ __forceinline__ RopeCursor rope_start(const RopeArgs &a, const RopePlan &p)
+{
+    RopeCursor c;
+    const int64_t total = (int64_t)a.B * a.T * p.steps, warps = (int64_t)gridDim.x * RP_WARPS;
+    const int64_t w = (int64_t)blockIdx.x * RP_WARPS + (threadIdx.x >> 5), each = total / warps, more = total % warps;
+    const int64_t first = w * each + (w < more ? w : more);
+    c.left = (int)each + (w < more);
+    c.step = 0;
+    c.t = RopeToken{ 0, -1, 0, 0, 0 };
+    if (c.left == 0) return c;
+    c.step = (int)(first % p.steps);
+    c.t = rope_token(a, (int)(first / p.steps));
+    rope_seek(c, a, p);
+    return c;
+}
+
+__device__ __forceinline__ void rope_next(RopeCursor &c, const RopeArgs &a, const RopePlan &p)
+{
+    --c.left;
+    if (++c.step < p.steps || c.left <= 0) return;
+    c.step = 0;
+    c.t = rope_token(a, c.t.tok + 1);
+    rope_seek(c, a, p);
+}
+
+// The angles of position pos: each pair's once, by one lane, through the warp's 2*pairs words of shared memory.
+template <int VEC, bool INTER, int NU>
+__device__ __forceinline__ void rope_angles(const RopeArgs &a, int pos, float *table, const RopeUnit<VEC> *u, float *cs, float *sn)
+{
+    __syncwarp();   // the words before are read
+    for (int i = threadIdx.x & 31; i < a.pairs; i += 32) {
+        const double turns = (double)pos * (a.freq[i] * RP_INV_2PI);
+        float s, c;
+        sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+        table[i] = c * a.amplitude;
+        table[a.pairs + i] = s * a.amplitude;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < NU; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int at = INTER && VEC == 4 ? (i < 2 ? u[j].p0 + i : u[j].p1 + i - 2) : u[j].p0 + i;
+            const bool has = INTER && VEC == 4 && i >= 2 ? u[j].p1 >= 0 : u[j].p0 >= 0;
+            cs[j * VEC + i] = has ? table[at] : 1.f;
+            sn[j * VEC + i] = has ? table[a.pairs + at] : 0.f;
+        }
+}
+
+// A step's rows: which kind, the lane's head of that kind (none past the last: `on` false, the row then read is another
+// one's), where it stands in qkv and in the head-major buffer.
+enum RopeKind { ROPE_Q, ROPE_K, ROPE_V };
+
+struct RopeRow {
+    int kind;
+    bool on;
+    int64_t flat, head;   // element offsets
+};
+
+__device__ __forceinline__ RopeRow rope_row(const RopeArgs &a, const RopePlan &p, const RopeCursor &c, int row)
+{
+    RopeRow r;
+    const int kv = c.step - p.sq;
+    r.kind = kv < 0 ? ROPE_Q : kv < p.sk ? ROPE_K : ROPE_V;
+    const int count = kv < 0 ? a.H : a.Hkv, at = kv < 0 ? c.step : kv < p.sk ? kv : kv - p.sk;
+    int h = at * p.rpw + row;
+    r.on = row < p.rpw && h < count;
+    h = r.on ? h : at * p.rpw;
+    r.flat = ((int64_t)c.t.tok * (a.H + 2 * a.Hkv) + (kv < 0 ? 0 : kv < p.sk ? a.H : a.H + a.Hkv) + h) * a.dk;
+    r.head = kv < 0 ? (((int64_t)c.t.b * a.H + h) * a.T + c.t.s) * a.dk : (((int64_t)c.t.b * a.Hkv + h) * a.kv_rows + c.t.kv) * a.dk;
+    return r;
+}
+
 template <int VEC, bool INTER>
-__global__ void __launch_bounds__(RP_THREADS) qkv_norm_rope_kernel(const RopeArgs a, const RopePlan p)
+__global__ void __launch_bounds__(RP_THREADS, RP_FWD_CTAS) qkv_norm_rope_kernel(const RopeArgs a, const RopePlan p)
 {
     constexpr int NU = VEC == 4 ? 1 : 4;   // units a lane covers: 32 lanes hold 256 floats either way
-    extern __shared__ double smem[];
-    const RopeTokens tk = rope_tokens(smem, p, a.pairs);
-    const int64_t tokens = (int64_t)a.B * a.T, tok0 = (int64_t)blockIdx.x * p.tok_cta;
-    const int ntok = (int)(tokens - tok0 < p.tok_cta ? tokens - tok0 : p.tok_cta);
-    rope_place(a, tk, tok0, ntok, a.kv_rows);
-    __syncthreads();
-
-    const int heads = a.H + 2 * a.Hkv, h0 = blockIdx.y * p.heads_cta;
-    const int nh = heads - h0 < p.heads_cta ? heads - h0 : p.heads_cta;
-    const int lane = threadIdx.x & 31, li = lane & (p.lpr - 1), rpw = 32 / p.lpr;
-    const int step = (RP_THREADS / 32) * rpw, rows = ntok * nh;
+    extern __shared__ float smem[];
+    float *table = smem + (threadIdx.x >> 5) * 2 * a.pairs;
+    const int lane = threadIdx.x & 31, row = lane / p.lpr, li = lane - row * p.lpr;
     RopeUnit<VEC> u[NU];
 #pragma unroll
     for (int j = 0; j < NU; ++j) u[j] = rope_unit<VEC, INTER>(li + 32 * j, a.dk, a.pairs);
     const float inv_dk = 1.0f / (float)a.dk;
+    float cs[NU * VEC], sn[NU * VEC];
+    int angles_of = -1;
 
-    // (warp-uniform bounds: the norm's shuffles need every lane)
-    for (int w0 = (threadIdx.x >> 5) * rpw; w0 < rows; w0 += step) {
-        const int r = w0 + lane / p.lpr;
-        const int t = r < rows ? r / nh : 0, h = h0 + (r < rows ? r - t * nh : 0);
-        const int64_t qr = tk.q_row[t];
-        const bool on = r < rows && qr >= 0;
-        const float *src = a.qkv + ((tok0 + t) * heads + h) * a.dk;
-        Piece<VEC> x0[NU], x1[NU];
-        float ss = 0.f;
+    RopeCursor c = rope_start(a, p);
+    RopeRow nr;
+    Piece<VEC> n0[NU], n1[NU];   // the next step's rows, on their way while this step's are worked on
+    auto load = [&]() {
+        nr = rope_row(a, p, c, row);
+        const float *src = a.qkv + nr.flat;
 #pragma unroll
         for (int j = 0; j < NU; ++j) {
-            x0[j] = load_piece<VEC>(src, on ? u[j].v0 : -1);
-            x1[j] = load_piece<VEC>(src, on ? u[j].v1 : -1);
+            n0[j] = load_piece<VEC>(src, u[j].v0, 0);
+            n1[j] = load_piece<VEC>(src, u[j].v1, u[j].v0);
         }
+    };
+    if (c.left > 0) load();
+    while (c.left > 0) {   // (the same for all lanes of a warp: the norm's shuffles need every one)
+        Piece<VEC> x0[NU], x1[NU];
+#pragma unroll
+        for (int j = 0; j < NU; ++j) { x0[j] = n0[j]; x1[j] = n1[j]; }
+        const RopeRow r = nr;
+        const int tok = c.t.tok, pos = c.t.p;
+        rope_next(c, a, p);
+        if (c.left > 0) load();
         if (a.bias) {
-            const float *bias = a.bias + (int64_t)h * a.dk;
+            const float *bias = a.bias + (r.flat - (int64_t)tok * (a.H + 2 * a.Hkv) * a.dk);
 #pragma unroll
             for (int j = 0; j < NU; ++j) {
-                const Piece<VEC> b0 = load_piece<VEC>(bias, u[j].v0), b1 = load_piece<VEC>(bias, u[j].v1);
+                const Piece<VEC> b0 = load_piece<VEC>(bias, u[j].v0, 0), b1 = load_piece<VEC>(bias, u[j].v1, u[j].v0);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) { x0[j].x[i] += b0.x[i]; x1[j].x[i] += b1.x[i]; }
             }
         }
-        const float *g = h < a.H ? a.gq : h < a.H + a.Hkv ? a.gk : nullptr;
-        if (a.gq || a.gk) {
+        if (r.kind != ROPE_V) {
+            if (tok != angles_of) {
+                rope_angles<VEC, INTER, NU>(a, pos, table, u, cs, sn);
+                angles_of = tok;
+            }
+            if (const float *g = r.kind == ROPE_Q ? a.gq : a.gk) {
+                float ss = 0.f;
 #pragma unroll
-            for (int j = 0; j < NU; ++j)
+                for (int j = 0; j < NU; ++j) {
+                    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) ss += x0[j].x[i] * x0[j].x[i] + x1[j].x[i] * x1[j].x[i];
-            ss = lanes_sum(ss, p.lpr);
-        }
-        if (g) {
-            const float rs = rsqrtf(ss * inv_dk + a.eps);
+                    for (int i = 0; i < VEC; ++i) { s0 += x0[j].x[i] * x0[j].x[i]; s1 += x1[j].x[i] * x1[j].x[i]; }
+                    ss += s0 + (u[j].v1 >= 0 ? s1 : 0.f);
+                }
+                lanes_sum<1>(&ss, li, p.lpr);
+                const float rs = rsqrtf(ss * inv_dk + a.eps);
 #pragma unroll
-            for (int j = 0; j < NU; ++j) {
-                const Piece<VEC> g0 = load_piece<VEC>(g, u[j].v0), g1 = load_piece<VEC>(g, u[j].v1);
+                for (int j = 0; j < NU; ++j) {
+                    const Piece<VEC> g0 = load_piece<VEC>(g, u[j].v0, 0), g1 = load_piece<VEC>(g, u[j].v1, u[j].v0);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    x0[j].x[i] = x0[j].x[i] * rs * g0.x[i];
-                    x1[j].x[i] = x1[j].x[i] * rs * g1.x[i];
+                    for (int i = 0; i < VEC; ++i) {
+                        x0[j].x[i] = x0[j].x[i] * rs * g0.x[i];
+                        x1[j].x[i] = x1[j].x[i] * rs * g1.x[i];
+                    }
                 }
             }
-        }
-        if (!on) continue;   // (no shuffle follows; lanes without a row meet the loop's bound with the others)
-        if (h < a.H + a.Hkv) {
 #pragma unroll
-            for (int j = 0; j < NU; ++j) rotate_unit<VEC, false>(u[j], tk.cs + t * a.pairs, tk.sn + t * a.pairs, x0[j], x1[j]);
+            for (int j = 0; j < NU; ++j) rotate_unit<VEC, INTER, false>(u[j], cs + j * VEC, sn + j * VEC, x0[j], x1[j]);
         }
-        float *dst = h < a.H               ? a.q + (qr + (int64_t)h * a.T) * a.dk
-                     : h < a.H + a.Hkv     ? a.k + (tk.kv_row[t] + (int64_t)(h - a.H) * a.kv_rows) * a.dk
-                                           : a.v + (tk.kv_row[t] + (int64_t)(h - a.H - a.Hkv) * a.kv_rows) * a.dk;
+        if (r.on) {
+            float *dst = (r.kind == ROPE_Q ? a.q : r.kind == ROPE_K ? a.k : a.v) + r.head;
 #pragma unroll
-        for (int j = 0; j < NU; ++j) {
-            store_piece<VEC>(dst, u[j].v0, x0[j]);
-            store_piece<VEC>(dst, u[j].v1, x1[j]);
+            for (int j = 0; j < NU; ++j) {
+                store_piece<VEC>(dst, u[j].v0, x0[j]);
+                store_piece<VEC>(dst, u[j].v1, x1[j]);
+            }
         }
     }
 }
 
-// The gradient: the same ownership the other way, persistent CTAs.  A lane meets the same head elements in every row, so
-// the norm weights' gradients collect in its registers; groups are added in shared memory, CTAs by rope_dgamma_kernel,
-// each in a fixed order.
+// A step of the backward's rows that have a norm weight: d (rotated back) becomes dx, d*u is added to acc.
+template <int VEC, int NU>
+__device__ __forceinline__ void norm_back(const RopeArgs &a, const float *g, const RopeUnit<VEC> *u, int li, int lpr, float inv_dk, bool on,
+                                          Piece<VEC> *d0, Piece<VEC> *d1, const Piece<VEC> *x0, const Piece<VEC> *x1,
+                                          float (&acc)[2][NU][VEC])
+{
+    float sum[2] = { 0.f, 0.f };   // x^2, d*g*x
+    Piece<VEC> g0[NU], g1[NU];
+#pragma unroll
+    for (int j = 0; j < NU; ++j) {
+        g0[j] = load_piece<VEC>(g, u[j].v0, 0);
+        g1[j] = load_piece<VEC>(g, u[j].v1, u[j].v0);
+        float s0 = 0.f, s1 = 0.f, e0 = 0.f, e1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            g0[j].x[i] *= d0[j].x[i];
+            g1[j].x[i] *= d1[j].x[i];
+            s0 += x0[j].x[i] * x0[j].x[i];
+            s1 += x1[j].x[i] * x1[j].x[i];
+            e0 += g0[j].x[i] * x0[j].x[i];
+            e1 += g1[j].x[i] * x1[j].x[i];
+        }
+        sum[0] += s0 + (u[j].v1 >= 0 ? s1 : 0.f);
+        sum[1] += e0 + (u[j].v1 >= 0 ? e1 : 0.f);
+    }
+    lanes_sum<2>(sum, li, lpr);
+    const float rs = rsqrtf(sum[0] * inv_dk + a.eps), mean = sum[1] * rs * inv_dk;   // mean(d*g*u)
+#pragma unroll
+    for (int j = 0; j < NU; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float u0 = x0[j].x[i] * rs, u1 = x1[j].x[i] * rs;
+            if (on) {
+                acc[0][j][i] += d0[j].x[i] * u0;
+                acc[1][j][i] += d1[j].x[i] * u1;
+            }
+            d0[j].x[i] = rs * (g0[j].x[i] - u0 * mean);
+            d1[j].x[i] = rs * (g1[j].x[i] - u1 * mean);
+        }
+}
+
+// The gradient: the same ownership the other way.  A lane meets the same head elements in every row, so the norm weights'
+// gradients collect in its registers; rows are added in shared memory, CTAs by rope_dgamma_kernel, each in a fixed order.
 template <int VEC, bool INTER>
-__global__ void __launch_bounds__(RP_THREADS) qkv_norm_rope_bwd_kernel(const RopeArgs a, const RopePlan p)
+__global__ void __launch_bounds__(RP_THREADS, RP_BWD_CTAS) qkv_norm_rope_bwd_kernel(const RopeArgs a, const RopePlan p)
 {
     constexpr int NU = VEC == 4 ? 1 : 4;
-    extern __shared__ double smem[];
-    const RopeTokens tk = rope_tokens(smem, p, a.pairs);
-    const int64_t tokens = (int64_t)a.B * a.T, blocks = (tokens + p.tok_cta - 1) / p.tok_cta;
-    const int nh = a.H + 2 * a.Hkv;
-    const int lane = threadIdx.x & 31, li = lane & (p.lpr - 1), rpw = 32 / p.lpr, step = (RP_THREADS / 32) * rpw;
+    extern __shared__ float smem[];
+    float *table = smem + (threadIdx.x >> 5) * 2 * a.pairs;
+    const int lane = threadIdx.x & 31, row = lane / p.lpr, li = lane - row * p.lpr;
     RopeUnit<VEC> u[NU];
 #pragma unroll
     for (int j = 0; j < NU; ++j) u[j] = rope_unit<VEC, INTER>(li + 32 * j, a.dk, a.pairs);
     const float inv_dk = 1.0f / (float)a.dk;
+    float cs[NU * VEC], sn[NU * VEC];
+    int angles_of = -1;
     float acc[2][2][NU][VEC];   // [q, k][piece][unit]
 #pragma unroll
     for (int w = 0; w < 2; ++w)
@@ -287,118 +419,103 @@ __global__ void __launch_bounds__(RP_THREADS) qkv_norm_rope_bwd_kernel(const Rop
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) acc[w][e][j][i] = 0.f;
 
-    for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
-        const int64_t tok0 = blk * p.tok_cta;
-        const int ntok = (int)(tokens - tok0 < p.tok_cta ? tokens - tok0 : p.tok_cta), rows = ntok * nh;
-        __syncthreads();   // the previous block's angles are still being read
-        rope_place(a, tk, tok0, ntok, a.T);
-        __syncthreads();
-        for (int w0 = (threadIdx.x >> 5) * rpw; w0 < rows; w0 += step) {
-            const int r = w0 + lane / p.lpr;
-            const bool on = r < rows;
-            const int t = on ? r / nh : 0, h = on ? r - t * nh : 0;
-            const float *src = h < a.H           ? a.q + (tk.q_row[t] + (int64_t)h * a.T) * a.dk
-                               : h < a.H + a.Hkv ? a.k + (tk.kv_row[t] + (int64_t)(h - a.H) * a.T) * a.dk
-                                                 : a.v + (tk.kv_row[t] + (int64_t)(h - a.H - a.Hkv) * a.T) * a.dk;
-            const int64_t at = ((tok0 + t) * nh + h) * a.dk;
-            const float *g = h < a.H ? a.gq : h < a.H + a.Hkv ? a.gk : nullptr;
-            Piece<VEC> d0[NU], d1[NU], x0[NU], x1[NU];
+    RopeCursor c = rope_start(a, p);
+    RopeRow nr;
+    Piece<VEC> nd0[NU], nd1[NU], nx0[NU], nx1[NU];
+    auto load = [&]() {
+        nr = rope_row(a, p, c, row);
+        const float *src = (nr.kind == ROPE_Q ? a.q : nr.kind == ROPE_K ? a.k : a.v) + nr.head;
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+            nd0[j] = load_piece<VEC>(src, u[j].v0, 0);
+            nd1[j] = load_piece<VEC>(src, u[j].v1, u[j].v0);
+        }
+        if (nr.kind == ROPE_Q ? a.gq : nr.kind == ROPE_K ? a.gk : nullptr) {
+            const float *in = a.qkv + nr.flat;
 #pragma unroll
             for (int j = 0; j < NU; ++j) {
-                d0[j] = load_piece<VEC>(src, on ? u[j].v0 : -1);
-                d1[j] = load_piece<VEC>(src, on ? u[j].v1 : -1);
-                x0[j] = load_piece<VEC>(a.qkv + at, on && g ? u[j].v0 : -1);
-                x1[j] = load_piece<VEC>(a.qkv + at, on && g ? u[j].v1 : -1);
+                nx0[j] = load_piece<VEC>(in, u[j].v0, 0);
+                nx1[j] = load_piece<VEC>(in, u[j].v1, u[j].v0);
             }
-            if (h < a.H + a.Hkv) {
+        }
+    };
+    if (c.left > 0) load();
+    while (c.left > 0) {
+        Piece<VEC> d0[NU], d1[NU], x0[NU], x1[NU];
 #pragma unroll
-                for (int j = 0; j < NU; ++j) rotate_unit<VEC, true>(u[j], tk.cs + t * a.pairs, tk.sn + t * a.pairs, d0[j], d1[j]);
+        for (int j = 0; j < NU; ++j) { d0[j] = nd0[j]; d1[j] = nd1[j]; x0[j] = nx0[j]; x1[j] = nx1[j]; }
+        const RopeRow r = nr;
+        const int tok = c.t.tok, pos = c.t.p;
+        rope_next(c, a, p);
+        if (c.left > 0) load();
+        if (r.kind != ROPE_V) {
+            if (tok != angles_of) {
+                rope_angles<VEC, INTER, NU>(a, pos, table, u, cs, sn);
+                angles_of = tok;
             }
-            if (a.gq || a.gk) {
-                if (g && a.bias) {
-                    const float *bias = a.bias + (int64_t)h * a.dk;
+#pragma unroll
+            for (int j = 0; j < NU; ++j) rotate_unit<VEC, INTER, true>(u[j], cs + j * VEC, sn + j * VEC, d0[j], d1[j]);
+            if (const float *g = r.kind == ROPE_Q ? a.gq : a.gk) {
+                if (a.bias) {
+                    const float *bias = a.bias + (r.flat - (int64_t)tok * (a.H + 2 * a.Hkv) * a.dk);
 #pragma unroll
                     for (int j = 0; j < NU; ++j) {
-                        const Piece<VEC> b0 = load_piece<VEC>(bias, on ? u[j].v0 : -1), b1 = load_piece<VEC>(bias, on ? u[j].v1 : -1);
+                        const Piece<VEC> b0 = load_piece<VEC>(bias, u[j].v0, 0), b1 = load_piece<VEC>(bias, u[j].v1, u[j].v0);
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) { x0[j].x[i] += b0.x[i]; x1[j].x[i] += b1.x[i]; }
                     }
                 }
-                Piece<VEC> g0[NU], g1[NU];
-                float ss = 0.f, sd = 0.f;   // sum x^2, sum d*g*x
-#pragma unroll
-                for (int j = 0; j < NU; ++j) {
-                    g0[j] = load_piece<VEC>(g, g ? u[j].v0 : -1);
-                    g1[j] = load_piece<VEC>(g, g ? u[j].v1 : -1);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        ss += x0[j].x[i] * x0[j].x[i] + x1[j].x[i] * x1[j].x[i];
-                        sd += d0[j].x[i] * g0[j].x[i] * x0[j].x[i] + d1[j].x[i] * g1[j].x[i] * x1[j].x[i];
-                    }
-                }
-                ss = lanes_sum(ss, p.lpr);
-                sd = lanes_sum(sd, p.lpr);
-                if (g) {
-                    const float rs = rsqrtf(ss * inv_dk + a.eps), mean = sd * rs * inv_dk;   // mean(d*g*u)
-                    const bool is_q = h < a.H;
-#pragma unroll
-                    for (int j = 0; j < NU; ++j)
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) {
-                            const float u0 = x0[j].x[i] * rs, u1 = x1[j].x[i] * rs;
-                            const float e0 = d0[j].x[i] * u0, e1 = d1[j].x[i] * u1;
-                            acc[0][0][j][i] += is_q ? e0 : 0.f;
-                            acc[0][1][j][i] += is_q ? e1 : 0.f;
-                            acc[1][0][j][i] += is_q ? 0.f : e0;
-                            acc[1][1][j][i] += is_q ? 0.f : e1;
-                            d0[j].x[i] = rs * (d0[j].x[i] * g0[j].x[i] - u0 * mean);
-                            d1[j].x[i] = rs * (d1[j].x[i] * g1[j].x[i] - u1 * mean);
-                        }
-                }
+                if (r.kind == ROPE_Q) norm_back<VEC, NU>(a, g, u, li, p.lpr, inv_dk, r.on, d0, d1, x0, x1, acc[0]);
+                else norm_back<VEC, NU>(a, g, u, li, p.lpr, inv_dk, r.on, d0, d1, x0, x1, acc[1]);
             }
-            if (!on) continue;
+        }
+        if (r.on) {
+            float *dst = a.dqkv + r.flat;
 #pragma unroll
             for (int j = 0; j < NU; ++j) {
-                store_piece<VEC>(a.dqkv + at, u[j].v0, d0[j]);
-                store_piece<VEC>(a.dqkv + at, u[j].v1, d1[j]);
+                store_piece<VEC>(dst, u[j].v0, d0[j]);
+                store_piece<VEC>(dst, u[j].v1, d1[j]);
             }
         }
     }
     if (!a.partial) return;
-    // [group][dk] per norm weight, then one thread per element adds the groups in order
-    float *red = reinterpret_cast<float *>(smem);
-    const int groups = RP_THREADS / p.lpr, group = threadIdx.x / p.lpr;
+    // [row][dk] per norm weight, then one thread per element adds the rows in order
+    const int rows = RP_WARPS * p.rpw, mine = (threadIdx.x >> 5) * p.rpw + row;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         __syncthreads();
+        if (row < p.rpw) {
 #pragma unroll
-        for (int j = 0; j < NU; ++j)
+            for (int j = 0; j < NU; ++j)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                if (u[j].v0 >= 0) red[group * a.dk + u[j].v0 * VEC + i] = acc[w][0][j][i];
-                if (u[j].v1 >= 0) red[group * a.dk + u[j].v1 * VEC + i] = acc[w][1][j][i];
-            }
+                for (int i = 0; i < VEC; ++i) {
+                    if (u[j].v0 >= 0) smem[mine * a.dk + u[j].v0 * VEC + i] = acc[w][0][j][i];
+                    if (u[j].v1 >= 0) smem[mine * a.dk + u[j].v1 * VEC + i] = acc[w][1][j][i];
+                }
+        }
         __syncthreads();
-        if (threadIdx.x < a.dk) {
+        for (int d = threadIdx.x; d < a.dk; d += RP_THREADS) {
             float s = 0.f;
-            for (int k = 0; k < groups; ++k) s += red[k * a.dk + threadIdx.x];
-            a.partial[((int64_t)blockIdx.x * 2 + w) * a.dk + threadIdx.x] = s;
+            for (int k = 0; k < rows; ++k) s += smem[k * a.dk + d];
+            a.partial[((int64_t)blockIdx.x * 2 + w) * a.dk + d] = s;
         }
     }
 }
 
-// dg[w][d] += sum over blocks of partial[block][w][d], in 64 bits and in block order within each of 32 strands
-__global__ void __launch_bounds__(1024) rope_dgamma_kernel(const float *partial, int blocks, int dk, float *dgq, float *dgk)
+// dg[w][d] += sum over blocks of partial[block][w][d], in 64 bits: 64 strands, each in block order, then in strand order
+__global__ void __launch_bounds__(512) rope_dgamma_kernel(const float *partial, int blocks, int dk, float *dgq, float *dgk)
 {
-    __shared__ double red[32][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
+    __shared__ double red[64][9];
+    const int x = threadIdx.x & 7, c = blockIdx.x * 8 + x, strand = threadIdx.x >> 3;
     double s = 0.0;
-    if (c < 2 * dk)
-        for (int b = strand; b < blocks; b += 32) s += (double)partial[(int64_t)b * 2 * dk + c];
-    red[strand][threadIdx.x & 31] = s;
+    if (c < 2 * dk) {
+#pragma unroll 8
+        for (int b = strand; b < blocks; b += 64) s += (double)partial[(int64_t)b * 2 * dk + c];
+    }
+    red[strand][x] = s;
     __syncthreads();
     if (strand == 0 && c < 2 * dk) {
-        for (int k = 1; k < 32; ++k) s += red[k][threadIdx.x];
+        for (int k = 1; k < 64; ++k) s += red[k][x];
         float *dst = c < dk ? dgq : dgk;
         const int d = c < dk ? c : c - dk;
         if (dst) dst[d] = (float)((double)dst[d] + s);
@@ -420,41 +537,37 @@ static bool rope_vec(const RopeArgs &a, const float *dgq, const float *dgk)
 static RopePlan rope_plan(const RopeArgs &a, bool vec, int sm_count, bool backward)
 {
     RopePlan p;
-    const int heads = a.H + 2 * a.Hkv;
     p.lpr = 32;
-    if (vec) {
-        const int units = a.interleaved ? (a.dk / 4 + 1) / 2 : a.pairs / 4 + (a.dk / 4 - a.pairs / 2 + 1) / 2;
-        p.lpr = 1;
-        while (p.lpr < units) p.lpr <<= 1;
-    }
-    const int groups = RP_THREADS / p.lpr;
-    const int64_t tokens = (int64_t)a.B * a.T;
-    // Tokens per CTA: eight rows a group at least (the angles and the tokens' places cost a barrier), while every SM keeps
-    // eight CTAs' worth of rows.
-    p.tok_cta = 1;
-    while (p.tok_cta < 16 && p.tok_cta * heads < 8 * groups && tokens >= (int64_t)2 * p.tok_cta * 8 * sm_count) p.tok_cta *= 2;
-    p.heads_cta = heads;
+    if (vec) p.lpr = a.interleaved ? (a.dk / 4 + 1) / 2 : a.pairs / 4 + (a.dk / 4 - a.pairs / 2 + 1) / 2;
+    p.rpw = 32 / p.lpr;
+    p.sq = (a.H + p.rpw - 1) / p.rpw;
+    p.sk = (a.Hkv + p.rpw - 1) / p.rpw;
+    p.steps = p.sq + 2 * p.sk;
+    const int64_t steps = (int64_t)a.B * a.T * p.steps, need = (steps + RP_WARPS - 1) / RP_WARPS;
+    // One set of resident CTAs; where that leaves a warp more than 16 steps, up to four sets, so that an SM that is done early
+    // takes more (the forward of 16384 tokens above: one set 148 us, two 136, four 134; 768 tokens: 7.8, 8.6 and 11.1).  The
+    // backward keeps to one, every CTA of it being a term of the norm weights' sums.
+    int64_t most = (int64_t)sm_count * (backward ? RP_BWD_CTAS : RP_FWD_CTAS);
     if (!backward) {
-        // few tokens: the heads of a token are dealt out too, down to one row a group
-        while (p.heads_cta > groups && (tokens + p.tok_cta - 1) / p.tok_cta * ((heads + p.heads_cta - 1) / p.heads_cta) < 4 * sm_count)
-            p.heads_cta = (p.heads_cta + 1) / 2;
+        const int64_t sets = need / (16 * most);
+        most *= sets < 1 ? 1 : sets > 4 ? 4 : sets;
     }
+    p.blocks = (int)(need < most ? need : most);
     return p;
 }
 
 static size_t rope_smem(const RopeArgs &a, const RopePlan &p, bool backward)
 {
-    size_t n = (size_t)p.tok_cta * (2 * sizeof(int64_t) + 2 * (size_t)a.pairs * sizeof(float));
-    const size_t red = backward ? (size_t)(RP_THREADS / p.lpr) * a.dk * sizeof(float) : 0;
-    return n > red ? n : red;   // at most 33 KB (16 tokens of 128 pairs)
+    const size_t n = RP_WARPS * 2 * (size_t)a.pairs * sizeof(float);
+    const size_t red = backward ? RP_WARPS * (size_t)p.rpw * a.dk * sizeof(float) : 0;
+    return n > red ? n : red;   // at most 8 KB
 }
 
 int launch_qkv_norm_rope(const RopeArgs &a, int sm_count, cudaStream_t st)
 {
     const bool vec = rope_vec(a, nullptr, nullptr);
     const RopePlan p = rope_plan(a, vec, sm_count, false);
-    const int64_t blocks = ((int64_t)a.B * a.T + p.tok_cta - 1) / p.tok_cta;
-    const dim3 grid((unsigned)blocks, (unsigned)((a.H + 2 * a.Hkv + p.heads_cta - 1) / p.heads_cta));
+    const int grid = p.blocks;
     const size_t smem = rope_smem(a, p, false);
     if (vec && a.interleaved) qkv_norm_rope_kernel<4, true><<<grid, RP_THREADS, smem, st>>>(a, p);
     else if (vec) qkv_norm_rope_kernel<4, false><<<grid, RP_THREADS, smem, st>>>(a, p);
@@ -463,23 +576,16 @@ int launch_qkv_norm_rope(const RopeArgs &a, int sm_count, cudaStream_t st)
     return (int)cudaGetLastError();
 }
 
-static int bwd_blocks(const RopeArgs &a, const RopePlan &p, int sm_count)
-{
-    const int64_t blocks = ((int64_t)a.B * a.T + p.tok_cta - 1) / p.tok_cta;
-    const int64_t most = (int64_t)sm_count * 4;
-    return (int)(blocks < most ? blocks : most);
-}
-
 int qkv_norm_rope_bwd_blocks(const RopeArgs &a, int sm_count)
 {
-    return bwd_blocks(a, rope_plan(a, rope_vec(a, nullptr, nullptr), sm_count, true), sm_count);
+    return rope_plan(a, rope_vec(a, nullptr, nullptr), sm_count, true).blocks;
 }
 
 int launch_qkv_norm_rope_bwd(const RopeArgs &a, float *dgq, float *dgk, int sm_count, cudaStream_t st, int *launches)
 {
     const bool vec = rope_vec(a, nullptr, nullptr);
     const RopePlan p = rope_plan(a, vec, sm_count, true);
-    const int grid = bwd_blocks(a, p, sm_count);
+    const int grid = p.blocks;
     const size_t smem = rope_smem(a, p, true);
     if (vec && a.interleaved) qkv_norm_rope_bwd_kernel<4, true><<<grid, RP_THREADS, smem, st>>>(a, p);
     else if (vec) qkv_norm_rope_bwd_kernel<4, false><<<grid, RP_THREADS, smem, st>>>(a, p);
@@ -488,7 +594,7 @@ int launch_qkv_norm_rope_bwd(const RopeArgs &a, float *dgq, float *dgk, int sm_c
     *launches = 1;
     int e = (int)cudaGetLastError();
     if (e || !a.partial) return e;
-    rope_dgamma_kernel<<<(2 * a.dk + 31) / 32, 1024, 0, st>>>(a.partial, grid, a.dk, dgq, dgk);
+    rope_dgamma_kernel<<<(2 * a.dk + 7) / 8, 512, 0, st>>>(a.partial, grid, a.dk, dgq, dgk);
     *launches = 2;
     return (int)cudaGetLastError();
 }

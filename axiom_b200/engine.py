@@ -16,6 +16,7 @@ ENGINE_SO = os.path.join(PKG, "lib", "libaxiom_b200.so")
 
 ACT = {"none": 0, None: 0, "relu": 1, "gelu": 2}
 ROPE_SCALING = {"none": 0, None: 0, "linear": 1, "turns": 2, "index": 3}
+_TYPE_NAME = {}   # element types met so far, by name
 ROPE_PAIRING = {"half": 0, "interleaved": 1}
 FP32_MODES = {"3xtf32": 0, "bf16x3": 1, "bf16": 2}
 
@@ -405,56 +406,70 @@ class Engine:
         self._check(self.lib.axb_rope_frequencies(rot, base, ROPE_SCALING[scaling], factor, low, high, original_len, out))
         return list(out[:rot // 2])
 
+    # (These calls run in a few microseconds on the device: what is written here more tersely than elsewhere is what made
+    # half of a small call's time.  Messages are formed where they are needed.)
     @staticmethod
-    def _addr(t, dtype=None):
-        # dtype: the name of the element type a buffer must have ("float32" unless said otherwise)
-        if t is None or isinstance(t, int):
+    def _addr(t, dtype="float32"):
+        # dtype: the name of the element type a buffer must have
+        if t is None or t.__class__ is int:
             return t
-        if not t.is_contiguous() or str(t.dtype) != "torch." + (dtype or "float32"):
-            raise ValueError(f"a contiguous {dtype or 'float32'} tensor is wanted, got {t.dtype}, strides {tuple(t.stride())}")
+        if _TYPE_NAME.get(t.dtype) != dtype:
+            if _TYPE_NAME.setdefault(t.dtype, str(t.dtype)[6:]) != dtype:   # ("torch.float32": the binding imports no torch)
+                raise ValueError(f"a {dtype} tensor is wanted, got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"a contiguous tensor is wanted, got strides {tuple(t.stride())}")
+        if not t.is_cuda:
+            raise ValueError(f"a tensor on the engine's device is wanted, got {t.device}")
         return t.data_ptr()
 
-    def _rope(self, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos):
-        p = self._addr
+    @staticmethod
+    def _wants(what):
+        raise ValueError(what)
+
+    def _rope(self, rows, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos):
+        width, p = (H + 2 * Hkv) * dk, self._addr
+        if qkv is not None and qkv.shape != (rows, width) and not qkv.shape[0] == rows == 0:
+            self._wants(f"qkv: [{rows}, {width}] is wanted")
+        if bias is not None and bias.numel() != width:
+            self._wants(f"bias: [{width}] is wanted")
+        if (gq is not None and gq.numel() != dk) or (gk is not None and gk.numel() != dk):
+            self._wants(f"norm weights: [{dk}] is wanted")
+        if pos is not None and pos.numel() != rows:
+            self._wants(f"pos: {rows} positions are wanted")
         return (p(qkv), p(bias), p(gq), p(gk), eps, p(freq, "float64"), 0 if freq is None else 2 * freq.numel(), ROPE_PAIRING[pairing],
                 amplitude, p(pos, "int32"))
 
-    @staticmethod
-    def _shape(ok, what):
-        if not ok:
-            raise ValueError(what)
-
-    def _check_rope(self, rows, H, Hkv, dk, qkv, bias, gq, gk, pos):
-        width = (H + 2 * Hkv) * dk
-        self._shape(qkv is None or tuple(qkv.shape) == (rows, width) or qkv.shape[0] == rows == 0, f"qkv: [{rows}, {width}] is wanted")
-        self._shape(bias is None or bias.numel() == width, f"bias: [{width}] is wanted")
-        self._shape(all(g is None or g.numel() == dk for g in (gq, gk)), f"norm weights: [{dk}] is wanted")
-        self._shape(pos is None or pos.numel() == rows, f"pos: {rows} positions are wanted")
+    def _heads(self, B, Q, K, V, names):
+        # (sequences' heads, key heads, tokens, rows of a key head, head dim) of head-major buffers
+        (BH, T, dk), shape = Q.shape, K.shape
+        H, Hkv = (BH // B, shape[0] // B) if B else (1, 1)
+        if B * H != BH or B * Hkv != shape[0] or shape != V.shape or shape[2] != dk:
+            self._wants(f"{names}: head-major shapes")
+        return H, Hkv, T, shape[1], dk
 
     def qkv_norm_rope(self, qkv, Qh, Kh, Vh, B, bias=None, gq=None, gk=None, eps=1e-6, freq=None, pairing="half", amplitude=1.0,
                       pos=None):
         """qkv [B*S, (H + 2*Hkv)*dk] -> head-major Qh [B*H, S, dk], Kh, Vh [B*Hkv, S, dk]: bias, per-head RMS norm, rotation."""
-        (BH, S, dk), BHkv = Qh.shape, Kh.shape[0]
-        H, Hkv = (BH // B, BHkv // B) if B else (1, 1)
-        self._shape(B * H == BH and B * Hkv == BHkv and tuple(Kh.shape) == tuple(Vh.shape) == (BHkv, S, dk), "Qh, Kh, Vh: head-major shapes")
-        self._check_rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, pos)
+        H, Hkv, S, rows, dk = self._heads(B, Qh, Kh, Vh, "Qh, Kh, Vh")
+        if rows != S:
+            self._wants("Qh, Kh, Vh: head-major shapes")
         p = self._addr
-        self._check(self.lib.axb_qkv_norm_rope(*self._rope(qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos), B, S, H, Hkv, dk,
-                                               p(Qh), p(Kh), p(Vh)))
+        self._check(self.lib.axb_qkv_norm_rope(*self._rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos),
+                                               B, S, H, Hkv, dk, p(Qh), p(Kh), p(Vh)))
         return Qh, Kh, Vh
 
     def qkv_norm_rope_bwd(self, dQh, dKh, dVh, dqkv, B, qkv=None, bias=None, gq=None, gk=None, eps=1e-6, freq=None, pairing="half",
                           amplitude=1.0, pos=None, dgq=None, dgk=None, workspace=None):
         """dqkv from the head-major gradients; dgq, dgk (the norm weights' gradients) are added to."""
-        (BH, S, dk), BHkv = dQh.shape, dKh.shape[0]
-        H, Hkv = (BH // B, BHkv // B) if B else (1, 1)
-        self._shape(B * H == BH and B * Hkv == BHkv and tuple(dKh.shape) == tuple(dVh.shape) == (BHkv, S, dk), "dQh, dKh, dVh: head-major shapes")
-        self._check_rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, pos)
-        self._shape(tuple(dqkv.shape) == (B * S, (H + 2 * Hkv) * dk) and all(g is None or g.numel() == dk for g in (dgq, dgk)),
-                    "dqkv, dgq, dgk: shapes")
+        H, Hkv, S, rows, dk = self._heads(B, dQh, dKh, dVh, "dQh, dKh, dVh")
+        if rows != S:
+            self._wants("dQh, dKh, dVh: head-major shapes")
+        if dqkv.shape != (B * S, (H + 2 * Hkv) * dk) or any(g is not None and g.numel() != dk for g in (dgq, dgk)):
+            self._wants("dqkv, dgq, dgk: shapes")
         p = self._addr
-        self._check(self.lib.axb_qkv_norm_rope_bwd(*self._rope(qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos), p(dQh), p(dKh), p(dVh),
-                                                   B, S, H, Hkv, dk, p(dqkv), p(dgq), p(dgk), self._workspace(workspace)))
+        self._check(self.lib.axb_qkv_norm_rope_bwd(*self._rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos),
+                                                   p(dQh), p(dKh), p(dVh), B, S, H, Hkv, dk, p(dqkv), p(dgq), p(dgk),
+                                                   self._workspace(workspace)))
         return dqkv
 
     def attention_workspace_bytes(self):
@@ -466,37 +481,41 @@ class Engine:
     def _workspace(self, ws):
         if ws is None or isinstance(ws, int):
             return ws
-        self._shape(ws.is_contiguous() and ws.numel() * ws.element_size() >= self.attention_workspace_bytes(), "workspace: too small")
+        if not ws.is_contiguous() or ws.numel() * ws.element_size() < self.attention_workspace_bytes():
+            self._wants("workspace: too small")
         return ws.data_ptr()
 
     def kv_cache_extend(self, qkv, Qh, K_cache, V_cache, lens, n_new=None, bias=None, gq=None, gk=None, eps=1e-6, freq=None,
                         pairing="half", amplitude=1.0, pos=None):
         """The tokens qkv [B*T, (H + 2*Hkv)*dk] of a ragged batch: queries to Qh [B*H, T, dk], keys and values to cache rows
         lens[b] + t of K_cache, V_cache [B*Hkv, max_seq, dk]."""
-        B, (BH, T, dk), (BHkv, max_seq, _) = lens.numel(), Qh.shape, K_cache.shape
-        H, Hkv = (BH // B, BHkv // B) if B else (1, 1)
-        self._shape(B * H == BH and B * Hkv == BHkv and tuple(K_cache.shape) == tuple(V_cache.shape) == (BHkv, max_seq, dk),
-                    "Qh, K_cache, V_cache: head-major shapes")
-        self._check_rope(B * T, H, Hkv, dk, qkv, bias, gq, gk, pos)
-        self._shape(n_new is None or n_new.numel() == B, "n_new: one count for each sequence")
+        B = lens.numel()
+        H, Hkv, T, max_seq, dk = self._heads(B, Qh, K_cache, V_cache, "Qh, K_cache, V_cache")
+        if n_new is not None and n_new.numel() != B:
+            self._wants("n_new: one count for each sequence")
         p = self._addr
-        self._check(self.lib.axb_kv_cache_extend(*self._rope(qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos), p(lens, "int32"),
-                                                 p(n_new, "int32"), B, T, H, Hkv, max_seq, dk, p(Qh), p(K_cache), p(V_cache)))
+        self._check(self.lib.axb_kv_cache_extend(*self._rope(B * T, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos),
+                                                 p(lens, "int32"), p(n_new, "int32"), B, T, H, Hkv, max_seq, dk, p(Qh), p(K_cache),
+                                                 p(V_cache)))
         return Qh
 
     def kv_cache_attend_tree(self, K_cache, V_cache, Q, out, lens, scale, n_new=None, mask=None, workspace=None):
         """Attention of Q [B*H, T, dk] over cache rows [0, lens[b]) and the new rows lens[b] + j that mask (int64 bit words
         [B, T, ceil(T/64)], or [T, ceil(T/64)] for all sequences; None: j <= t) lets token t see."""
-        B, (BH, T, dk), (BHkv, max_seq, _) = lens.numel(), Q.shape, K_cache.shape
-        H, Hkv = (BH // B, BHkv // B) if B else (1, 1)
-        self._shape(B * H == BH and B * Hkv == BHkv and tuple(K_cache.shape) == tuple(V_cache.shape) == (BHkv, max_seq, dk) and
-                    tuple(out.shape) == tuple(Q.shape), "Q, out, K_cache, V_cache: head-major shapes")
-        words = (T + 63) // 64
-        self._shape(mask is None or tuple(mask.shape) in ((B, T, words), (T, words)), f"mask: [{B}, {T}, {words}] or [{T}, {words}] is wanted")
-        self._shape(n_new is None or n_new.numel() == B, "n_new: one count for each sequence")
+        B = lens.numel()
+        H, Hkv, T, max_seq, dk = self._heads(B, Q, K_cache, V_cache, "Q, K_cache, V_cache")
+        if out.shape != Q.shape:
+            self._wants("out: the shape of Q is wanted")
+        each = 0   # a mask for every sequence
+        if mask is not None:
+            words, each = (T + 63) // 64, int(mask.dim() == 3)
+            if mask.shape != ((B, T, words) if each else (T, words)):
+                self._wants(f"mask: [{B}, {T}, {words}] or [{T}, {words}] is wanted")
+        if n_new is not None and n_new.numel() != B:
+            self._wants("n_new: one count for each sequence")
         p = self._addr
-        self._check(self.lib.axb_kv_cache_attend_tree(p(K_cache), p(V_cache), p(Q), p(mask, "int64"), int(mask is not None and mask.dim() == 3),
-                                                      p(lens, "int32"), p(n_new, "int32"), p(out), B, H, Hkv, T, max_seq, dk, scale,
+        self._check(self.lib.axb_kv_cache_attend_tree(p(K_cache), p(V_cache), p(Q), p(mask, "int64"), each, p(lens, "int32"),
+                                                      p(n_new, "int32"), p(out), B, H, Hkv, T, max_seq, dk, scale,
                                                       self._workspace(workspace)))
         return out
 
@@ -504,8 +523,9 @@ class Engine:
         """Cache rows lens[b] + keep[b, i] move to lens[b] + i for i < n_keep[b]; lens_out[b] = lens[b] + n_keep[b]."""
         B, T, (BHkv, max_seq, dk) = lens.numel(), keep.shape[-1], K_cache.shape
         Hkv = BHkv // B if B else 1
-        self._shape(B * Hkv == BHkv and tuple(K_cache.shape) == tuple(V_cache.shape) and keep.numel() == B * T and n_keep.numel() == B and
-                    (lens_out is None or lens_out.numel() == B), "K_cache, V_cache, keep, n_keep, lens_out: shapes")
+        if (B * Hkv != BHkv or K_cache.shape != V_cache.shape or keep.numel() != B * T or n_keep.numel() != B or
+                (lens_out is not None and lens_out.numel() != B)):
+            self._wants("K_cache, V_cache, keep, n_keep, lens_out: shapes")
         p = self._addr
         self._check(self.lib.axb_kv_cache_compact(p(K_cache), p(V_cache), p(keep, "int32"), p(n_keep, "int32"), p(lens, "int32"),
                                                   p(lens_out, "int32"), B, Hkv, T, max_seq, dk))
