@@ -25,20 +25,23 @@
 
 namespace axb {
 
-static constexpr int TT_ROWS = 128, TT_THREADS = 640;
+static constexpr int TT_THREADS = 640;
 enum { CERR_LOAD = 94, CERR_CONVERT = 95, CERR_MMA = 96, CERR_SOFTMAX = 97 };
 
-template <int NSLAB>
+template <int NSLAB, bool FEW>
 struct TreeTc {
     static constexpr bool WIDE = NSLAB > 2;
+    static constexpr int ROWS = FEW ? 64 : 128;                // query rows (a product has 128 either way)
+    static constexpr int SOFTMAX = 2 * ROWS;                   // threads at work on them
     static constexpr int DKP = 32 * NSLAB;
     static constexpr int KB = WIDE ? 64 : 128;                 // keys of a block
-    static constexpr int QSLAB = TT_ROWS * 128, SLAB = KB * 128;   // bytes of 32 columns
+    static constexpr int QSLAB = ROWS * 128, SLAB = KB * 128;   // bytes of 32 columns
     static constexpr int QPLANE = NSLAB * QSLAB, PLANE = NSLAB * SLAB;
-    static constexpr int KS = WIDE ? 2 : 1, VS = WIDE ? 1 : 2; // raw buffers
+    static constexpr int KS = WIDE || FEW ? 2 : 1, VS = WIDE && !FEW ? 1 : 2; // raw buffers
     static constexpr int OB = WIDE ? 1 : 2;                    // accumulators of P.V
+    static constexpr int SB = WIDE ? 2 : 1;                    // score buffers
     // tensor memory columns
-    static constexpr int T_S = 0, T_PLO = 2 * KB, T_O = 3 * KB, T_QLO = T_O + OB * DKP;
+    static constexpr int T_S = 0, T_P = SB * KB, T_PLO = T_P + KB, T_O = T_PLO + KB, T_QLO = T_O + OB * DKP;
     static constexpr int COLS = 512;
     static_assert(T_QLO + (WIDE ? DKP : 0) <= COLS, "tensor memory");
     static constexpr int HEADER = 3072;   // barriers, words, then the softmax threads' maxima
@@ -49,7 +52,8 @@ struct TreeTc {
 
 enum {
     TB_Q_FULL, TB_Q_EMPTY, TB_K_RAW, TB_K_FULL = TB_K_RAW + 2, TB_K_EMPTY, TB_V_RAW = TB_K_EMPTY + 2, TB_V_FULL = TB_V_RAW + 2, TB_V_EMPTY,
-    TB_S_FULL = TB_V_EMPTY + 2, TB_P_FULL = TB_S_FULL + 2, TB_PLO_FULL = TB_P_FULL + 2, TB_KLO_EMPTY, TB_VLO_EMPTY, TB_O_FULL, TB_O_EMPTY = TB_O_FULL + 2, TB_DRAIN = TB_O_EMPTY + 2,
+    TB_S_FULL = TB_V_EMPTY + 2, TB_S_EMPTY = TB_S_FULL + 2, TB_P_FULL = TB_S_EMPTY + 2, TB_PLO_FULL, TB_KLO_EMPTY, TB_VLO_EMPTY, TB_O_FULL,
+    TB_O_EMPTY, TB_DRAIN = TB_O_EMPTY + 2,
     TB_COUNT = TB_DRAIN + 2
 };
 
@@ -65,12 +69,14 @@ __device__ __forceinline__ uint32_t lo_bits(uint32_t x)
 // the three products of a block's scores / outputs, issued by one thread.  B: block parity.  Everything that an instruction
 // names is a constant offset from the bases, so that it takes no moves into the registers that tcgen05.mma reads (with
 // addresses formed at run time an instruction cost the issuing thread 110 cycles where the pipe takes 48 to 64).
-template <int NSLAB, int B>
+template <int NSLAB, bool FEW, int B>
 __device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, uint32_t idesc, uint32_t klo_empty)
 {
-    using C = TreeTc<NSLAB>;
+    using C = TreeTc<NSLAB, FEW>;
     const uint64_t dk = smem_desc_kmajor(0, 128);
-    auto desc = [&](uint32_t at) { return dk | (uint64_t)(((base + at) & 0x3FFFFu) >> 4); };
+    uint32_t b0 = (base & 0x3FFFFu) >> 4;
+    asm volatile("" : "+r"(b0));
+    auto desc = [&](uint32_t at) { return (dk & 0xFFFFFFFF00000000ull) | ((uint32_t)dk + b0 + (at >> 4)); };
     constexpr uint32_t khi = C::K_AT + (B % C::KS) * C::PLANE;
 #pragma unroll
     for (int pr = 0; pr < 3; ++pr) {   // hi.lo, whose lo tile the next block waits for, lo.hi, hi.hi
@@ -78,31 +84,30 @@ __device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, uint3
 #pragma unroll
         for (int ks = 0; ks < 4 * NSLAB; ++ks) {   // (columns from dk on are zero)
             const uint64_t bd = desc(kk + (ks >> 2) * C::SLAB + (ks & 3) * 32);
-            if (C::WIDE && pr == 1) tc_mma_ts_tf32(tmem + C::T_S + B * C::KB, tmem + C::T_QLO + ks * 8, bd, idesc, 1);
-            else tc_mma<KIND_TF32>(tmem + C::T_S + B * C::KB, desc(qq + (ks >> 2) * C::QSLAB + (ks & 3) * 32), bd, idesc, pr | ks);
+            if (C::WIDE && pr == 1) tc_mma_ts_tf32(tmem + C::T_S + (B % C::SB) * C::KB, tmem + C::T_QLO + ks * 8, bd, idesc, 1);
+            else tc_mma<KIND_TF32>(tmem + C::T_S + (B % C::SB) * C::KB, desc(qq + (ks >> 2) * C::QSLAB + (ks & 3) * 32), bd, idesc, pr | ks);
         }
         if (pr == 0) tc_commit(klo_empty);
     }
 }
 
-// part 0: hi.lo and hi.hi; part 1: lo.hi, whose operand comes last
-template <int NSLAB, int B, int PART>
+// part 0: hi.lo, whose lo tile the next block waits for, and hi.hi; part 1: lo.hi, whose operand comes last
+template <int NSLAB, bool FEW, int B, int PART>
 __device__ __forceinline__ void issue_outputs(uint32_t base, uint32_t tmem, uint32_t idesc, uint32_t vlo_empty)
 {
-    using C = TreeTc<NSLAB>;
+    using C = TreeTc<NSLAB, FEW>;
     const uint64_t dm = smem_desc_mnmajor_sw128_32b(0, C::SLAB, 512);
-    auto desc = [&](uint32_t at) { return dm | (uint64_t)(((base + at) & 0x3FFFFu) >> 4); };
+    uint32_t b0 = (base & 0x3FFFFu) >> 4;
+    asm volatile("" : "+r"(b0));
+    auto desc = [&](uint32_t at) { return (dm & 0xFFFFFFFF00000000ull) | ((uint32_t)dm + b0 + (at >> 4)); };
     constexpr uint32_t vhi = C::V_AT + (B % C::VS) * C::PLANE;
     const uint32_t d = tmem + C::T_O + (B % C::OB) * C::DKP;
-    if (PART == 0) {
 #pragma unroll
-        for (int ks = 0; ks < C::KB / 8; ++ks) tc_mma_ts_tf32(d, tmem + C::T_S + B * C::KB + ks * 8, desc(C::VLO_AT + ks * 1024), idesc, ks);
-        tc_commit(vlo_empty);
+    for (int pr = PART ? 2 : 0; pr < (PART ? 3 : 2); ++pr) {
 #pragma unroll
-        for (int ks = 0; ks < C::KB / 8; ++ks) tc_mma_ts_tf32(d, tmem + C::T_S + B * C::KB + ks * 8, desc(vhi + ks * 1024), idesc, 1);
-    } else {
-#pragma unroll
-        for (int ks = 0; ks < C::KB / 8; ++ks) tc_mma_ts_tf32(d, tmem + C::T_PLO + ks * 8, desc(vhi + ks * 1024), idesc, 1);
+        for (int ks = 0; ks < C::KB / 8; ++ks)
+            tc_mma_ts_tf32(d, tmem + (pr == 2 ? C::T_PLO : C::T_P) + ks * 8, desc((pr == 0 ? C::VLO_AT : vhi) + ks * 1024), idesc, pr | ks);
+        if (pr == 0) tc_commit(vlo_empty);
     }
 }
 
@@ -128,11 +133,11 @@ __device__ __forceinline__ uint32_t seen_bits(const KvTreeArgs &a, int b, int t,
     return skip ? (bits << skip) | ((1u << skip) - 1u) : bits;
 }
 
-template <int NSLAB>
+template <int NSLAB, bool FEW>
 __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ TreeTcMaps tm)
 {
-    using C = TreeTc<NSLAB>;
-    constexpr int KB = C::KB, OH = C::DKP / 2;   // OH: output columns of a softmax thread
+    using C = TreeTc<NSLAB, FEW>;
+    constexpr int ROWS = C::ROWS, KB = C::KB, OH = C::DKP / 2, FOLD = OH % 32 || C::WIDE ? 16 : 32;   // OH: output columns of a softmax thread
     extern __shared__ __align__(1024) uint8_t sm[];
     const uint32_t base = smem_u32(sm);
     auto bar = [&](int i) -> uint32_t { return base + 8u * (uint32_t)i; };
@@ -140,8 +145,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(sm + 288);
     volatile int *words = reinterpret_cast<volatile int *>(sm + 304);
     volatile int &s_gave_up = words[0], &s_last = words[1], *s_odd = words + 2;   // s_odd: block it + 1 holds non-finite new values
-    int *s_row = reinterpret_cast<int *>(sm + 512);   // [TT_ROWS]
-    float (*s_max)[2][TT_ROWS] = reinterpret_cast<float (*)[2][TT_ROWS]>(sm + 1024);   // [block parity][half][row]
+    int *s_row = reinterpret_cast<int *>(sm + 512);   // [ROWS]
+    float (*s_max)[2][ROWS] = reinterpret_cast<float (*)[2][ROWS]>(sm + 1024);   // [block parity][half][row]
     if (base & 1023) {   // the swizzles are functions of the address (it starts at a multiple of 1 KB; refused, should it ever not)
         if (threadIdx.x == 0 && a.err) atomicCAS(a.err, 0, (int)CERR_LOAD);
         return;
@@ -154,16 +159,17 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
         mbar_init(bar(TB_Q_FULL), 256);
         mbar_init(bar(TB_K_FULL), 256);
         mbar_init(bar(TB_V_FULL), 256);
-        mbar_init(bar(TB_PLO_FULL), 256);
+        mbar_init(bar(TB_P_FULL), C::SOFTMAX);
+        mbar_init(bar(TB_PLO_FULL), C::SOFTMAX);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(TB_P_FULL + i), 256);
-            mbar_init(bar(TB_O_EMPTY + i), 256);
+            mbar_init(bar(TB_S_EMPTY + i), C::SOFTMAX);
+            mbar_init(bar(TB_O_EMPTY + i), C::SOFTMAX);
         }
         mbar_fence_init();
         s_gave_up = 0;
         for (int i = 0; i < 4; ++i) s_odd[i] = 0;
     }
-    constexpr TreeLine line = { TT_ROWS, KB, 1 };
+    constexpr TreeLine line = { ROWS, KB, 1 };
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;
     if (warp == 19) {
@@ -222,40 +228,38 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
             }
         } else if (warp == 18 && lane == 0) {
             // ----------------------------------------------------- scores
-            const uint32_t idesc = make_idesc<KIND_TF32>(TT_ROWS, KB);
+            const uint32_t idesc = make_idesc<KIND_TF32>(128, KB);
             while (ok && next_piece(a, line, cur, p)) {
                 if (!wait(TB_Q_FULL, np & 1)) { ok = false; break; }
                 ++np;
                 for (int i = 0; i < p.count; ++i, ++it) {
-                    const uint32_t b = it & 1;
-                    // score buffer b held P hi of block it - 2, the A operand of that block's product
-                    if (it >= 2 && !wait(TB_O_FULL + b, ((it - 2) >> 1) & 1)) { ok = false; break; }
+                    // the softmax threads have the scores of block it - SB in registers
+                    if (it >= C::SB && !wait(TB_S_EMPTY + it % C::SB, (it / C::SB - 1) & 1)) { ok = false; break; }
                     if (!wait(TB_K_FULL, it & 1)) { ok = false; break; }
                     tc_fence_after_sync();
-                    if (b) issue_scores<NSLAB, 1>(base, tmem, idesc, bar(TB_KLO_EMPTY));
-                    else issue_scores<NSLAB, 0>(base, tmem, idesc, bar(TB_KLO_EMPTY));
-                    tc_commit(bar(TB_S_FULL + b));
+                    if (it & 1) issue_scores<NSLAB, FEW, 1>(base, tmem, idesc, bar(TB_KLO_EMPTY));
+                    else issue_scores<NSLAB, FEW, 0>(base, tmem, idesc, bar(TB_KLO_EMPTY));
+                    tc_commit(bar(TB_S_FULL + it % C::SB));
                     tc_commit(bar(TB_K_EMPTY + it % C::KS));
                     if (i == p.count - 1) tc_commit(bar(TB_Q_EMPTY));
                 }
             }
         } else if (warp == 19 && lane == 0) {
             // ----------------------------------------------------- outputs
-            const uint32_t idesc = make_idesc<KIND_TF32>(TT_ROWS, (a.dk + 15) / 16 * 16) | (1u << 16);   // B is MN-major
+            const uint32_t idesc = make_idesc<KIND_TF32>(128, (a.dk + 15) / 16 * 16) | (1u << 16);   // B is MN-major
             while (ok && next_piece(a, line, cur, p)) {
                 for (int i = 0; i < p.count; ++i, ++it) {
-                    const uint32_t b = it & 1;
-                    if (!wait(TB_P_FULL + b, (it >> 1) & 1)) { ok = false; break; }
+                    if (!wait(TB_P_FULL, it & 1)) { ok = false; break; }
                     if (!wait(TB_V_FULL, it & 1)) { ok = false; break; }
                     if (it >= C::OB && !wait(TB_O_EMPTY + it % C::OB, (it / C::OB - 1) & 1)) { ok = false; break; }
                     tc_fence_after_sync();
-                    if (b) issue_outputs<NSLAB, 1, 0>(base, tmem, idesc, bar(TB_VLO_EMPTY));
-                    else issue_outputs<NSLAB, 0, 0>(base, tmem, idesc, bar(TB_VLO_EMPTY));
+                    if (it & 1) issue_outputs<NSLAB, FEW, 1, 0>(base, tmem, idesc, bar(TB_VLO_EMPTY));
+                    else issue_outputs<NSLAB, FEW, 0, 0>(base, tmem, idesc, bar(TB_VLO_EMPTY));
                     if (!wait(TB_PLO_FULL, it & 1)) { ok = false; break; }
                     tc_fence_after_sync();
-                    if (b) issue_outputs<NSLAB, 1, 1>(base, tmem, idesc, 0);
-                    else issue_outputs<NSLAB, 0, 1>(base, tmem, idesc, 0);
-                    tc_commit(bar(TB_O_FULL + b));
+                    if (it & 1) issue_outputs<NSLAB, FEW, 1, 1>(base, tmem, idesc, 0);
+                    else issue_outputs<NSLAB, FEW, 0, 1>(base, tmem, idesc, 0);
+                    tc_commit(bar(TB_O_FULL));
                     tc_commit(bar(TB_V_EMPTY + it % C::VS));
                 }
             }
@@ -323,14 +327,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
             if (np && !wait_all(TB_Q_EMPTY, (np - 1) & 1)) { ok = false; break; }
             ++np;
             // the piece's query rows: row r of the key head is head r / n, token r % n.  s_row: rows of Q from the key head's first
-            if (ct < TT_ROWS) {
-                const int r = p.block * TT_ROWS + ct, gh = r / p.s.n;
+            if (ct < ROWS) {
+                const int r = p.block * ROWS + ct, gh = r / p.s.n;
                 s_row[ct] = r < p.s.rows ? gh * a.T + (r - gh * p.s.n) : -1;
             }
             conv_sync();
             const float *q0 = a.Q + ((int64_t)p.b * a.H + p.hk * heads_per) * a.T * a.dk;
 #pragma unroll 4
-            for (int i = ct; i < TT_ROWS * (C::DKP / 4); i += 256) {
+            for (int i = ct; i < ROWS * (C::DKP / 4); i += 256) {
                 const int r = i / (C::DKP / 4), c = i - r * (C::DKP / 4), row = s_row[r];
                 const bool get = row >= 0 && 4 * c < a.dk;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + C::Q_AT + (c >> 3) * C::QSLAB + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
@@ -340,7 +344,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
             asm volatile("cp.async.wait_all;" ::: "memory");
             if (C::WIDE) {
                 conv_sync();
-                if (ct < TT_ROWS) {   // thread = row: lane of tensor memory
+                if (ct < ROWS) {   // thread = row: lane of tensor memory
                     const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::T_QLO;
 #pragma unroll 1
                     for (int sl = 0; sl < NSLAB; ++sl) {
@@ -357,7 +361,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
                 }
             } else {
 #pragma unroll 4
-                for (int i = ct; i < TT_ROWS * (C::DKP / 4); i += 256) {   // (the pieces this thread brought)
+                for (int i = ct; i < ROWS * (C::DKP / 4); i += 256) {   // (the pieces this thread brought)
                     const int r = i / (C::DKP / 4), c = i - r * (C::DKP / 4);
                     uint8_t *at = sm + C::Q_AT + (c >> 3) * C::QSLAB + r * 128 + (((c & 7) ^ (r & 7)) << 4);
                     const uint4 x = *reinterpret_cast<const uint4 *>(at);
@@ -392,10 +396,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;   // row = lane of tensor memory
         const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };   // the two warps of 32 rows
-        auto all_sync = [&] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        auto all_sync = [&] { asm volatile("bar.sync 1, %0;" ::"n"(C::SOFTMAX) : "memory"); };
         float o[OH], m, l;
-        while (next_piece(a, line, cur, p)) {
-            const int r = p.block * TT_ROWS + row, gh = r / p.s.n, tok = r < p.s.rows ? r - gh * p.s.n : 0;
+        while ((warp & 3) * 32 < ROWS && next_piece(a, line, cur, p)) {   // (with 64 rows the warps of lanes 64 to 127 have none)
+            const int r = p.block * ROWS + row, gh = r / p.s.n, tok = r < p.s.rows ? r - gh * p.s.n : 0;
             const bool mine = r < p.s.rows;
             m = -INFINITY;
             l = 0.f;
@@ -406,12 +410,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
                 tc_fence_after_sync();
                 const bool odd = s_odd[jt & 3] == (int)jt + 1;
 #pragma unroll
-                for (int h = 0; h < OH / 16; ++h) {
-                    uint32_t x[16];
-                    tmem_ld_32x32_x16(lane_base + C::T_O + (jt % C::OB) * C::DKP + half * OH + 16 * h, x);
+                for (int h = 0; h < OH / FOLD; ++h) {
+                    uint32_t x[FOLD];
+                    const uint32_t at = lane_base + C::T_O + (jt % C::OB) * C::DKP + half * OH + FOLD * h;
+                    if constexpr (FOLD == 32) tmem_ld_32x32(at, x);
+                    else tmem_ld_32x32_x16(at, x);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) o[16 * h + c] += __uint_as_float(x[c]);
+                    for (int c = 0; c < FOLD; ++c) o[FOLD * h + c] += __uint_as_float(x[c]);
                 }
                 tc_fence_before_sync();
                 mbar_arrive(bar(TB_O_EMPTY + jt % C::OB));
@@ -423,43 +429,58 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
                         if (j < 0 || j >= p.s.n || !tree_sees(a, p.b, tok, j)) continue;
                         const float *src = a.V + (((int64_t)p.b * a.Hkv + p.hk) * a.max_seq + key) * a.dk + half * OH;
 #pragma unroll
-                        for (int c = 0; c < OH; ++c)
-                            if (half * OH + c < a.dk) {
-                                const float x = __ldg(src + c);
-                                if (!finite_f(x)) o[c] += x;
-                            }
+                        for (int c = 0; c < OH; c += 4) {   // (dk is a multiple of 4)
+                            if (half * OH + c >= a.dk) continue;
+                            float4 v;   // (volatile: not all of the row's loads at once, o has the registers)
+                            asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(src + c));
+                            if (!finite_f(v.x)) o[c] += v.x;
+                            if (!finite_f(v.y)) o[c + 1] += v.y;
+                            if (!finite_f(v.z)) o[c + 2] += v.z;
+                            if (!finite_f(v.w)) o[c + 3] += v.w;
+                        }
                     }
                 }
+                if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll
-                for (int c = 0; c < OH; ++c) o[c] *= f;
+                    for (int c = 0; c < OH; ++c) o[c] *= f;
+                }
             };
             for (int i = 0; i < p.count; ++i, ++it) {
                 const uint32_t b = it & 1;
                 const int key0 = (p.t0 + i) * KB;
-                const uint32_t s_addr = lane_base + C::T_S + b * KB + half * (KB / 2), lo_addr = lane_base + C::T_PLO + half * (KB / 2);
-                const int first = key0 + half * (KB / 2) - p.s.len;   // new-token index of this thread's first column
+                constexpr int NCH = KB / 64;   // a thread's columns, 32 at a time
+                const int first = key0 + half * (KB / 2) - p.s.len;   // new-token index of its first column
                 const bool tail = first + KB / 2 > 0;
-                if (ok && !wait_all(TB_S_FULL + b, (it >> 1) & 1)) ok = false;
+                if (ok && !wait_all(TB_S_FULL + it % C::SB, (it / C::SB) & 1)) ok = false;
                 float mx = -INFINITY;
+                uint32_t x[NCH][32], see[NCH];
                 if (ok) {
                     tc_fence_after_sync();
-                    float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
-#pragma unroll 1
-                    for (int c0 = 0; c0 < KB / 2; c0 += 32) {
-                        uint32_t x[32];
-                        tmem_ld_32x32(s_addr + c0, x);
-                        tmem_ld_wait();
-                        const uint32_t see = tail ? seen_bits(a, p.b, tok, p.s.n, first + c0) : 0xFFFFFFFFu;
-                        if (see == 0xFFFFFFFFu) {
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(x[c]) * a.c_log2);
-                        } else {
+                    for (int c0 = 0; c0 < NCH; ++c0) tmem_ld_32x32(lane_base + C::T_S + (it % C::SB) * KB + half * (KB / 2) + 32 * c0, x[c0]);
+                    tmem_ld_wait();
+                    tc_fence_before_sync();
+                    mbar_arrive(bar(TB_S_EMPTY + it % C::SB));
+                    // the largest of c * score: of the scores themselves, or the smallest where c is negative
+                    const uint32_t flip = a.c_log2 < 0.f ? 0x80000000u : 0u;
+                    float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+#pragma unroll
+                    for (int c0 = 0; c0 < NCH; ++c0) {
+                        see[c0] = tail ? seen_bits(a, p.b, tok, p.s.n, first + 32 * c0) : 0xFFFFFFFFu;
+                        if (tail || flip) {
 #pragma unroll
                             for (int c = 0; c < 32; ++c)
-                                if (see >> c & 1) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(x[c]) * a.c_log2);
+                                if (see[c0] >> c & 1) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(x[c0][c] ^ flip));
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 32; c += 8)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    t4[e] = fmaxf(t4[e], fmaxf(__uint_as_float(x[c0][c + 2 * e]), __uint_as_float(x[c0][c + 2 * e + 1])));
                         }
                     }
                     mx = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                    if (mx != -INFINITY) mx *= fabsf(a.c_log2);   // (nothing seen: as it is, 0 * -inf would be NaN)
                 }
                 s_max[b][half][row] = mx;
                 pair_sync();
@@ -472,38 +493,34 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
                 }
                 const float neg = m == -INFINITY ? 0.f : -m;
                 float sum[4] = { 0.f, 0.f, 0.f, 0.f };
-#pragma unroll 1
-                for (int c0 = 0; c0 < KB / 2; c0 += 32) {
-                    uint32_t x[32];
-                    tmem_ld_32x32(s_addr + c0, x);
-                    tmem_ld_wait();
-                    const uint32_t see = tail ? seen_bits(a, p.b, tok, p.s.n, first + c0) : 0xFFFFFFFFu;
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        float e = ex2_approx(fmaf(__uint_as_float(x[c]), a.c_log2, neg));
-                        if (!(see >> c & 1)) e = 0.f;
-                        sum[c & 3] += e;
-                        x[c] = __float_as_uint(e);
+                for (int c0 = 0; c0 < NCH; ++c0) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) x[c0][c] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[c0][c]), a.c_log2, neg)));
+                    if (tail) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (!(see[c0] >> c & 1)) x[c0][c] = 0;
                     }
-                    tmem_st_32x32(s_addr + c0, x);
-                }
-                tmem_st_wait();
-                l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-                tc_fence_before_sync();
-                mbar_arrive(bar(TB_P_FULL + b));   // P hi: two of the three products can start
-                // P lo is a single buffer: the product of the block before must have read it
-                if (i > 0) {
-                    if (!wait_all(TB_O_FULL + (b ^ 1), ((it - 1) >> 1) & 1)) { ok = false; continue; }
-                    if (C::OB == 1) fold(it - 1, key0 - KB, corr);   // the single accumulator has to be free for this block's product
-                }
-#pragma unroll 1
-                for (int c0 = 0; c0 < KB / 2; c0 += 32) {
-                    uint32_t x[32];
-                    tmem_ld_32x32(s_addr + c0, x);
-                    tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) x[c] = lo_bits(x[c]);
-                    tmem_st_32x32(lo_addr + c0, x);
+                    for (int c = 0; c < 32; ++c) sum[c & 3] += __uint_as_float(x[c0][c]);
+                }
+                l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                // P is single: the product of the block before must have read it
+                if (i > 0 && !wait_all(TB_O_FULL, (it - 1) & 1)) { ok = false; continue; }
+                tc_fence_after_sync();
+                const uint32_t p_at = lane_base + C::T_P + half * (KB / 2);
+#pragma unroll
+                for (int c0 = 0; c0 < NCH; ++c0) tmem_st_32x32(p_at + 32 * c0, x[c0]);
+                tmem_st_wait();
+                tc_fence_before_sync();
+                mbar_arrive(bar(TB_P_FULL));   // P hi: two of the three products can start (with one accumulator: once it is folded)
+                if (i > 0 && C::OB == 1) fold(it - 1, key0 - KB, corr);
+#pragma unroll
+                for (int c0 = 0; c0 < NCH; ++c0) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) x[c0][c] = lo_bits(x[c0][c]);
+                    tmem_st_32x32(p_at + (C::T_PLO - C::T_P) + 32 * c0, x[c0]);
                 }
                 tmem_st_wait();
                 tc_fence_before_sync();
@@ -511,7 +528,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
                 if (i > 0 && C::OB == 2) fold(it - 1, key0 - KB, corr);
             }
             if (ok) {
-                if (wait_all(TB_O_FULL + ((it - 1) & 1), ((it - 1) >> 1) & 1)) fold(it - 1, (p.t0 + p.count - 1) * KB, 1.f);
+                if (wait_all(TB_O_FULL, (it - 1) & 1)) fold(it - 1, (p.t0 + p.count - 1) * KB, 1.f);
                 else ok = false;
             }
             s_max[(it - 1) & 1][half][row] = l;   // (the last block's maxima have been read: its product had to wait for that)
@@ -527,8 +544,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
             auto put = [&](float4 *s) {
 #pragma unroll
                 for (int c = 0; c < OH / 4; ++c)
-                    s[(half * (OH / 4) + c) * TT_ROWS + row] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-                if (half == 0) reinterpret_cast<float2 *>(s + C::DKP / 4 * TT_ROWS)[row] = make_float2(m, l);
+                    s[(half * (OH / 4) + c) * ROWS + row] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                if (half == 0) reinterpret_cast<float2 *>(s + C::DKP / 4 * ROWS)[row] = make_float2(m, l);
             };
             auto arrive_last = [&](int *counter, int of) -> bool {
                 __threadfence();
@@ -550,18 +567,25 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
 #pragma unroll 1
                 for (int k = from; k < to; k += step) {
                     const float4 *s = slot(p.first + k);
-                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(s + C::DKP / 4 * TT_ROWS) + row);
+                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(s + C::DKP / 4 * ROWS) + row);
                     const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
                     const float f0 = ex2_approx(m - ref), f1 = ex2_approx(ml.x - ref);
                     m = m_new;
                     l = l * f0 + ml.y * f1;
 #pragma unroll
-                    for (int c = 0; c < OH / 4; ++c) {
-                        const float4 x = __ldcg(s + (half * (OH / 4) + c) * TT_ROWS + row);
-                        o[4 * c] = o[4 * c] * f0 + x.x * f1;
-                        o[4 * c + 1] = o[4 * c + 1] * f0 + x.y * f1;
-                        o[4 * c + 2] = o[4 * c + 2] * f0 + x.z * f1;
-                        o[4 * c + 3] = o[4 * c + 3] * f0 + x.w * f1;
+                    for (int c0 = 0; c0 < OH / 4; c0 += 4) {   // 16 columns' loads at a time: o has the registers
+                        float4 x[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) x[c] = __ldcg(s + (half * (OH / 4) + c0 + c) * ROWS + row);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float *d = o + 4 * (c0 + c);
+                            d[0] = d[0] * f0 + x[c].x * f1;
+                            d[1] = d[1] * f0 + x[c].y * f1;
+                            d[2] = d[2] * f0 + x[c].z * f1;
+                            d[3] = d[3] * f0 + x[c].w * f1;
+                        }
+                        asm volatile("" ::: "memory");
                     }
                 }
             };
@@ -605,29 +629,35 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
 
 // ---------------------------------------------------------------------- host
 
-template <int NSLAB>
+template <int NSLAB, bool FEW>
 static int launch_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st)
 {
-    using C = TreeTc<NSLAB>;
+    using C = TreeTc<NSLAB, FEW>;
     static PerDeviceOnce once;
     if (once.first()) {
-        cudaError_t e = cudaFuncSetAttribute(kv_tree_tc_kernel<NSLAB>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(kv_tree_tc_kernel<NSLAB, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return (int)e;
     }
     TreeTcMaps tm;
     int e = encode_f32_batched_tmap(&tm.k, a.K, (int64_t)a.B * a.Hkv, a.max_seq, a.dk, a.dk, C::KB, false);
     if (!e) e = encode_f32_batched_tmap(&tm.v, a.V, (int64_t)a.B * a.Hkv, a.max_seq, a.dk, a.dk, C::KB, true);
     if (e) return e;
-    kv_tree_tc_kernel<NSLAB><<<sm_count, TT_THREADS, C::SMEM, st>>>(a, tm);
+    kv_tree_tc_kernel<NSLAB, FEW><<<sm_count, TT_THREADS, C::SMEM, st>>>(a, tm);
     return (int)cudaGetLastError();
 }
 
 int launch_kv_tree_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st)
 {
-    if (a.dk <= 32) return launch_tc<1>(a, sm_count, st);
-    if (a.dk <= 64) return launch_tc<2>(a, sm_count, st);
-    if (a.dk <= 96) return launch_tc<3>(a, sm_count, st);
-    return launch_tc<4>(a, sm_count, st);
+    if (a.H / a.Hkv <= 64 / a.T) {
+        if (a.dk <= 32) return launch_tc<1, true>(a, sm_count, st);
+        if (a.dk <= 64) return launch_tc<2, true>(a, sm_count, st);
+        if (a.dk <= 96) return launch_tc<3, true>(a, sm_count, st);
+        return launch_tc<4, true>(a, sm_count, st);
+    }
+    if (a.dk <= 32) return launch_tc<1, false>(a, sm_count, st);
+    if (a.dk <= 64) return launch_tc<2, false>(a, sm_count, st);
+    if (a.dk <= 96) return launch_tc<3, false>(a, sm_count, st);
+    return launch_tc<4, false>(a, sm_count, st);
 }
 
 }  // namespace axb
