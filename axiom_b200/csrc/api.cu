@@ -1410,7 +1410,7 @@ inline bool overlaps(const void *p, int64_t n, const void *q, int64_t m)   // n,
 
 // counters first (zero between calls), then room for either call's partial results
 constexpr size_t kAttnCounters = 4096;
-static_assert(sizeof(int) * 3 * 256 <= kAttnCounters, "three counters per SM");
+static_assert(sizeof(int) * 3 * 256 <= kAttnCounters && sizeof(KvTreeShared) * 256 <= KT_SHARED_BYTES, "per SM: three counters, a shared item");
 
 size_t attn_workspace_bytes()
 {
@@ -1604,7 +1604,8 @@ extern "C" int axb_kv_cache_attend_tree(const float *K_cache, const float *V_cac
     KvTreeArgs a;
     a.K = K_cache; a.V = V_cache; a.Q = Q; a.mask = mask; a.lens = lens; a.n_new = n_new; a.out = out;
     a.counters = (int *)workspace;
-    a.slots = reinterpret_cast<float *>((char *)workspace + kAttnCounters);
+    a.shared = reinterpret_cast<KvTreeShared *>((char *)workspace + kAttnCounters);
+    a.slots = reinterpret_cast<float *>((char *)workspace + kAttnCounters + KT_SHARED_BYTES);
     a.words = (int)((T + 63) / 64);
     a.mask_stride = mask_per_seq ? T * a.words : 0;
     a.max_seq = max_seq; a.err = cur().err_word; a.c_log2 = scale * 1.4426950408889634f;

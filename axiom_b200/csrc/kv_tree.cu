@@ -704,7 +704,7 @@ static inline bool kt_aligned16(const void *p) { return (reinterpret_cast<uintpt
 
 size_t kv_tree_workspace_bytes(int sm_count)
 {
-    return (size_t)sm_count * 2 * KT_SLOT_BYTES;
+    return KT_SHARED_BYTES + (size_t)sm_count * 2 * KT_SLOT_BYTES;
 }
 
 template <int DKP, int NR>

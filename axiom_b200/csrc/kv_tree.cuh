@@ -7,6 +7,11 @@
 
 namespace axb {
 
+// what the kernel that adds up an item's pieces has to know of it; it stands at the CTA that holds the item's first key tile
+struct KvTreeShared {
+    int pieces, b, hk, block, n, rows;   // pieces 0: none; n, rows: the sequence's new tokens and query rows of a key head
+};
+
 struct KvTreeArgs {
     const float *K, *V;          // [B*Hkv, max_seq, dk]
     const float *Q;              // [B*H, T, dk]
@@ -14,13 +19,15 @@ struct KvTreeArgs {
     const int32_t *lens, *n_new; // [B]; n_new nullptr: T for every sequence
     float *out;                  // [B*H, T, dk]
     int *counters;               // three per SM, zero on entry and on exit
-    float *slots;                // kv_tree_workspace_bytes(): partial results, two slots per SM
+    KvTreeShared *shared;        // kv_tree_workspace_bytes(): one per SM, then
+    float *slots;                // partial results, two slots per SM
     int64_t max_seq, mask_stride;
     int *err;
     float c_log2;                // scale * log2(e)
     int B, H, Hkv, T, dk, words;
 };
 
+constexpr size_t KT_SHARED_BYTES = 256 * sizeof(KvTreeShared);   // (whole lines: the slots behind it begin one)
 constexpr size_t KT_SLOT_BYTES = 128 * (128 + 2) * sizeof(float);   // the largest variant's partial result
 size_t kv_tree_workspace_bytes(int sm_count);
 // query rows of a key head from which on the tensor-memory kernel (kv_tree_tc.cu) takes over; it wants 16-byte pieces

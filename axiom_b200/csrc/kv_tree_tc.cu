@@ -66,47 +66,47 @@ __device__ __forceinline__ uint32_t lo_bits(uint32_t x)
     return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u)) + 0x1000u;
 }
 
-// the three products of a block's scores / outputs, issued by one thread.  B: block parity.  Everything that an instruction
-// names is a constant offset from the bases, so that it takes no moves into the registers that tcgen05.mma reads (with
-// addresses formed at run time an instruction cost the issuing thread 110 cycles where the pipe takes 48 to 64).
-template <int NSLAB, bool FEW, int B>
-__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, uint32_t idesc, uint32_t klo_empty)
+// The three products of a block's scores / outputs, issued by one thread: four steps of eight at a time, in loops — the kernel's
+// roles share the SM's instruction cache, and unrolled whole (for either buffer of K and V) this code alone kept it turning over:
+// the softmax warps then waited for their instructions (5.9 against 4.4 thousand cycles a block).
+template <int NSLAB, bool FEW>
+__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, uint32_t it, uint32_t idesc, uint32_t klo_empty)
 {
     using C = TreeTc<NSLAB, FEW>;
-    const uint64_t dk = smem_desc_kmajor(0, 128);
-    uint32_t b0 = (base & 0x3FFFFu) >> 4;
-    asm volatile("" : "+r"(b0));
-    auto desc = [&](uint32_t at) { return (dk & 0xFFFFFFFF00000000ull) | ((uint32_t)dk + b0 + (at >> 4)); };
-    constexpr uint32_t khi = C::K_AT + (B % C::KS) * C::PLANE;
+    const uint64_t dk = smem_desc_kmajor(base, 128);   // (every offset below stays inside the CTA's 256 KB window)
+    const uint32_t d = tmem + C::T_S + it % C::SB * C::KB, khi = C::K_AT + it % C::KS * C::PLANE;
 #pragma unroll
     for (int pr = 0; pr < 3; ++pr) {   // hi.lo, whose lo tile the next block waits for, lo.hi, hi.hi
-        const uint32_t kk = pr == 0 ? C::KLO_AT : khi, qq = C::Q_AT + (pr == 1 && !C::WIDE ? C::QPLANE : 0);
+        uint64_t kd = dk + ((pr == 0 ? C::KLO_AT : khi) >> 4), qd = dk + ((C::Q_AT + (pr == 1 && !C::WIDE ? C::QPLANE : 0)) >> 4);
+        uint32_t qt = tmem + C::T_QLO;
+#pragma unroll 1
+        for (int sl = 0; sl < NSLAB; ++sl, kd += C::SLAB >> 4, qd += C::QSLAB >> 4, qt += 32) {   // (columns from dk on are zero)
 #pragma unroll
-        for (int ks = 0; ks < 4 * NSLAB; ++ks) {   // (columns from dk on are zero)
-            const uint64_t bd = desc(kk + (ks >> 2) * C::SLAB + (ks & 3) * 32);
-            if (C::WIDE && pr == 1) tc_mma_ts_tf32(tmem + C::T_S + (B % C::SB) * C::KB, tmem + C::T_QLO + ks * 8, bd, idesc, 1);
-            else tc_mma<KIND_TF32>(tmem + C::T_S + (B % C::SB) * C::KB, desc(qq + (ks >> 2) * C::QSLAB + (ks & 3) * 32), bd, idesc, pr | ks);
+            for (int ks = 0; ks < 4; ++ks) {
+                if (C::WIDE && pr == 1) tc_mma_ts_tf32(d, qt + ks * 8, kd + ks * 2, idesc, 1);
+                else tc_mma<KIND_TF32>(d, qd + ks * 2, kd + ks * 2, idesc, pr | sl | ks);
+            }
         }
         if (pr == 0) tc_commit(klo_empty);
     }
 }
 
 // part 0: hi.lo, whose lo tile the next block waits for, and hi.hi; part 1: lo.hi, whose operand comes last
-template <int NSLAB, bool FEW, int B, int PART>
-__device__ __forceinline__ void issue_outputs(uint32_t base, uint32_t tmem, uint32_t idesc, uint32_t vlo_empty)
+template <int NSLAB, bool FEW, int PART>
+__device__ __forceinline__ void issue_outputs(uint32_t base, uint32_t tmem, uint32_t it, uint32_t idesc, uint32_t vlo_empty)
 {
     using C = TreeTc<NSLAB, FEW>;
-    const uint64_t dm = smem_desc_mnmajor_sw128_32b(0, C::SLAB, 512);
-    uint32_t b0 = (base & 0x3FFFFu) >> 4;
-    asm volatile("" : "+r"(b0));
-    auto desc = [&](uint32_t at) { return (dm & 0xFFFFFFFF00000000ull) | ((uint32_t)dm + b0 + (at >> 4)); };
-    constexpr uint32_t vhi = C::V_AT + (B % C::VS) * C::PLANE;
-    const uint32_t d = tmem + C::T_O + (B % C::OB) * C::DKP;
+    const uint64_t dm = smem_desc_mnmajor_sw128_32b(base, C::SLAB, 512);
+    const uint32_t d = tmem + C::T_O + it % C::OB * C::DKP, vhi = C::V_AT + it % C::VS * C::PLANE;
 #pragma unroll
     for (int pr = PART ? 2 : 0; pr < (PART ? 3 : 2); ++pr) {
+        uint64_t vd = dm + ((pr == 0 ? C::VLO_AT : vhi) >> 4);
+        uint32_t pt = tmem + (pr == 2 ? C::T_PLO : C::T_P);
+#pragma unroll 1
+        for (int k0 = 0; k0 < C::KB / 32; ++k0, vd += 4 * 64, pt += 32) {
 #pragma unroll
-        for (int ks = 0; ks < C::KB / 8; ++ks)
-            tc_mma_ts_tf32(d, tmem + (pr == 2 ? C::T_PLO : C::T_P) + ks * 8, desc((pr == 0 ? C::VLO_AT : vhi) + ks * 1024), idesc, pr | ks);
+            for (int ks = 0; ks < 4; ++ks) tc_mma_ts_tf32(d, pt + ks * 8, vd + ks * 64, idesc, pr | k0 | ks);
+        }
         if (pr == 0) tc_commit(vlo_empty);
     }
 }
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     int *s_line = reinterpret_cast<int *>(sm + 256);
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(sm + 288);
     volatile int *words = reinterpret_cast<volatile int *>(sm + 304);
-    volatile int &s_gave_up = words[0], &s_last = words[1], *s_odd = words + 2;   // s_odd: block it + 1 holds non-finite new values
+    volatile int &s_gave_up = words[0], *s_odd = words + 2;   // s_odd: block it + 1 holds non-finite new values
     int *s_row = reinterpret_cast<int *>(sm + 512);   // [ROWS]
     float (*s_max)[2][ROWS] = reinterpret_cast<float (*)[2][ROWS]>(sm + 1024);   // [block parity][half][row]
     if (base & 1023) {   // the swizzles are functions of the address (it starts at a multiple of 1 KB; refused, should it ever not)
@@ -169,6 +169,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
         s_gave_up = 0;
         for (int i = 0; i < 4; ++i) s_odd[i] = 0;
     }
+    if (threadIdx.x == 0) a.shared[blockIdx.x] = KvTreeShared{ 0, 0, 0, 0, 0, 0 };   // (this thread replaces it where the CTA begins a shared item)
     constexpr TreeLine line = { ROWS, KB, 1 };
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;
@@ -237,8 +238,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
                     if (it >= C::SB && !wait(TB_S_EMPTY + it % C::SB, (it / C::SB - 1) & 1)) { ok = false; break; }
                     if (!wait(TB_K_FULL, it & 1)) { ok = false; break; }
                     tc_fence_after_sync();
-                    if (it & 1) issue_scores<NSLAB, FEW, 1>(base, tmem, idesc, bar(TB_KLO_EMPTY));
-                    else issue_scores<NSLAB, FEW, 0>(base, tmem, idesc, bar(TB_KLO_EMPTY));
+                    issue_scores<NSLAB, FEW>(base, tmem, it, idesc, bar(TB_KLO_EMPTY));
                     tc_commit(bar(TB_S_FULL + it % C::SB));
                     tc_commit(bar(TB_K_EMPTY + it % C::KS));
                     if (i == p.count - 1) tc_commit(bar(TB_Q_EMPTY));
@@ -253,12 +253,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
                     if (!wait(TB_V_FULL, it & 1)) { ok = false; break; }
                     if (it >= C::OB && !wait(TB_O_EMPTY + it % C::OB, (it / C::OB - 1) & 1)) { ok = false; break; }
                     tc_fence_after_sync();
-                    if (it & 1) issue_outputs<NSLAB, FEW, 1, 0>(base, tmem, idesc, bar(TB_VLO_EMPTY));
-                    else issue_outputs<NSLAB, FEW, 0, 0>(base, tmem, idesc, bar(TB_VLO_EMPTY));
+                    issue_outputs<NSLAB, FEW, 0>(base, tmem, it, idesc, bar(TB_VLO_EMPTY));
                     if (!wait(TB_PLO_FULL, it & 1)) { ok = false; break; }
                     tc_fence_after_sync();
-                    if (it & 1) issue_outputs<NSLAB, FEW, 1, 1>(base, tmem, idesc, 0);
-                    else issue_outputs<NSLAB, FEW, 0, 1>(base, tmem, idesc, 0);
+                    issue_outputs<NSLAB, FEW, 1>(base, tmem, it, idesc, 0);
                     tc_commit(bar(TB_O_FULL));
                     tc_commit(bar(TB_V_EMPTY + it % C::VS));
                 }
@@ -396,7 +394,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;   // row = lane of tensor memory
         const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };   // the two warps of 32 rows
-        auto all_sync = [&] { asm volatile("bar.sync 1, %0;" ::"n"(C::SOFTMAX) : "memory"); };
         float o[OH], m, l;
         while ((warp & 3) * 32 < ROWS && next_piece(a, line, cur, p)) {   // (with 64 rows the warps of lanes 64 to 127 have none)
             const int r = p.block * ROWS + row, gh = r / p.s.n, tok = r < p.s.rows ? r - gh * p.s.n : 0;
@@ -535,79 +532,16 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
             pair_sync();
             l += s_max[(it - 1) & 1][half ^ 1][row];
 
-            // pieces of a shared item: [16-byte column][row] outputs, then [row] (maximum, sum).  Up to GROUP pieces are added by
-            // the CTA that arrives last; more in groups first, whose sums take the place of the group's first piece.
-            constexpr int GROUP = 12;
-            auto slot = [&](int cta) {
-                return reinterpret_cast<float4 *>(a.slots) + (size_t)tree_slot(cta, cta == p.first) * (KT_SLOT_BYTES / 16);
-            };
-            auto put = [&](float4 *s) {
+            if (p.pieces > 1) {
+                // a piece of a shared item: [16-byte column][row] outputs, then [row] (maximum, sum), for the kernel behind this one
+                float4 *s = reinterpret_cast<float4 *>(a.slots) + (size_t)tree_slot(blockIdx.x, p.t0 == 0) * (KT_SLOT_BYTES / 16);
 #pragma unroll
                 for (int c = 0; c < OH / 4; ++c)
                     s[(half * (OH / 4) + c) * ROWS + row] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
                 if (half == 0) reinterpret_cast<float2 *>(s + C::DKP / 4 * ROWS)[row] = make_float2(m, l);
-            };
-            auto arrive_last = [&](int *counter, int of) -> bool {
-                __threadfence();
-                all_sync();
-                if (threadIdx.x == 0) {
-                    s_last = atomicAdd(counter, 1) == of - 1;
-                    if (s_last) *counter = 0;
-                }
-                all_sync();
-                const bool last = s_last != 0;
-                __threadfence();
-                return last;
-            };
-            auto add_up = [&](int from, int to, int step) {   // pieces first + from, first + from + step, ... in line order
-                m = -INFINITY;
-                l = 0.f;
-#pragma unroll
-                for (int c = 0; c < OH; ++c) o[c] = 0.f;
-#pragma unroll 1
-                for (int k = from; k < to; k += step) {
-                    const float4 *s = slot(p.first + k);
-                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(s + C::DKP / 4 * ROWS) + row);
-                    const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
-                    const float f0 = ex2_approx(m - ref), f1 = ex2_approx(ml.x - ref);
-                    m = m_new;
-                    l = l * f0 + ml.y * f1;
-#pragma unroll
-                    for (int c0 = 0; c0 < OH / 4; c0 += 4) {   // 16 columns' loads at a time: o has the registers
-                        float4 x[4];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) x[c] = __ldcg(s + (half * (OH / 4) + c0 + c) * ROWS + row);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            float *d = o + 4 * (c0 + c);
-                            d[0] = d[0] * f0 + x[c].x * f1;
-                            d[1] = d[1] * f0 + x[c].y * f1;
-                            d[2] = d[2] * f0 + x[c].z * f1;
-                            d[3] = d[3] * f0 + x[c].w * f1;
-                        }
-                        asm volatile("" ::: "memory");
-                    }
-                }
-            };
-            bool write = p.pieces == 1;
-            if (!write) {
-                const int k = (int)blockIdx.x - p.first;
-                put(slot(blockIdx.x));
-                if (p.pieces <= GROUP) {
-                    write = arrive_last(a.counters + p.first, p.pieces);
-                    if (write) add_up(0, p.pieces, 1);
-                } else {
-                    // counters: [items by first CTA][first groups by first CTA][other groups by their first CTA]
-                    const int g0 = k / GROUP * GROUP, in_group = p.pieces - g0 < GROUP ? p.pieces - g0 : GROUP;
-                    if (arrive_last(a.counters + (g0 ? 2 : 1) * gridDim.x + p.first + g0, in_group)) {
-                        add_up(g0, g0 + in_group, 1);
-                        put(slot(p.first + g0));   // (each thread wrote over what it alone had read)
-                        write = arrive_last(a.counters + p.first, (p.pieces + GROUP - 1) / GROUP);
-                        if (write) add_up(0, p.pieces, GROUP);
-                    }
-                }
+                if (p.t0 == 0 && threadIdx.x == 0) a.shared[blockIdx.x] = KvTreeShared{ p.pieces, p.b, p.hk, p.block, p.s.n, p.s.rows };
             }
-            if (write && mine) {
+            if (p.pieces == 1 && mine) {
                 float *dst = a.out + (((int64_t)p.b * a.H + p.hk * heads_per + gh) * a.T + tok) * a.dk + half * OH;
                 const float inv = l == 0.f ? 0.f : 1.0f / l;   // nothing seen: 0
 #pragma unroll
@@ -627,6 +561,105 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     }
 }
 
+// The shared items' pieces added up, in line order within each of a unit's groups of threads and then over the groups.  A unit is
+// a few rows of an item: fewer where more pieces want more groups.  (The CTA that arrived last used to do it, one piece after the
+// other on one SM and with a counter's round trip for every piece: 30 us for 148 pieces of 128 rows.)
+template <int DKP, int ROWS>
+struct TreeJoin {
+    static constexpr int COLS = DKP / 4, RG = COLS > 16 ? 16 : COLS > 8 ? 32 : 64, THREADS = RG * COLS;   // rows x groups of a unit
+    // as many groups as leave each four pieces, and two rows to a unit (the rows of a 16-byte column then fill a 32-byte sector)
+    static __device__ __forceinline__ int groups(int pieces)
+    {
+        int g = 1;
+        while (g < RG / 2 && 8 * g <= pieces) g <<= 1;
+        return g;
+    }
+};
+
+template <int DKP, int ROWS>
+__global__ void __launch_bounds__(TreeJoin<DKP, ROWS>::THREADS, 2) kv_tree_join_kernel(const KvTreeArgs a, int ctas)
+{
+    using J = TreeJoin<DKP, ROWS>;
+    __shared__ float4 s_o[J::THREADS];
+    __shared__ float2 s_ml[J::RG];
+    __shared__ int s_upto[256], s_warp[8], s_unit[2];
+    __shared__ KvTreeShared s_item[256];
+    const int tid = threadIdx.x, lane = tid & 31;
+    // units up to and including CTA tid's item
+    if (tid < 256) {
+        int units = 0;
+        if (tid < ctas) {
+            const KvTreeShared it = a.shared[tid];
+            s_item[tid] = it;
+            const int rows = it.rows - it.block * ROWS < ROWS ? it.rows - it.block * ROWS : ROWS, per = J::RG / J::groups(it.pieces);
+            if (it.pieces) units = (rows + per - 1) / per;
+        }
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, units, o);
+            if (lane >= o) units += v;
+        }
+        s_upto[tid] = units;
+        if (lane == 31) s_warp[tid >> 5] = units;
+    }
+    __syncthreads();
+    if (tid < 256)
+        for (int w = 0; w < tid >> 5; ++w) s_upto[tid] += s_warp[w];
+    __syncthreads();
+    for (int unit = blockIdx.x; unit < s_upto[255]; unit += gridDim.x) {
+        if (tid < 256) {
+            const int before = tid ? s_upto[tid - 1] : 0;
+            if (unit >= before && unit < s_upto[tid]) {
+                s_unit[0] = tid;
+                s_unit[1] = unit - before;
+            }
+        }
+        __syncthreads();
+        const int first = s_unit[0];
+        const KvTreeShared it = s_item[first];
+        const int groups = J::groups(it.pieces), per = J::RG / groups;
+        const int r = tid % per, c = tid / per % J::COLS, g = tid / (per * J::COLS), row = s_unit[1] * per + r;
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float2 ml, float4 x) {
+            const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
+            const float f0 = ex2_approx(m - ref), f1 = ex2_approx(ml.x - ref);
+            m = m_new;
+            l = l * f0 + ml.y * f1;
+            o.x = o.x * f0 + x.x * f1;
+            o.y = o.y * f0 + x.y * f1;
+            o.z = o.z * f0 + x.z * f1;
+            o.w = o.w * f0 + x.w * f1;
+        };
+        constexpr int UN = 4;   // pieces on their way at a time
+        for (int k0 = g; k0 < it.pieces; k0 += UN * groups) {
+            float2 ml[UN];
+            float4 x[UN];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const int k = k0 + u * groups;
+                const float4 *s = reinterpret_cast<const float4 *>(a.slots) + (size_t)tree_slot(first + k, k == 0) * (KT_SLOT_BYTES / 16);
+                const bool has = k < it.pieces && row < ROWS;
+                ml[u] = has ? __ldcg(reinterpret_cast<const float2 *>(s + J::COLS * ROWS) + row) : make_float2(-INFINITY, 0.f);
+                x[u] = has ? __ldcg(s + c * ROWS + row) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < UN; ++u) add(ml[u], x[u]);
+        }
+        s_o[tid] = o;
+        if (c == 0) s_ml[g * per + r] = make_float2(m, l);
+        __syncthreads();
+        if (g == 0) {
+            for (int k = 1; k < groups; ++k) add(s_ml[k * per + r], s_o[tid + k * per * J::COLS]);
+            const int at = it.block * ROWS + row, gh = at / it.n, heads_per = a.H / a.Hkv;
+            if (row < ROWS && at < it.rows && 4 * c < a.dk) {
+                const float inv = l == 0.f ? 0.f : 1.0f / l;   // nothing seen: 0
+                *reinterpret_cast<float4 *>(a.out + (((int64_t)it.b * a.H + it.hk * heads_per + gh) * a.T + at - gh * it.n) * a.dk + 4 * c) =
+                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------------- host
 
 template <int NSLAB, bool FEW>
@@ -643,6 +676,9 @@ static int launch_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st)
     if (!e) e = encode_f32_batched_tmap(&tm.v, a.V, (int64_t)a.B * a.Hkv, a.max_seq, a.dk, a.dk, C::KB, true);
     if (e) return e;
     kv_tree_tc_kernel<NSLAB, FEW><<<sm_count, TT_THREADS, C::SMEM, st>>>(a, tm);
+    if ((e = (int)cudaGetLastError()) != 0) return e;
+    using J = TreeJoin<C::DKP, C::ROWS>;
+    kv_tree_join_kernel<C::DKP, C::ROWS><<<2 * sm_count, J::THREADS, 0, st>>>(a, sm_count);
     return (int)cudaGetLastError();
 }
 
