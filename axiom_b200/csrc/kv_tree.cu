@@ -376,7 +376,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
         mbar_init(merge_empty, 1);
         mbar_fence_init();
     }
-    constexpr TreeLine line = { ROWS, KT_KEYS, C::GROUPS };
+    constexpr TreeLine line = { ROWS, KT_KEYS, C::GROUPS, C::ASYNC ? 0 : 4 };
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;   // (its barriers make the initialised ones above visible)
     TreePiece p;
@@ -731,11 +731,12 @@ static int launch_tree_rows(const KvTreeArgs &a, const TreeMaps &tm, int tma, in
     return launch_tree<128, NR>(a, tm, tma, sm_count, st);
 }
 
-int launch_kv_cache_attend_tree(const KvTreeArgs &a, int sm_count, cudaStream_t st)
+int launch_kv_cache_attend_tree(const KvTreeArgs &a, int sm_count, cudaStream_t st, int *launches)
 {
+    *launches = 1;
     const int tma = a.dk % 4 == 0 && kt_aligned16(a.K) && kt_aligned16(a.V) && kt_aligned16(a.Q) && kt_aligned16(a.out);
     const int64_t rows = (int64_t)(a.H / a.Hkv) * a.T;   // of a key head, if every token is there
-    if (tma && rows > KT_TC_ROWS) return launch_kv_tree_tc(a, sm_count, st);
+    if (tma && rows > kt_warp_rows(a.dk)) return launch_kv_tree_tc(a, sm_count, st, launches);
     TreeMaps tm = {};
     if (tma) {
         int e = encode_f32_batched_tmap(&tm.k, a.K, (int64_t)a.B * a.Hkv, a.max_seq, a.dk, a.dk, KT_KEYS, false);

@@ -30,10 +30,13 @@ struct KvTreeArgs {
 constexpr size_t KT_SHARED_BYTES = 256 * sizeof(KvTreeShared);   // (whole lines: the slots behind it begin one)
 constexpr size_t KT_SLOT_BYTES = 128 * (128 + 2) * sizeof(float);   // the largest variant's partial result
 size_t kv_tree_workspace_bytes(int sm_count);
-// query rows of a key head from which on the tensor-memory kernel (kv_tree_tc.cu) takes over; it wants 16-byte pieces
-constexpr int KT_TC_ROWS = 32;
-int launch_kv_tree_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st);
-int launch_kv_cache_attend_tree(const KvTreeArgs &a, int sm_count, cudaStream_t st);
+// query rows of a key head up to which the warp-level kernel is at least as fast as the tensor-memory one (kv_tree_tc.cu), which
+// costs the same for one row or 64.  8 sequences, 8 key heads, 41000 cached rows, warp-level against tensor memory: 16 rows of
+// 128 75 / 120 us, 24 rows 141 / 119, 32 rows of 96 107 / 96, of 64 82 / 82, of 32 53 / 69.
+constexpr int kt_warp_rows(int dk) { return dk > 64 ? 16 : 32; }
+// *launches receives the number of kernels enqueued
+int launch_kv_tree_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st, int *launches);
+int launch_kv_cache_attend_tree(const KvTreeArgs &a, int sm_count, cudaStream_t st, int *launches);
 
 // rows lens[b] + keep[b][i] -> lens[b] + i for i < n_keep[b] in both caches; lens_out[b] = lens[b] + n_keep[b] (or nullptr)
 int launch_kv_cache_compact(float *K, float *V, const int32_t *keep, const int32_t *n_keep, const int32_t *lens, int32_t *lens_out,

@@ -7,14 +7,16 @@
 
 namespace axb {
 
-// query rows of an item, keys of a tile, tiles that a CTA works on side by side (a shorter stretch takes as long, and an item
-// cut into fewer pieces is added up sooner)
+// query rows of an item; keys of a tile; tiles that a CTA works on side by side (a shorter stretch takes as long, and an item
+// cut into fewer pieces is added up sooner); the tiles in whose time a CTA gets from one item to the next: room for them is
+// left on the line behind every item
 struct TreeLine {
-    int block_rows, tile_keys, min_stretch;
+    int block_rows, tile_keys, min_stretch, gap;
 };
 
 struct TreeSeq {
     int len, n, rows, blocks, tiles;   // cached rows, new tokens, query rows of a key head, row blocks, key tiles
+    int room;                          // of an item on the line
 };
 
 __device__ __forceinline__ TreeSeq tree_seq(const KvTreeArgs &a, const TreeLine &ln, int b, bool *bad = nullptr)
@@ -28,11 +30,12 @@ __device__ __forceinline__ TreeSeq tree_seq(const KvTreeArgs &a, const TreeLine 
     s.rows = s.n * (a.H / a.Hkv);
     s.blocks = (s.rows + ln.block_rows - 1) / ln.block_rows;
     s.tiles = s.n ? (s.len + s.n + ln.tile_keys - 1) / ln.tile_keys : 0;
+    s.room = s.n ? s.tiles + ln.gap : 0;
     return s;
 }
 
 // (the launcher refuses batches whose line could pass 2^31 tiles)
-__device__ __forceinline__ int tree_tiles(const KvTreeArgs &a, const TreeSeq &s) { return a.Hkv * s.blocks * s.tiles; }
+__device__ __forceinline__ int tree_tiles(const KvTreeArgs &a, const TreeSeq &s) { return a.Hkv * s.blocks * s.room; }
 
 struct TreeCursor {
     int b;
@@ -119,9 +122,13 @@ __device__ __forceinline__ bool next_piece(const KvTreeArgs &a, const TreeLine &
             ++c.b;
             continue;
         }
-        const int item = (c.pos - c.base) / p.s.tiles, item_pos = c.base + item * p.s.tiles;
+        const int item = (c.pos - c.base) / p.s.room, item_pos = c.base + item * p.s.room;
         p.b = c.b;
         p.t0 = c.pos - item_pos;
+        if (p.t0 >= p.s.tiles) {   // the gap behind an item
+            c.pos = item_pos + p.s.room;
+            continue;
+        }
         p.hk = item / p.s.blocks;
         p.block = item - p.hk * p.s.blocks;
         p.count = min(p.s.tiles - p.t0, c.end - c.pos);

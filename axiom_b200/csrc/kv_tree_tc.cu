@@ -137,7 +137,7 @@ template <int NSLAB, bool FEW>
 __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ TreeTcMaps tm)
 {
     using C = TreeTc<NSLAB, FEW>;
-    constexpr int ROWS = C::ROWS, KB = C::KB, OH = C::DKP / 2, FOLD = OH % 32 || C::WIDE ? 16 : 32;   // OH: output columns of a softmax thread
+    constexpr int GAP = 2, ROWS = C::ROWS, KB = C::KB, OH = C::DKP / 2, FOLD = OH % 32 || C::WIDE ? 16 : 32;   // OH: output columns of a softmax thread
     extern __shared__ __align__(1024) uint8_t sm[];
     const uint32_t base = smem_u32(sm);
     auto bar = [&](int i) -> uint32_t { return base + 8u * (uint32_t)i; };
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
         for (int i = 0; i < 4; ++i) s_odd[i] = 0;
     }
     if (threadIdx.x == 0) a.shared[blockIdx.x] = KvTreeShared{ 0, 0, 0, 0, 0, 0 };   // (this thread replaces it where the CTA begins a shared item)
-    constexpr TreeLine line = { ROWS, KB, 1 };
+    constexpr TreeLine line = { ROWS, KB, 1, GAP };
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;
     if (warp == 19) {
@@ -368,6 +368,17 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
             }
             fence_proxy_async_smem();
             mbar_arrive(bar(TB_Q_FULL));
+            {   // the next piece's rows into L2: there is one Q buffer, and the scores wait for it
+                TreeCursor ahead = cur;
+                TreePiece pn;
+                if (next_piece(a, line, ahead, pn)) {
+                    const int r = pn.block * ROWS + (ct >> 2) % ROWS, gh = r / pn.s.n;
+                    if (r < pn.s.rows && (ct & 3) * 32 < a.dk && ct < 4 * ROWS) {
+                        const float *src = a.Q + (((int64_t)pn.b * a.H + pn.hk * heads_per + gh) * a.T + r - gh * pn.s.n) * a.dk + (ct & 3) * 32;
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+                    }
+                }
+            }
             // K and V blocks in whichever order they can be taken (every warp for itself: its part of a tile is its own)
             uint32_t kt = it, vt = it;
             const uint32_t end = it + p.count;
@@ -391,6 +402,22 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
         // ---------------------------------------------------------- softmax
+        if (FEW && (warp & 3) >= 2) {
+            // The products' rows 64 to 127 come from nowhere and go nowhere; zeros take the least power (at full rate the chip's
+            // limit sets the clock).
+            uint32_t zero[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) zero[c] = 0;
+            const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+            if (warp < 4) {
+#pragma unroll 1
+                for (int c = 0; c < 2 * KB; c += 32) tmem_st_32x32(at + C::T_P + c, zero);
+            } else if (C::WIDE) {
+#pragma unroll 1
+                for (int c = 0; c < C::DKP; c += 32) tmem_st_32x32(at + C::T_QLO + c, zero);
+            }
+            tmem_st_wait();
+        }
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;   // row = lane of tensor memory
         const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };   // the two warps of 32 rows
@@ -682,8 +709,9 @@ static int launch_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st)
     return (int)cudaGetLastError();
 }
 
-int launch_kv_tree_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st)
+int launch_kv_tree_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st, int *launches)
 {
+    *launches = 2;
     if (a.H / a.Hkv <= 64 / a.T) {
         if (a.dk <= 32) return launch_tc<1, true>(a, sm_count, st);
         if (a.dk <= 64) return launch_tc<2, true>(a, sm_count, st);

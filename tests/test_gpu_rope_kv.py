@@ -318,7 +318,16 @@ ATTEND = [
     (40, 2, 2, 1, 64, list(range(0, 400, 10)), True, "tree"),
     (1, 4, 2, 1, 128, [40000], False, "tree"),
     (7, 3, 16, 8, 64, [5000, 0, 1, 2, 3, 64, 4000], True, None),
-    # more than 32 query rows to a key head: 128-row blocks
+    # more rows to a key head than the warp-level kernel takes: up to 64 of them ...
+    (2, 6, 8, 2, 128, [700, 64], True, "tree"),
+    (3, 8, 8, 2, 96, [0, 130, 4097], True, "tree"),
+    (2, 5, 12, 3, 72, [63, 1], False, "shared"),
+    (1, 17, 1, 1, 128, [47], False, "tree"),             # the new tokens end with a block
+    (2, 16, 8, 2, 64, [900, 127], True, "tree"),
+    (4, 9, 14, 2, 36, [0, 2000, 119, 5], True, "tree"),
+    (70, 3, 16, 2, 128, list(range(0, 700, 10)), True, "tree"),
+    (1, 16, 4, 1, 100, [20000], False, "tree"),          # one item over every CTA
+    # ... and more
     (2, 1, 64, 1, 64, [300, 1000], False, None),
     (2, 3, 12, 1, 32, [0, 129], True, "tree"),
     (3, 33, 2, 2, 128, [63, 64, 0], True, "tree"),
@@ -437,6 +446,43 @@ def test_values_in_unseen_rows_reach_nobody(engine, case, bad):
                 assert bool(torch.isfinite(got[b, :, t, 7]).all()) != hit
                 rest = torch.cat((got[b, :, t, :7], got[b, :, t, 8:]), -1)
                 assert torch.equal(rest, torch.cat((clean.view(B, H, T, dk)[b, :, t, :7], clean.view(B, H, T, dk)[b, :, t, 8:]), -1))
+
+
+@pytest.mark.parametrize("case", [(2, 3, 4, 2, 64, [100, 333], True, "tree"), (2, 12, 8, 2, 128, [100, 333], True, "tree"),
+                                  (2, 12, 8, 2, 64, [300, 20], True, "tree"), (1, 140, 2, 1, 64, [200], False, "tree"),
+                                  (1, 140, 1, 1, 96, [64], False, None)], ids=lambda c: "-".join(map(str, c[:5])))
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1.0])
+def test_scales(engine, case, scale):
+    """A negative scale turns the order of the scores round, zero gives the mean of the rows seen."""
+    s = attend_case(case, 73)
+    s["scale"] = scale
+    check_attend(s, run_attend(engine, s))
+
+
+def test_many_short_sequences(engine):
+    """More sequences than CTAs, than threads of a CTA: the work line is found in steps of 32 sequences."""
+    rng = np.random.RandomState(5)
+    for T, H, dk in ((1, 2, 32), (5, 8, 68)):
+        B, g = 1300, gen(75)
+        lens, n = rng.randint(0, 50, B), rng.randint(0, T + 1, B)
+        s = dict(K=randn(g, B, 60, dk), V=randn(g, B, 60, dk), Q=randn(g, B * H, T, dk), out=randn(g, B * H, T, dk), lens=ints(lens), n_new=ints(n),
+                 mask=None, scale=0.2)
+        check_attend(s, run_attend(engine, s))
+
+
+@pytest.mark.parametrize("case", [(4, 2, 8, 2, 128, [3000, 5, 700, 64], True, "tree"), (3, 4, 16, 4, 128, [2000, 900, 0], True, "tree"),
+                                  (3, 16, 16, 4, 128, [4000, 300, 64], True, "tree"), (3, 16, 16, 4, 64, [4000, 300, 64], True, "tree"),
+                                  (2, 64, 12, 4, 64, [2500, 1000], True, "tree"), (2, 40, 8, 2, 112, [1500, 100], True, "tree")],
+                         ids=lambda c: "-".join(map(str, c[:5])))
+def test_the_same_call_many_times(engine, case):
+    """Loads, products and partial results land in a different order every time; the result has the same bits."""
+    s = attend_case(case, 77)
+    first = run_attend(engine, s)
+    out = s["out"].clone()
+    for _ in range(150):
+        engine.kv_cache_attend_tree(s["K"], s["V"], s["Q"], out, s["lens"], s["scale"], n_new=s["n_new"], mask=s["mask"])
+        assert torch.equal(out, first)
+    assert engine.device_error() == 0
 
 
 def test_large_scores(engine):
