@@ -365,17 +365,15 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
     // pieces (ASYNC): prepared, done with; partial results: all there, taken
     const uint32_t piece_full = bar0 + 8u * (4 * C::STAGES), piece_empty = piece_full + 16, merge_full = piece_full + 32, merge_empty = piece_full + 40;
     auto ktile = [&](int stage) { return tiles + stage * 2 * C::TILE; };
-    if (tid == 0) {
-        s_gave_up = 0;
-        for (int i = 0; i < 4 * C::STAGES; ++i) mbar_init(bar0 + 8u * i, i < 2 * C::STAGES ? C::SLICES : (tma ? 1 : 32));
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(piece_full + 8 * i, 1);
-            mbar_init(piece_empty + 8 * i, KT_CONSUMERS + 1);
-        }
-        mbar_init(merge_full, KT_CONSUMERS);
-        mbar_init(merge_empty, 1);
+    // a call of a few microseconds: a thread a barrier, the descriptors on their way
+    static_assert(4 * C::STAGES + 6 <= KT_CONSUMERS * 32, "barriers");
+    if (tid < 4 * C::STAGES + 6) {
+        const int k = tid - 4 * C::STAGES;
+        mbar_init(bar0 + 8u * tid, k < -2 * C::STAGES ? C::SLICES : k < 0 ? (tma ? 1 : 32) : k == 2 || k == 3 ? KT_CONSUMERS + 1 : k == 4 ? KT_CONSUMERS : 1);
         mbar_fence_init();
     }
+    if (tid == 0) s_gave_up = 0;
+    if (tma && lane == 0 && (warp == KT_CONSUMERS || warp == KT_CONSUMERS + 1)) tma_prefetch_desc(warp == KT_CONSUMERS ? &tm.k : &tm.v);
     constexpr TreeLine line = { ROWS, KT_KEYS, C::GROUPS, C::ASYNC ? 0 : 4 };
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;   // (its barriers make the initialised ones above visible)

@@ -154,18 +154,15 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     static_assert(8 * TB_COUNT <= 256, "barriers");
 
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < TB_COUNT; ++i) mbar_init(bar(i), 1);
-        mbar_init(bar(TB_Q_FULL), 256);
-        mbar_init(bar(TB_K_FULL), 256);
-        mbar_init(bar(TB_V_FULL), 256);
-        mbar_init(bar(TB_P_FULL), C::SOFTMAX);
-        mbar_init(bar(TB_PLO_FULL), C::SOFTMAX);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(TB_S_EMPTY + i), C::SOFTMAX);
-            mbar_init(bar(TB_O_EMPTY + i), C::SOFTMAX);
-        }
+    if (threadIdx.x < TB_COUNT) {   // a thread a barrier
+        const int i = threadIdx.x;
+        const bool conv = i == TB_Q_FULL || i == TB_K_FULL || i == TB_V_FULL;
+        const bool soft = i == TB_P_FULL || i == TB_PLO_FULL || (i >= TB_S_EMPTY && i < TB_S_EMPTY + 2) || (i >= TB_O_EMPTY && i < TB_O_EMPTY + 2);
+        mbar_init(bar(i), conv ? 256 : soft ? C::SOFTMAX : 1);
         mbar_fence_init();
+    }
+    if (lane == 0 && (warp == 16 || warp == 17)) tma_prefetch_desc(warp == 17 ? &tm.v : &tm.k);
+    if (threadIdx.x == 0) {
         s_gave_up = 0;
         for (int i = 0; i < 4; ++i) s_odd[i] = 0;
     }
@@ -205,7 +202,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
             const bool v = warp == 17;
             const int stages = v ? C::VS : C::KS, b_raw = v ? TB_V_RAW : TB_K_RAW, b_empty = v ? TB_V_EMPTY : TB_K_EMPTY;
             const void *map = v ? &tm.v : &tm.k;
-            tma_prefetch_desc(map);
             while (ok && next_piece(a, line, cur, p)) {
                 const int head = p.b * a.Hkv + p.hk;
                 for (int i = 0; i < p.count; ++i, ++it) {
