@@ -1588,8 +1588,8 @@ extern "C" int axb_kv_cache_attend_tree(const float *K_cache, const float *V_cac
     if (dk > 128) return fail(AXB_ERR_NOT_IMPLEMENTED, "kv_cache_attend_tree: head dim %lld > 128", (long long)dk);
     if (H > 65535 || B > INT32_MAX / Hkv || max_seq > (1 << 30) || T > INT32_MAX / H || (B && T * H > INT32_MAX / B))
         return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: dimension too large");
-    // the work line counts tiles of at least 32 keys and 8 query rows, and up to 4 more an item, in 31 bits
-    if (B && (max_seq / 32 + 5) > (1 << 30) / (B * Hkv) / ((H / Hkv * T + 7) / 8 > 0 ? (H / Hkv * T + 7) / 8 : 1))
+    // the work line counts tiles of at least 32 keys and 8 query rows, and up to 8 more an item, in 31 bits
+    if (B && (max_seq / 32 + 9) > (1 << 30) / (B * Hkv) / ((H / Hkv * T + 7) / 8 > 0 ? (H / Hkv * T + 7) / 8 : 1))
         return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: more than 2^30 tiles");
     if (!isfinite(scale)) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: scale %g", (double)scale);
     if (B == 0 || T == 0) return ensure_ready();

@@ -22,14 +22,14 @@
 //
 // Work split: the tiles of 32 keys of all (sequence, key head, row block) items form one line, cut into equal pieces,
 // one per SM (kv_tree_line.cuh) — lengths differ by orders of magnitude in a batch, and the device knows them, not the
-// host.  A piece that
-// does not hold an item's whole line leaves (max, sum, unnormalised output) in its workspace slot; the CTA that
-// arrives last at the item's counter adds the pieces in line order (nobody waits; the result does not depend on who was
-// last) and clears the counter.
+// host.  A piece that does not hold an item's whole line leaves (max, sum, unnormalised output) in its workspace slot; the
+// CTA that arrives last at the item's counter adds the pieces in line order (nobody waits; the result does not depend on
+// who was last) and clears the counter.
 //
 // One CTA per SM: two producer warps feed K and V tiles through a ring; eight warps each take 16 keys of a tile with
 // a running softmax of their own, added up at the end of a piece — up to 8 rows (16 of narrower heads) by a merger warp
-// while the eight are at the next piece, which a scout warp has prepared.
+// while the eight are at the next piece, which a scout warp has prepared.  32 sequences of 400 to 4100 rows, 8 key heads of 128
+// (592 MB): 98 us, 6.0 TB/s, 0.92 of the copy bandwidth; without scout and merger 117.
 #include "kv_tree.cuh"
 
 #include "errors.cuh"
@@ -56,6 +56,9 @@ struct TreeCfg {
     // adds up and writes the finished one while the consumers go on; otherwise the consumers do both themselves, between
     // barriers (each costs a piece some 7,000 cycles, in which the ring stands still).
     static constexpr bool ASYNC = NR == 1 || (NR == 2 && DKP <= 96);
+    // From one item to the next a CTA takes the time of several tiles (256 sequences of 280 rows, 8 key heads of 128, 599 MB: no
+    // room for it on the line 173 us, 3 tiles 154, 5 140, 8 139; of 64: 97, -, 80, 80).
+    static constexpr int GAP = ASYNC ? 5 : 8;
     static constexpr bool SPLIT_Q = NR < 4;                           // Q lies in shared memory as hi and lo
     static constexpr int TILE = KT_KEYS * DKP * 4;                    // bytes of a K or V tile
     static constexpr int Q_BYTES = ROWS * DKP * 4 * (SPLIT_Q ? 2 : 1);
@@ -374,7 +377,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
     }
     if (tid == 0) s_gave_up = 0;
     if (tma && lane == 0 && (warp == KT_CONSUMERS || warp == KT_CONSUMERS + 1)) tma_prefetch_desc(warp == KT_CONSUMERS ? &tm.k : &tm.v);
-    constexpr TreeLine line = { ROWS, KT_KEYS, C::GROUPS, C::ASYNC ? 0 : 4 };
+    constexpr TreeLine line = { ROWS, KT_KEYS, C::GROUPS, C::GAP };
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;   // (its barriers make the initialised ones above visible)
     TreePiece p;

@@ -4,17 +4,25 @@
 //     core reads its tf32 part), the remainder rounded to tf32 the lo operand.
 // The work line of kv_tree_line.cuh, cut into one stretch per CTA, replaces the grid over query tiles; key blocks of 128
 // (head dim <= 64) or 64 keys.  Twenty warps:
-//   0-7   softmax: two threads per query row, half the block's columns each (they swap maxima through shared memory).  P hi is
-//         written over the scores in tensor memory, P lo beside them: both are the A operand of P.V as they lie.  The
-//         exponent's reference stays until a score passes it by 2^8; every block's P.V starts from zero and is folded into
-//         fp32 registers, so the tensor core's truncating accumulation never spans more than a block.
+//   0-7   softmax: two threads per query row, half the block's columns each (they swap maxima through shared memory).  Scores
+//         leave tensor memory once and stay in registers; P hi and lo go to columns of their own, the A operands of P.V as
+//         they lie, when the block before has read its own.  The exponent's reference stays until a score passes it by
+//         2^8; every block's P.V starts from zero and is folded into fp32 registers, so the tensor core's truncating
+//         accumulation never spans more than a block.
 //   8-15  Q of a piece (gathered rows -> swizzled shared memory, lo part there or, for head dims above 64, in tensor
 //         memory), the lo parts of the K and V blocks, and what must not reach the V product: rows behind the last token,
 //         and infinities or NaN in new rows (those are added row by row);
-//   16, 17  TMA of K and V (the operand whose chain is the longer one has two raw buffers: V for head dims up to 64, K above);
+//   16, 17  TMA of K and V (with 128 rows one operand has two raw buffers, the one whose chain is the longer: V for head dims up
+//         to 64, K above; with 64 both do);
 //   18, 19  one thread each issues the score and the P.V products.
-// Shared memory is full either way (224 KB): Q 64 KB, five K / V tiles of 32 KB.  A block costs the same for one row or 128; up to
-// 32 rows the warp-level kernel is the faster one.
+// Shared memory is full either way (224 KB): Q, K and V and their lo parts, seven tiles of 32 KB.
+//
+// What bounds it: 128 rows a product whatever the query rows, so a block of 64 keys of head dim 128 costs the pipe 3,840 cycles
+// (48 products of 48 cycles, 24 of 64) and its operands 4,100 cycles of shared memory, against 2,800 in which HBM brings its
+// keys; 4,500 to 5,900 were measured, the softmax threads' 3,500 to 4,500 among them, at a clock that the power limit holds at
+// 1.77 GHz.  8 sequences, 8 key heads of 128 with 64 rows, 41000 cached rows (338 MB): 120 us; with P over the scores, where
+// a block's scores had to wait for the products of the last but one, 162.  6 key heads of 64 with 256 rows: 72 us, 112 TFLOP/s
+// of the three products' 273.
 #include "errors.cuh"
 #include "gemm_tc.cuh"
 #include "kv_tree_line.cuh"
@@ -137,6 +145,7 @@ template <int NSLAB, bool FEW>
 __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ TreeTcMaps tm)
 {
     using C = TreeTc<NSLAB, FEW>;
+    // (GAP, blocks of room for the way to the next item: none 123 and 78 us for the two batches above, 2 120 and 72, 4 122 and 76)
     constexpr int GAP = 2, ROWS = C::ROWS, KB = C::KB, OH = C::DKP / 2, FOLD = OH % 32 || C::WIDE ? 16 : 32;   // OH: output columns of a softmax thread
     extern __shared__ __align__(1024) uint8_t sm[];
     const uint32_t base = smem_u32(sm);
