@@ -1414,7 +1414,7 @@ static_assert(sizeof(int) * 3 * 256 <= kAttnCounters && sizeof(KvTreeShared) * 2
 
 size_t attn_workspace_bytes()
 {
-    const size_t tree = kv_tree_workspace_bytes(cur().sm_count), bwd = (size_t)cur().sm_count * 4 * 2 * 256 * sizeof(float);
+    const size_t tree = kv_tree_workspace_bytes(cur().sm_count), bwd = qkv_norm_rope_bwd_bytes(cur().sm_count);
     return kAttnCounters + (tree > bwd ? tree : bwd);
 }
 
@@ -1515,6 +1515,8 @@ extern "C" int axb_qkv_norm_rope(const float *qkv, const float *bqkv, const floa
     const int64_t nq = B * S * H * dk, nk = B * S * Hkv * dk, n = nq + 2 * nk;
     if (overlaps(qkv, n, Qh, nq) || overlaps(qkv, n, Kh, nk) || overlaps(qkv, n, Vh, nk))
         return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope: an output overlaps qkv");
+    if (overlaps(Qh, nq, Kh, nk) || overlaps(Qh, nq, Vh, nk) || overlaps(Kh, nk, Vh, nk))
+        return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope: two outputs overlap");
     if ((st = ensure_ready())) return st;
     OnDevice on;
     a.q = Qh; a.k = Kh; a.v = Vh;
@@ -1567,6 +1569,8 @@ extern "C" int axb_kv_cache_extend(const float *qkv, const float *bqkv, const fl
     const int64_t nq = B * T * H * dk, n = nq + 2 * B * T * Hkv * dk, nc = B * Hkv * max_seq * dk;
     if (overlaps(qkv, n, Qh, nq) || overlaps(qkv, n, K_cache, nc) || overlaps(qkv, n, V_cache, nc))
         return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_extend: an output overlaps qkv");
+    if (overlaps(Qh, nq, K_cache, nc) || overlaps(Qh, nq, V_cache, nc) || overlaps(K_cache, nc, V_cache, nc))
+        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_extend: two outputs overlap");
     if ((st = ensure_ready())) return st;
     OnDevice on;
     a.lens = lens; a.n_new = n_new;

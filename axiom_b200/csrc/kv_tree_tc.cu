@@ -52,7 +52,7 @@ struct TreeTc {
     static constexpr int T_S = 0, T_P = SB * KB, T_PLO = T_P + KB, T_O = T_PLO + KB, T_QLO = T_O + OB * DKP;
     static constexpr int COLS = 512;
     static_assert(T_QLO + (WIDE ? DKP : 0) <= COLS, "tensor memory");
-    static constexpr int HEADER = 3072;   // barriers, words, then the softmax threads' maxima
+    static constexpr int HEADER = 3 * 1024;   // barriers, words, then the softmax threads' maxima
     static constexpr int Q_AT = HEADER, K_AT = Q_AT + QPLANE * (WIDE ? 1 : 2), KLO_AT = K_AT + KS * PLANE, V_AT = KLO_AT + PLANE,
                          VLO_AT = V_AT + VS * PLANE, SMEM = VLO_AT + PLANE;
     static_assert(SMEM <= 227 * 1024, "shared memory");   // all of it: the kernel has no static shared memory
@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     volatile int &s_gave_up = words[0], *s_odd = words + 2;   // s_odd: block it + 1 holds non-finite new values
     int *s_row = reinterpret_cast<int *>(sm + 512);   // [ROWS]
     float (*s_max)[2][ROWS] = reinterpret_cast<float (*)[2][ROWS]>(sm + 1024);   // [block parity][half][row]
+    if (threadIdx.x == 0) a.shared[blockIdx.x] = KvTreeShared{ 0, 0, 0, 0, 0, 0 };   // (this thread replaces it where the CTA begins a shared item)
     if (base & 1023) {   // the swizzles are functions of the address (it starts at a multiple of 1 KB; refused, should it ever not)
         if (threadIdx.x == 0 && a.err) atomicCAS(a.err, 0, (int)CERR_LOAD);
         return;
@@ -175,7 +176,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
         s_gave_up = 0;
         for (int i = 0; i < 4; ++i) s_odd[i] = 0;
     }
-    if (threadIdx.x == 0) a.shared[blockIdx.x] = KvTreeShared{ 0, 0, 0, 0, 0, 0 };   // (this thread replaces it where the CTA begins a shared item)
     constexpr TreeLine line = { ROWS, KB, 1, GAP };
     TreeCursor cur;
     if (!tree_start(a, line, s_line, cur)) return;

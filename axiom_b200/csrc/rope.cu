@@ -576,9 +576,9 @@ int launch_qkv_norm_rope(const RopeArgs &a, int sm_count, cudaStream_t st)
     return (int)cudaGetLastError();
 }
 
-int qkv_norm_rope_bwd_blocks(const RopeArgs &a, int sm_count)
+size_t qkv_norm_rope_bwd_bytes(int sm_count)
 {
-    return rope_plan(a, rope_vec(a, nullptr, nullptr), sm_count, true).blocks;
+    return (size_t)sm_count * RP_BWD_CTAS * 2 * 256 * sizeof(float);
 }
 
 int launch_qkv_norm_rope_bwd(const RopeArgs &a, float *dgq, float *dgk, int sm_count, cudaStream_t st, int *launches)

@@ -17,7 +17,7 @@ struct RopeArgs {
     const int32_t *lens, *n_new; // cache form only: [B]; n_new nullptr = T for every sequence
     float *q, *k, *v;            // head-major [B*H, T, dk], [B*Hkv, kv_rows, dk] twice (read by the backward)
     float *dqkv;                 // backward: the gradient of qkv
-    float *partial;              // backward: [grid][2*dk] partial sums of the norm weights' gradients
+    float *partial;              // backward, qkv_norm_rope_bwd_bytes(): [grid][2*dk] partial sums of the norm weights' gradients
     int64_t kv_rows;             // T, or the rows of a cache
     int *err;
     float eps, amplitude;
@@ -25,8 +25,8 @@ struct RopeArgs {
 };
 
 int launch_qkv_norm_rope(const RopeArgs &a, int sm_count, cudaStream_t st);
-// blocks of the backward kernel (the partial buffer holds 2*dk floats for each)
-int qkv_norm_rope_bwd_blocks(const RopeArgs &a, int sm_count);
+// the most that the backward's partial sums take, whatever the shape
+size_t qkv_norm_rope_bwd_bytes(int sm_count);
 // dgq / dgk [dk] are added to (nullptr: not wanted); *launches receives the number of kernels enqueued
 int launch_qkv_norm_rope_bwd(const RopeArgs &a, float *dgq, float *dgk, int sm_count, cudaStream_t st, int *launches);
 

@@ -454,7 +454,8 @@ AXB_API int axb_rope_frequencies(int64_t rot, double base, int scaling, double f
      * g / sqrt(mean(x^2) + eps), g = gq, gk [dk]  (NULL: that tensor is not normed)
      rotation of the first rot elements by p * freq[i], the results times amplitude   (rot == 0: none, freq may be NULL)
    p = pos[b*S + s] (int32), or s when pos is NULL.  freq: [rot/2] doubles on the device.  H is a multiple of Hkv; rot is
-   even and at most dk; dk <= 256.  The outputs may not overlap qkv. */
+   even and at most dk; dk <= 256.  The outputs may overlap
+   neither qkv nor one another. */
 AXB_API int axb_qkv_norm_rope(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
                               const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos, int64_t B,
                               int64_t S, int64_t H, int64_t Hkv, int64_t dk, float *Qh, float *Kh, float *Vh);

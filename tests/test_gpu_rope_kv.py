@@ -499,6 +499,23 @@ def test_large_scores(engine):
     assert bool(close.all())
 
 
+def test_binding_refuses_wrong_types_and_strides(engine):
+    z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    lens, keep = z(2, dtype=torch.int32), z(2, 5, dtype=torch.int32)
+    ok = dict(K_cache=z(4, 32, 16), V_cache=z(4, 32, 16), Q=z(8, 3, 16), out=z(8, 3, 16), lens=lens, scale=1.0)
+    for bad, what in ((dict(lens=lens.long()), "int32"), (dict(Q=z(3, 8, 16).transpose(0, 1)), "contiguous"), (dict(Q=z(8, 3, 16).double()), "float32"),
+                      (dict(mask=z(2, 3, 1, dtype=torch.int32)), "int64"), (dict(mask=z(3, 2, dtype=torch.int64)), "mask"),
+                      (dict(out=z(8, 2, 16)), "out"), (dict(V_cache=z(4, 31, 16)), "head-major"), (dict(n_new=z(3, dtype=torch.int32)), "n_new"),
+                      (dict(workspace=z(64)), "workspace")):
+        with pytest.raises(ValueError, match=what):
+            engine.kv_cache_attend_tree(**{**ok, **bad})
+    with pytest.raises(ValueError, match="float64"):
+        engine.qkv_norm_rope(z(6, 128), z(8, 3, 16), z(4, 3, 16), z(4, 3, 16), 2, freq=z(8))
+    with pytest.raises(ValueError, match="int32"):
+        engine.kv_cache_compact(ok["K_cache"], ok["V_cache"], keep.long(), lens, lens.clone())
+    assert engine.device_error() == 0
+
+
 def test_empty_calls(engine):
     z = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
     lens0, lens = ints([]), ints([2])

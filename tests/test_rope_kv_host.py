@@ -84,18 +84,20 @@ SHARED = [(dict(freq=None), NULL_ARG), (dict(rot=66), INVALID_SHAPE), (dict(rot=
 REFUSED = (
     [("axb_qkv_norm_rope", rope_call, o, st) for o, st in SHARED] +
     [("axb_qkv_norm_rope", rope_call, o, st) for o, st in [(dict(Q=None), NULL_ARG), (dict(V=None), NULL_ARG), (dict(S=-1), INVALID_SHAPE),
-                                                           (dict(K=P[0] + 64), INVALID_SHAPE)]] +
+                                                           (dict(K=P[0] + 64), INVALID_SHAPE), (dict(V=P[3]), INVALID_SHAPE), (dict(K=P[2] + 256), INVALID_SHAPE)]] +
     [("axb_qkv_norm_rope_bwd", bwd_call, o, st) for o, st in SHARED] +
     [("axb_qkv_norm_rope_bwd", bwd_call, o, st) for o, st in [(dict(gq=None), NULL_ARG), (dict(gk=None), NULL_ARG), (dict(dqkv=None), NULL_ARG),
                                                               (dict(dqkv=P[0]), INVALID_SHAPE), (dict(dqkv=P[3]), INVALID_SHAPE)]] +
     [("axb_kv_cache_extend", extend_call, {("T" if k == "S" else k): v for k, v in o.items()}, st) for o, st in SHARED] +
     [("axb_kv_cache_extend", extend_call, o, st) for o, st in [(dict(lens=None), NULL_ARG), (dict(K=None), NULL_ARG), (dict(max_seq=0), INVALID_SHAPE),
-                                                               (dict(max_seq=1 << 31), INVALID_SHAPE), (dict(V=P[0]), INVALID_SHAPE)]] +
+                                                               (dict(max_seq=1 << 31), INVALID_SHAPE), (dict(V=P[0]), INVALID_SHAPE), (dict(V=P[3] + 512), INVALID_SHAPE),
+                                                               (dict(Q=P[4]), INVALID_SHAPE)]] +
     [("axb_kv_cache_attend_tree", attend_call, o, st) for o, st in [
         (dict(K=None), NULL_ARG), (dict(V=None), NULL_ARG), (dict(Q=None), NULL_ARG), (dict(lens=None), NULL_ARG), (dict(out=None), NULL_ARG),
         (dict(B=-1), INVALID_SHAPE), (dict(T=-1), INVALID_SHAPE), (dict(H=5), INVALID_SHAPE), (dict(Hkv=0), INVALID_SHAPE), (dict(dk=0), INVALID_SHAPE),
         (dict(dk=129), NOT_IMPLEMENTED), (dict(max_seq=0), INVALID_SHAPE), (dict(max_seq=1 << 31), INVALID_SHAPE), (dict(scale=float("inf")), INVALID_SHAPE),
-        (dict(T=1 << 30), INVALID_SHAPE), (dict(out=P[2]), INVALID_SHAPE), (dict(out=P[0]), INVALID_SHAPE)]] +
+        (dict(T=1 << 30), INVALID_SHAPE), (dict(max_seq=(1 << 30) + 1), INVALID_SHAPE), (dict(max_seq=1 << 30, B=64), INVALID_SHAPE),
+        (dict(B=1 << 30), INVALID_SHAPE), (dict(out=P[2]), INVALID_SHAPE), (dict(out=P[0]), INVALID_SHAPE)]] +
     [("axb_kv_cache_compact", compact_call, o, st) for o, st in [
         (dict(K=None), NULL_ARG), (dict(keep=None), NULL_ARG), (dict(n_keep=None), NULL_ARG), (dict(lens=None), NULL_ARG), (dict(Hkv=0), INVALID_SHAPE),
         (dict(T=-1), INVALID_SHAPE), (dict(max_seq=0), INVALID_SHAPE), (dict(dk=0), INVALID_SHAPE), (dict(lens_out=P[4]), INVALID_SHAPE),
@@ -122,6 +124,12 @@ def test_binding_refuses_wrong_tensors(eng):
         eng.qkv_norm_rope(z(6, 100), z(8, 3, 16), z(4, 3, 16), z(4, 3, 16), 2)
     with pytest.raises(ValueError):
         eng.kv_cache_compact(k, k.clone(), z(2, 5, dtype=torch.int64), lens, lens)
+
+
+def test_binding_refuses_host_tensors(eng):
+    k = torch.zeros(4, 32, 16)
+    with pytest.raises(ValueError, match="engine's device"):
+        eng.kv_cache_attend_tree(k, k.clone(), torch.zeros(8, 3, 16), torch.zeros(8, 3, 16), torch.zeros(2, dtype=torch.int32), 1.0)
 
 
 def test_restated_gradient_against_differences():
