@@ -16,7 +16,6 @@ ENGINE_SO = os.path.join(PKG, "lib", "libaxiom_b200.so")
 
 ACT = {"none": 0, None: 0, "relu": 1, "gelu": 2}
 ROPE_SCALING = {"none": 0, None: 0, "linear": 1, "turns": 2, "index": 3}
-_TYPE_NAME = {}   # element types met so far, by name
 ROPE_PAIRING = {"half": 0, "interleaved": 1}
 FP32_MODES = {"3xtf32": 0, "bf16x3": 1, "bf16": 2}
 
@@ -62,6 +61,29 @@ def _ptr(t):
 
 _i64 = C.c_int64
 _f = C.c_float
+
+
+# The addresses of the buffers of the calls that run in a few microseconds on the device: written for the time it takes.
+_TYPE_NAME = {}   # element types met so far, by name ("torch.float32": the binding imports no torch)
+
+
+def _addr(t, dtype="float32"):
+    """t's address: a contiguous device tensor of the named element type, an address already, or None."""
+    if t is None:
+        return None
+    try:
+        if _TYPE_NAME[t.dtype] == dtype and t.is_cuda and t.is_contiguous():
+            return t.data_ptr()
+    except (AttributeError, KeyError):
+        if isinstance(t, int):
+            return t
+        _TYPE_NAME[t.dtype] = str(t.dtype)[6:]
+        return _addr(t, dtype)
+    if _TYPE_NAME[t.dtype] != dtype:
+        raise ValueError(f"a {dtype} tensor is wanted, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"a contiguous tensor is wanted, got strides {tuple(t.stride())}")
+    raise ValueError(f"a tensor on the engine's device is wanted, got {t.device}")
 
 
 class Engine:
@@ -406,28 +428,12 @@ class Engine:
         self._check(self.lib.axb_rope_frequencies(rot, base, ROPE_SCALING[scaling], factor, low, high, original_len, out))
         return list(out[:rot // 2])
 
-    # (These calls run in a few microseconds on the device: what is written here more tersely than elsewhere is what made
-    # half of a small call's time.  Messages are formed where they are needed.)
-    @staticmethod
-    def _addr(t, dtype="float32"):
-        # dtype: the name of the element type a buffer must have
-        if t is None or t.__class__ is int:
-            return t
-        if _TYPE_NAME.get(t.dtype) != dtype:
-            if _TYPE_NAME.setdefault(t.dtype, str(t.dtype)[6:]) != dtype:   # ("torch.float32": the binding imports no torch)
-                raise ValueError(f"a {dtype} tensor is wanted, got {t.dtype}")
-        if not t.is_contiguous():
-            raise ValueError(f"a contiguous tensor is wanted, got strides {tuple(t.stride())}")
-        if not t.is_cuda:
-            raise ValueError(f"a tensor on the engine's device is wanted, got {t.device}")
-        return t.data_ptr()
-
     @staticmethod
     def _wants(what):
         raise ValueError(what)
 
     def _rope(self, rows, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos):
-        width, p = (H + 2 * Hkv) * dk, self._addr
+        width, p = (H + 2 * Hkv) * dk, _addr
         if qkv is not None and qkv.shape != (rows, width) and not qkv.shape[0] == rows == 0:
             self._wants(f"qkv: [{rows}, {width}] is wanted")
         if bias is not None and bias.numel() != width:
@@ -453,7 +459,7 @@ class Engine:
         H, Hkv, S, rows, dk = self._heads(B, Qh, Kh, Vh, "Qh, Kh, Vh")
         if rows != S:
             self._wants("Qh, Kh, Vh: head-major shapes")
-        p = self._addr
+        p = _addr
         self._check(self.lib.axb_qkv_norm_rope(*self._rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos),
                                                B, S, H, Hkv, dk, p(Qh), p(Kh), p(Vh)))
         return Qh, Kh, Vh
@@ -466,7 +472,7 @@ class Engine:
             self._wants("dQh, dKh, dVh: head-major shapes")
         if dqkv.shape != (B * S, (H + 2 * Hkv) * dk) or any(g is not None and g.numel() != dk for g in (dgq, dgk)):
             self._wants("dqkv, dgq, dgk: shapes")
-        p = self._addr
+        p = _addr
         self._check(self.lib.axb_qkv_norm_rope_bwd(*self._rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos),
                                                    p(dQh), p(dKh), p(dVh), B, S, H, Hkv, dk, p(dqkv), p(dgq), p(dgk),
                                                    self._workspace(workspace)))
@@ -493,7 +499,7 @@ class Engine:
         H, Hkv, T, max_seq, dk = self._heads(B, Qh, K_cache, V_cache, "Qh, K_cache, V_cache")
         if n_new is not None and n_new.numel() != B:
             self._wants("n_new: one count for each sequence")
-        p = self._addr
+        p = _addr
         self._check(self.lib.axb_kv_cache_extend(*self._rope(B * T, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos),
                                                  p(lens, "int32"), p(n_new, "int32"), B, T, H, Hkv, max_seq, dk, p(Qh), p(K_cache),
                                                  p(V_cache)))
@@ -513,7 +519,7 @@ class Engine:
                 self._wants(f"mask: [{B}, {T}, {words}] or [{T}, {words}] is wanted")
         if n_new is not None and n_new.numel() != B:
             self._wants("n_new: one count for each sequence")
-        p = self._addr
+        p = _addr
         self._check(self.lib.axb_kv_cache_attend_tree(p(K_cache), p(V_cache), p(Q), p(mask, "int64"), each, p(lens, "int32"),
                                                       p(n_new, "int32"), p(out), B, H, Hkv, T, max_seq, dk, scale,
                                                       self._workspace(workspace)))
@@ -526,7 +532,7 @@ class Engine:
         if (B * Hkv != BHkv or K_cache.shape != V_cache.shape or keep.numel() != B * T or n_keep.numel() != B or
                 (lens_out is not None and lens_out.numel() != B)):
             self._wants("K_cache, V_cache, keep, n_keep, lens_out: shapes")
-        p = self._addr
+        p = _addr
         self._check(self.lib.axb_kv_cache_compact(p(K_cache), p(V_cache), p(keep, "int32"), p(n_keep, "int32"), p(lens, "int32"),
                                                   p(lens_out, "int32"), B, Hkv, T, max_seq, dk))
         return lens_out
