@@ -126,12 +126,15 @@ __device__ __forceinline__ void tree_tile(const KvTreeArgs &a, TreeWarp<DKP, NR>
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // S^T: rows g, g+8 = keys row0 + perm(g) (+ 8), columns 2t, 2t+1 of each eight query rows; the cross products in chains of
     // their own, which shortens the dependent chain
-    float sc[NR][4], x1[NR][4], x2[NR == 1 ? NR : 1][4];
+    // (and the sum of the large ones in two: every accumulation cuts its sum off)
+    constexpr int CH = NR <= 2 ? 2 : 1;
+    float sc[NR][4], sc1[CH == 2 ? NR : 1][4], x1[NR][4], x2[NR == 1 ? NR : 1][4];
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             sc[n][e] = x1[n][e] = 0.f;
+            if (CH == 2) sc1[CH == 2 ? n : 0][e] = 0.f;
             if (NR == 1) x2[0][e] = 0.f;
         }
     const int krow = row0 + key_perm(g);
@@ -159,7 +162,7 @@ __device__ __forceinline__ void tree_tile(const KvTreeArgs &a, TreeWarp<DKP, NR>
             mma_tf32(sc[n], hi[0], __float_as_uint(q.x), __float_as_uint(q.y));
             mma_tf32(NR == 1 ? x2[0] : x1[n], hi[0], __float_as_uint(r.x), __float_as_uint(r.y));
             mma_tf32(x1[n], lo[1], __float_as_uint(q.z), __float_as_uint(q.w));
-            mma_tf32(sc[n], hi[1], __float_as_uint(q.z), __float_as_uint(q.w));
+            mma_tf32(CH == 2 ? sc1[CH == 2 ? n : 0] : sc[n], hi[1], __float_as_uint(q.z), __float_as_uint(q.w));
             mma_tf32(NR == 1 ? x2[0] : x1[n], hi[1], __float_as_uint(r.z), __float_as_uint(r.w));
         }
     }
@@ -172,7 +175,8 @@ __device__ __forceinline__ void tree_tile(const KvTreeArgs &a, TreeWarp<DKP, NR>
     for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float x = (sc[n][e] + (NR == 1 ? x1[n][e] + x2[0][e] : x1[n][e])) * a.c_log2;
+            const float top = CH == 2 ? sc[n][e] + sc1[CH == 2 ? n : 0][e] : sc[n][e];
+            float x = (top + (NR == 1 ? x1[n][e] + x2[0][e] : x1[n][e])) * a.c_log2;
             if (TAIL) {
                 const int j = key0 + krow + 8 * (e >> 1) - s.len;   // < 0: a cached row
                 if (j >= 0 && (j >= s.n || !tree_sees(a, b, toks[8 * n + 2 * t + (e & 1)], j))) x = -INFINITY;
