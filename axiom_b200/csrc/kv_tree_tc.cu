@@ -1,5 +1,5 @@
 // kv_tree_tc.cu — kv_cache_attend_tree when many query rows share a key head (wide trees, grouped heads, chunks of a
-// prompt): the same result as kv_tree.cu on tcgen05, 128 query rows of a key head at a time, head dim <= 128.
+// prompt): the same result as kv_tree.cu on tcgen05, 64 or 128 query rows of a key head at a time, head dim <= 128.
 //     S = Q.K^T, O = P.V as three tf32 products each over hi/lo parts; the value as it lies is the hi operand (the tensor
 //     core reads its tf32 part), the remainder rounded to tf32 the lo operand.
 // The work line of kv_tree_line.cuh, cut into one stretch per CTA, replaces the grid over query tiles; key blocks of 128
@@ -74,9 +74,9 @@ __device__ __forceinline__ uint32_t lo_bits(uint32_t x)
     return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u)) + 0x1000u;
 }
 
-// The three products of a block's scores / outputs, issued by one thread: four steps of eight at a time, in loops — the kernel's
-// roles share the SM's instruction cache, and unrolled whole (for either buffer of K and V) this code alone kept it turning over:
-// the softmax warps then waited for their instructions (5.9 against 4.4 thousand cycles a block).
+// The three products of a block's scores / outputs, issued by one thread: four steps of eight at a time, in loops.  Unrolled whole
+// the thread takes 55 cycles a product instead of 70 to 100, but the kernel's roles share the SM's instruction cache, and the call
+// took 129 us instead of 120 (64 rows of 128), 73 instead of 72 (256 rows of 64); with a copy for each of six buffer turns 177.
 template <int NSLAB, bool FEW>
 __device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, uint32_t it, uint32_t idesc, uint32_t klo_empty)
 {
