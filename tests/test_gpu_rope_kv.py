@@ -561,6 +561,81 @@ def test_other_stream_own_workspace_and_graphs(engine):
     assert torch.equal(eager, want[0]) and all(torch.equal(x, y) for x, y in zip(outs, want))
 
 
+def test_captured_steps(engine):
+    """A serving step (extend, attend, compact) and a training pass (forward, backward with the norms' gradients), each captured
+    on a stream of its own and replayed, give the bits of the eager calls; the gradients of norm weights add up over replays."""
+    g = gen(95)
+    B, T, H, Hkv, dk, max_seq = 3, 6, 8, 2, 128, 400
+    lens, n_new, keep, n_keep = ints([5, 300, 64]), ints([6, 2, 4]), ints([[0, 2, 5, 0, 0, 0], [1, 0, 0, 0, 0, 0], [0, 1, 3, 0, 0, 0]]), ints([3, 1, 3])
+    mask = tree_masks(np.random.RandomState(95), B, T)
+    freq = torch.tensor(ref.frequencies(dk), dtype=torch.float64, device="cuda")
+    gq, gk, bias = randn(g, dk), randn(g, dk), randn(g, (H + 2 * Hkv) * dk)
+    qkv, K0, V0 = randn(g, B * T, (H + 2 * Hkv) * dk), randn(g, B * Hkv, max_seq, dk), randn(g, B * Hkv, max_seq, dk)
+    grads = [randn(g, B * h, T, dk) for h in (H, Hkv, Hkv)]
+
+    def serve(K, V, Q, out, lens_out):
+        engine.kv_cache_extend(qkv, Q, K, V, lens, n_new=n_new, bias=bias, gq=gq, gk=gk, freq=freq)
+        engine.kv_cache_attend_tree(K, V, Q, out, lens, dk ** -0.5, n_new=n_new, mask=mask)
+        engine.kv_cache_compact(K, V, keep, n_keep, lens, lens_out)
+
+    def train(Q, K, V, dqkv, dgq, dgk):
+        engine.qkv_norm_rope(qkv, Q, K, V, B, bias=bias, gq=gq, gk=gk, freq=freq, pairing="interleaved")
+        engine.qkv_norm_rope_bwd(*grads, dqkv, B, qkv=qkv, bias=bias, gq=gq, gk=gk, freq=freq, pairing="interleaved", dgq=dgq, dgk=dgk)
+
+    z = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    state = lambda: [K0.clone(), V0.clone(), z(B * H, T, dk), z(B * H, T, dk), ints([0] * B)]  # noqa: E731
+    outputs = lambda: [*(z(B * h, T, dk) for h in (H, Hkv, Hkv)), torch.zeros_like(qkv), z(dk), z(dk)]  # noqa: E731
+    for step, make in ((serve, state), (train, outputs)):
+        want, got = make(), make()
+        step(*want)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=torch.cuda.Stream()):
+            engine.set_stream(torch.cuda.current_stream().cuda_stream)
+            try:
+                step(*got)
+            finally:
+                engine.set_stream(0)
+        for x, y in zip(got, make()):
+            x.copy_(y)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        if step is train:
+            gr.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(got[4:], want[4:]):                # the second sum starts from the first: two roundings
+                assert float((x - 2 * y).abs().max()) <= 2 * 2.0 ** -23 * float(y.abs().max())
+        del gr
+    assert engine.device_error() == 0
+
+
+def test_more_than_32_bits_of_elements(engine):
+    """Queries, keys and values of 2^31 elements and more: the last tokens' rows have the bits of a call of their own."""
+    S, H, Hkv, dk = 840016, 16, 2, 128
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 27 GB")
+    W, last = (H + 2 * Hkv) * dk, 5
+    assert S * W > 1 << 31
+    freq = torch.tensor(ref.frequencies(dk), dtype=torch.float64, device="cuda")
+    g = gen(97)
+    gq, gk = randn(g, dk), randn(g, dk)
+    qkv = torch.empty(S, W, device="cuda").fill_(0.5)
+    qkv[-last:] = randn(g, last, W)
+    big = [torch.empty(h, S, dk, device="cuda") for h in (H, Hkv, Hkv)]
+    engine.qkv_norm_rope(qkv, *big, 1, gq=gq, gk=gk, freq=freq)
+    small = [torch.empty(h, last, dk, device="cuda") for h in (H, Hkv, Hkv)]
+    pos = ints(range(S - last, S))
+    engine.qkv_norm_rope(qkv[-last:].contiguous(), *small, 1, gq=gq, gk=gk, freq=freq, pos=pos)
+    assert all(torch.equal(x[:, -last:], y) for x, y in zip(big, small))
+    dqkv, few = torch.empty(S, W, device="cuda"), torch.empty(last, W, device="cuda")
+    engine.qkv_norm_rope_bwd(*big, dqkv, 1, qkv=qkv, gq=gq, gk=gk, freq=freq)
+    engine.qkv_norm_rope_bwd(*small, few, 1, qkv=qkv[-last:].contiguous(), gq=gq, gk=gk, freq=freq, pos=pos)
+    assert torch.equal(dqkv[-last:], few)
+    del qkv, big, dqkv
+    torch.cuda.empty_cache()
+
+
 def test_cache_beyond_32_bit_offsets(engine):
     """Head 2 of a cache of 2^23 rows starts 2^31 elements (8 GiB) in; rows at both ends of it."""
     Hkv, dk, max_seq, T = 3, 128, (1 << 23) + 64, 4
@@ -582,6 +657,12 @@ def test_cache_beyond_32_bit_offsets(engine):
         assert torch.equal(K[:, L:L + 2], flat[1][:, [1, 3]]) and torch.equal(V[:, L:L + 2], flat[2][:, [1, 3]])
         assert torch.equal(K[:, L + 2:L + T], flat[1][:, 2:])
         if L == 200:
+            wide = randn(g, 10 * Hkv, T, dk)      # 40 rows to a key head: the tensor-memory kernel
+            got = torch.empty_like(wide)
+            engine.kv_cache_attend_tree(K, V, wide, got, ints([L]), 0.1)
+            short = [x[:, :L + T].contiguous() for x in (K, V)]
+            want, smag, vmag = ref.attend_tree(*short, wide, got, ints([L]), 0.1)
+            assert float((got.double() - want).abs().max()) < ref.attend_bound(smag, vmag, dk)
             out = torch.empty_like(Q)
             engine.kv_cache_attend_tree(K, V, Q, out, ints([L]), 0.1)
             short = [x[:, :L + T].contiguous() for x in (K, V)]
