@@ -40,7 +40,7 @@ ROPE = [
     (1, 1, 1, 1, 64, 64, "half", (1, 1), True, "none"),
     (2, 37, 4, 2, 64, 64, "half", (0, 0), False, "none"),
     (2, 37, 4, 2, 64, 64, "interleaved", (1, 1), True, "far"),
-    (1, 130, 8, 8, 128, 128, "half", (1, 0), False, "far"),
+    (1, 130, 8, 4, 128, 128, "half", (1, 0), False, "far"),
     (3, 19, 6, 1, 80, 32, "interleaved", (0, 1), True, "none"),
     (1, 7, 5, 5, 96, 48, "half", (1, 1), False, "negative"),
     (2, 11, 3, 3, 50, 50, "half", (1, 1), True, "far"),
