@@ -28,6 +28,8 @@ using namespace axb;
 
 namespace {
 
+constexpr size_t kAttnCounters = 4096;   // bytes at the head of an attention workspace
+
 struct Engine {
     bool ready = false;
     int device = 0;
@@ -499,6 +501,8 @@ extern "C" int axb_device_error(void)
     if (cudaMemcpy(&v, cur().err_word, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
     if (v) {
         cudaMemset(cur().err_word, 0, sizeof(int));
+        // a kernel that gave up may have left counters behind
+        if (v != AXB_DEVERR_ROWS && v != AXB_DEVERR_KEEP && cur().attn_ws) cudaMemset(cur().attn_ws, 0, kAttnCounters);
         if (v == AXB_DEVERR_ROWS) fail(AXB_ERR_INVALID_SHAPE, "a sequence's length and new tokens do not fit its cache rows (code %d)", v);
         else if (v == AXB_DEVERR_KEEP) fail(AXB_ERR_INVALID_SHAPE, "an accepted-token list is not ascending indices of the drafted rows (code %d)", v);
         else fail(AXB_ERR_BACKEND, "a kernel gave up on a bounded wait (code %d)", v);
@@ -1408,10 +1412,9 @@ inline bool overlaps(const void *p, int64_t n, const void *q, int64_t m)   // n,
     return p && q && a < b + (size_t)m * sizeof(float) && b < a + (size_t)n * sizeof(float);
 }
 
-// counters first (zero between calls), then room for either call's partial results
-constexpr size_t kAttnCounters = 4096;
-static_assert(sizeof(int) * 3 * 256 <= kAttnCounters && sizeof(KvTreeShared) * 256 <= KT_SHARED_BYTES, "per SM: three counters, a shared item");
+static_assert(sizeof(int) * 256 <= kAttnCounters && sizeof(KvTreeShared) * 256 <= KT_SHARED_BYTES, "per SM: a counter, a shared item");
 
+// counters first (zero between calls), then room for either call's partial results
 size_t attn_workspace_bytes()
 {
     const size_t tree = kv_tree_workspace_bytes(cur().sm_count), bwd = qkv_norm_rope_bwd_bytes(cur().sm_count);

@@ -1,4 +1,4 @@
-// kv_tree.cuh — launchers of the ragged-batch KV-cache kernels (kv_tree.cu): attention of T new tokens of every sequence
+// kv_tree.cuh — launchers of the ragged-batch KV-cache kernels (kv_tree.cu, kv_tree_tc.cu): attention of T new tokens of every sequence
 // over its cached rows and over one another (a chain or a drafted tree), and the move of accepted rows.
 #pragma once
 #include <cuda_runtime.h>
@@ -18,7 +18,7 @@ struct KvTreeArgs {
     const uint64_t *mask;        // [B or 1][T][words] bit j of token t: t attends to new token j; nullptr: j <= t
     const int32_t *lens, *n_new; // [B]; n_new nullptr: T for every sequence
     float *out;                  // [B*H, T, dk]
-    int *counters;               // three per SM, zero on entry and on exit
+    int *counters;               // one per SM, zero on entry and on exit (the warp-level kernel's)
     KvTreeShared *shared;        // kv_tree_workspace_bytes(): one per SM, then
     float *slots;                // partial results, two slots per SM
     int64_t max_seq, mask_stride;
