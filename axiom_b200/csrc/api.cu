@@ -1543,6 +1543,8 @@ extern "C" int axb_qkv_norm_rope_bwd(const float *qkv, const float *bqkv, const 
     const int64_t nq = B * S * H * dk, nk = B * S * Hkv * dk, n = nq + 2 * nk;
     if (overlaps(dqkv, n, dQh, nq) || overlaps(dqkv, n, dKh, nk) || overlaps(dqkv, n, dVh, nk) || ((gq || gk) && overlaps(dqkv, n, qkv, n)))
         return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope_bwd: dqkv overlaps an input");
+    if (overlaps(dqkv, n, dgq, dk) || overlaps(dqkv, n, dgk, dk) || (dgq != dgk && overlaps(dgq, dk, dgk, dk)))
+        return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope_bwd: two outputs overlap");
     if ((st = ensure_ready())) return st;
     OnDevice on;
     a.q = const_cast<float *>(dQh); a.k = const_cast<float *>(dKh); a.v = const_cast<float *>(dVh);

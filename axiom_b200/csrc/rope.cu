@@ -502,19 +502,25 @@ __global__ void __launch_bounds__(RP_THREADS, RP_BWD_CTAS) qkv_norm_rope_bwd_ker
     }
 }
 
-// dg[w][d] += sum over blocks of partial[block][w][d], in 64 bits: 64 strands, each in block order, then in strand order
+// dg[w][d] += sum over blocks of partial[block][w][d], in 64 bits: 64 strands, each in block order, then in strand order.
+// dgq == dgk (one weight for queries and keys): its element is one thread's, which adds both sums.
 __global__ void __launch_bounds__(512) rope_dgamma_kernel(const float *partial, int blocks, int dk, float *dgq, float *dgk)
 {
     __shared__ double red[64][9];
-    const int x = threadIdx.x & 7, c = blockIdx.x * 8 + x, strand = threadIdx.x >> 3;
+    const bool tied = dgq == dgk;
+    const int x = threadIdx.x & 7, c = blockIdx.x * 8 + x, strand = threadIdx.x >> 3, columns = tied ? dk : 2 * dk;
     double s = 0.0;
-    if (c < 2 * dk) {
+    if (c < columns) {
 #pragma unroll 8
         for (int b = strand; b < blocks; b += 64) s += (double)partial[(int64_t)b * 2 * dk + c];
+        if (tied) {
+#pragma unroll 8
+            for (int b = strand; b < blocks; b += 64) s += (double)partial[((int64_t)b * 2 + 1) * dk + c];
+        }
     }
     red[strand][x] = s;
     __syncthreads();
-    if (strand == 0 && c < 2 * dk) {
+    if (strand == 0 && c < columns) {
         for (int k = 1; k < 64; ++k) s += red[k][x];
         float *dst = c < dk ? dgq : dgk;
         const int d = c < dk ? c : c - dk;
@@ -594,7 +600,7 @@ int launch_qkv_norm_rope_bwd(const RopeArgs &a, float *dgq, float *dgk, int sm_c
     *launches = 1;
     int e = (int)cudaGetLastError();
     if (e || !a.partial) return e;
-    rope_dgamma_kernel<<<(2 * a.dk + 7) / 8, 512, 0, st>>>(a.partial, grid, a.dk, dgq, dgk);
+    rope_dgamma_kernel<<<((dgq == dgk ? 1 : 2) * a.dk + 7) / 8, 512, 0, st>>>(a.partial, grid, a.dk, dgq, dgk);
     *launches = 2;
     return (int)cudaGetLastError();
 }

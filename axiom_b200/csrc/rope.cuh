@@ -27,7 +27,7 @@ struct RopeArgs {
 int launch_qkv_norm_rope(const RopeArgs &a, int sm_count, cudaStream_t st);
 // the most that the backward's partial sums take, whatever the shape
 size_t qkv_norm_rope_bwd_bytes(int sm_count);
-// dgq / dgk [dk] are added to (nullptr: not wanted); *launches receives the number of kernels enqueued
+// dgq / dgk [dk] are added to (nullptr: not wanted; the same buffer twice: it receives both); *launches receives the number of kernels enqueued
 int launch_qkv_norm_rope_bwd(const RopeArgs &a, float *dgq, float *dgk, int sm_count, cudaStream_t st, int *launches);
 
 }  // namespace axb

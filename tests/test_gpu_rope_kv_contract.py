@@ -1,0 +1,33 @@
+"""What the rotary / ragged-batch KV-cache calls promise beside their results, on the GPU: buffers that are one, error codes,
+workspaces, accuracy where a lost tile or term would show.
+
+Tolerances are bounds, stated beside their use (u = 2^-24, half a step of fp32)."""
+import pytest
+import torch
+
+import rope_kv_ref as ref
+from test_gpu_rope_kv import U, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("B,S,H,Hkv,dk", [(1, 3, 2, 1, 2), (1, 50, 4, 2, 4), (2, 300, 8, 2, 64), (4, 700, 16, 8, 128), (1, 5, 2, 2, 33)])
+def test_one_gradient_buffer_for_both_norm_weights(engine, B, S, H, Hkv, dk):
+    """gq is gk and dgq is dgk (one weight for queries and keys): the buffer receives both sums, every time the same bits."""
+    g = gen(dk)
+    qkv, w, start = randn(g, B * S, (H + 2 * Hkv) * dk), 1 + 0.2 * randn(g, dk), randn(g, dk)
+    grads = [randn(g, B * h, S, dk) for h in (H, Hkv, Hkv)]
+    freq = torch.tensor(ref.frequencies(dk // 2 * 2), dtype=torch.float64).cuda()
+    how = dict(qkv=qkv, gq=w, gk=w, freq=freq)
+    dqkv, alone = torch.empty_like(qkv), [torch.zeros(dk, device="cuda") for _ in range(2)]
+    engine.qkv_norm_rope_bwd(*grads, dqkv, B, dgq=alone[0], dgk=alone[1], **how)
+    first = None
+    for _ in range(20):
+        both, again = start.clone(), torch.empty_like(qkv)
+        engine.qkv_norm_rope_bwd(*grads, again, B, dgq=both, dgk=both, **how)
+        first = both if first is None else first
+        assert torch.equal(both, first) and torch.equal(again, dqkv)
+    # the sums over CTAs are 64-bit: each of the two alone is rounded once, and so is the result
+    want = start.double() + alone[0].double() + alone[1].double()
+    room = U * (alone[0].abs() + alone[1].abs() + first.abs()).double() * 1.001
+    assert bool(((first.double() - want).abs() <= room).all())
