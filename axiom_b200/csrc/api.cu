@@ -501,8 +501,6 @@ extern "C" int axb_device_error(void)
     if (cudaMemcpy(&v, cur().err_word, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
     if (v) {
         cudaMemset(cur().err_word, 0, sizeof(int));
-        // a kernel that gave up may have left counters behind
-        if (v != AXB_DEVERR_ROWS && v != AXB_DEVERR_KEEP && cur().attn_ws) cudaMemset(cur().attn_ws, 0, kAttnCounters);
         if (v == AXB_DEVERR_ROWS) fail(AXB_ERR_INVALID_SHAPE, "a sequence's length and new tokens do not fit its cache rows (code %d)", v);
         else if (v == AXB_DEVERR_KEEP) fail(AXB_ERR_INVALID_SHAPE, "an accepted-token list is not ascending indices of the drafted rows (code %d)", v);
         else fail(AXB_ERR_BACKEND, "a kernel gave up on a bounded wait (code %d)", v);

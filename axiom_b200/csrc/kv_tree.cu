@@ -514,11 +514,12 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
         if (C::ASYNC && warp == KT_CONSUMERS + 3) {
             // ---- merger
             float4 *const parts = area + 2 * (C::Q_BYTES / 16) + lane;
-            for (uint32_t k = 0;; ++k) {
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(piece_full + 8 * (k & 1), (k / 2) & 1))) return;
+            uint32_t k = 0;
+            for (;; ++k) {
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(piece_full + 8 * (k & 1), (k / 2) & 1))) break;
                 p = s_piece[k & 1];
                 if (p.count == 0) return;
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(merge_full, k & 1))) return;
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(merge_full, k & 1))) break;
                 clear();
 #pragma unroll 1
                 for (int i = 0; i < KT_CONSUMERS; ++i) tree_add<DKP, NR>(w, parts + i * (C::PART_BYTES / 16), parts + i * (C::PART_BYTES / 16) + C::FRAGS * 32, 32);
@@ -529,13 +530,12 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
                 }
                 bool write = p.pieces == 1;
                 if (!write) {
-                    // the item's first CTA names its counter
                     float4 *f = slot(tree_slot(blockIdx.x, p.t0 == 0));
                     tree_put<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
                     __threadfence();
                     __syncwarp();
                     int last = 0;
-                    if (lane == 0) last = atomicAdd(a.counters + p.first, 1) == p.pieces - 1;
+                    if (lane == 0) last = tree_arrive(a, p);
                     write = __shfl_sync(0xffffffffu, last, 0) != 0;
                     if (write) {
                         __threadfence();
@@ -545,11 +545,13 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
                             const float4 *s = slot(tree_slot(p.first + i, i == 0));
                             tree_add<DKP, NR>(w, s, s + C::FRAGS * 32, 32);
                         }
-                        if (lane == 0) a.counters[p.first] = 0;
+                        if (lane == 0) tree_clear(a, p);
                     }
                 }
                 if (write) write_out(p);
             }
+            if (lane == 0) tree_leave(a, line, cur, k);
+            return;
         }
         const int v = warp - KT_CONSUMERS;
         const float *const cache = v ? a.V : a.K;
@@ -614,7 +616,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
             }
         }
     } else {
-        while (next_piece(a, line, cur, p)) {
+        while (next_piece(a, line, cur, p)) {   // (to the end also after a wait that ran out: the items' counters need every arrival)
             stage_q(p, area, s_toks[0], tid, KT_CONSUMERS * 32);
             clear();
             consumers_sync();
@@ -629,7 +631,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
                     __threadfence();
                 }
                 consumers_sync();
-                if (tid == 0) s_last = atomicAdd(a.counters + p.first, 1) == p.pieces - 1;
+                if (tid == 0) s_last = tree_arrive(a, p);
                 consumers_sync();
                 write = s_last != 0;
                 if (write) {
@@ -641,7 +643,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
                         tree_add<DKP, NR>(w, f, f + C::FRAGS * 32, 32);
                     }
                     tree_merge<DKP, NR>(w, area, warp);
-                    if (tid == 0) a.counters[p.first] = 0;
+                    if (tid == 0) tree_clear(a, p);
                 }
             }
             if (write && warp == 0) write_out(p);

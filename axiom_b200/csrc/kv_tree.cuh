@@ -18,7 +18,7 @@ struct KvTreeArgs {
     const uint64_t *mask;        // [B or 1][T][words] bit j of token t: t attends to new token j; nullptr: j <= t
     const int32_t *lens, *n_new; // [B]; n_new nullptr: T for every sequence
     float *out;                  // [B*H, T, dk]
-    int *counters;               // one per SM, zero on entry and on exit (the warp-level kernel's)
+    int *counters;               // one per SM, zero on entry and on exit, of a launch that gave up too (the warp-level kernel's)
     KvTreeShared *shared;        // kv_tree_workspace_bytes(): one per SM, then
     float *slots;                // partial results, two slots per SM
     int64_t max_seq, mask_stride;

@@ -144,6 +144,25 @@ __device__ __forceinline__ bool next_piece(const KvTreeArgs &a, const TreeLine &
 // last): two workspace slots a CTA are enough.
 __device__ __forceinline__ int tree_slot(int cta, bool begins) { return 2 * cta + (begins ? 1 : 0); }
 
+// A CTA is done with its piece of a shared item (one thread; what it leaves in its slot is visible by now).  True for the last of
+// the item's CTAs, which adds the pieces and clears the counter for the next call.  The item's first CTA names the counter.
+__device__ __forceinline__ bool tree_arrive(const KvTreeArgs &a, const TreePiece &p)
+{
+    return atomicAdd(a.counters + p.first, 1) == p.pieces - 1;
+}
+
+// (behind the sum: a store before it is one more thing that the fence in front of the slots' loads waits for, 0.3 us)
+__device__ __forceinline__ void tree_clear(const KvTreeArgs &a, const TreePiece &p) { a.counters[p.first] = 0; }
+
+// One thread of a CTA that gave up before its piece number `done`, c as tree_start left it: it arrives for the rest all the same,
+// so that every launch leaves the counters at zero, whatever became of its results.
+__device__ __forceinline__ void tree_leave(const KvTreeArgs &a, const TreeLine &ln, TreeCursor c, uint32_t done)
+{
+    TreePiece p;
+    for (uint32_t k = 0; next_piece(a, ln, c, p); ++k)
+        if (k >= done && p.pieces > 1 && tree_arrive(a, p)) tree_clear(a, p);
+}
+
 // whether token t sees new token j
 __device__ __forceinline__ bool tree_sees(const KvTreeArgs &a, int b, int t, int j)
 {

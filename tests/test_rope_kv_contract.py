@@ -1,6 +1,12 @@
-"""What the rotary / ragged-batch KV-cache calls promise beside their results, without a GPU: refusals of buffers that meet."""
+"""What the rotary / ragged-batch KV-cache calls promise beside their results, without a GPU: refusals of buffers that meet, counters
+that every launch leaves at zero."""
+import ctypes as C
+import os
+import subprocess
+
 import pytest
 
+from conftest import ROOT
 from test_rope_kv_host import INVALID_SHAPE, P, bwd_call, eng  # noqa: F401
 
 
@@ -18,3 +24,27 @@ def test_norm_gradients_side_by_side_or_in_one_buffer_are_not(eng, override):  #
         pytest.skip("needs a machine without a GPU")
     assert eng.lib.axb_qkv_norm_rope_bwd(*bwd_call(**override)) != INVALID_SHAPE
     assert "no CUDA device" in eng.last_error()
+
+
+@pytest.fixture(scope="module")
+def line(tmp_path_factory):
+    here, root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "kv_tree_line_host"), ROOT
+    so = str(tmp_path_factory.mktemp("line") / "line.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-w", "-shared", "-fPIC", "-I", here, "-I", os.path.join(root, "axiom_b200", "csrc"), "-I",
+                    os.path.join(root, "include"), os.path.join(here, "line.cpp"), "-o", so], check=True)
+    return C.CDLL(so)
+
+
+# block_rows, tile_keys, min_stretch, gap: the warp-level kernel's lines
+@pytest.mark.parametrize("how", [(8, 32, 4, 5), (16, 32, 4, 5), (32, 32, 4, 8)])
+@pytest.mark.parametrize("give_up", [0, 3, 50, 100])
+def test_the_work_line_and_its_counters(line, how, give_up):
+    """The kernels' own division of a batch: every tile once, at most two shared pieces a CTA, and counters at zero after a launch
+    in which CTAs gave up at any of their pieces (a counter left behind would make a later call add up pieces too early)."""
+    left, would_stay = C.c_int(), 0
+    for seed in range(60):
+        B, T, per, Hkv, max_seq, ctas = [(1, 1, 4, 1, 3000, 148), (3, 7, 2, 2, 900, 148), (40, 3, 4, 3, 700, 148), (9, 16, 1, 2, 5000, 148),
+                                         (2, 40, 3, 1, 333, 20), (300, 2, 4, 1, 90, 148)][seed % 6]
+        assert line.line_check(1000 * give_up + seed, B, T, per, Hkv, max_seq, *how, ctas, give_up, C.byref(left)) == 0, seed
+        would_stay += left.value
+    assert (would_stay > 0) == (give_up > 0)      # without the arrivals of those that gave up, counters would stay behind
