@@ -4,6 +4,7 @@
 // kernel cannot run the call fails with a status and a message.
 #include "../../include/axiom_b200.h"
 
+#include "device_error.cuh"
 #include "elementwise.cuh"
 #include "errors.cuh"
 #include "gemm_tc.cuh"
@@ -47,7 +48,7 @@ struct Engine {
     size_t sk_partial_floats = 0;
     int *sk_counters = nullptr;
     int sk_counter_cap = 0;
-    int *err_word = nullptr;
+    int *err_word = nullptr;        // ERR_WORDS of them; the kernels that refuse nothing know the first alone
     int *gemm_counters = nullptr;   // split-K arrival counters of the tensor-core GEMM (zero between launches)
     // output range of the last skinny kernel, which lets the next one start under it: a skinny call whose WEIGHTS lie
     // in that range must not prefetch them early
@@ -375,8 +376,8 @@ extern "C" int axb_init(int device)
         return fail(AXB_ERR_BACKEND, "device %d is sm_%d%d; this engine holds sm_100a code only", device, prop.major, prop.minor);
     en.device = device;
     en.sm_count = prop.multiProcessorCount;
-    if ((e = cudaMalloc(&en.err_word, sizeof(int))) != cudaSuccess) return cuda_fail("cudaMalloc", e);
-    cudaMemset(en.err_word, 0, sizeof(int));
+    if ((e = cudaMalloc(&en.err_word, ERR_WORDS * sizeof(int))) != cudaSuccess) return cuda_fail("cudaMalloc", e);
+    cudaMemset(en.err_word, 0, ERR_WORDS * sizeof(int));
     if ((e = cudaMalloc(&en.gemm_counters, kSplitCounters * sizeof(int))) != cudaSuccess) return cuda_fail("cudaMalloc", e);
     cudaMemset(en.gemm_counters, 0, kSplitCounters * sizeof(int));
     const char *mode = getenv("AX_B200_FP32_MODE");
@@ -497,10 +498,12 @@ extern "C" const char *axb_last_error(void) { return cur().msg; }
 extern "C" int axb_device_error(void)
 {
     if (!cur().ready || !cur().err_word) return 0;
-    int v = 0;
-    if (cudaMemcpy(&v, cur().err_word, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
-    if (v) {
-        cudaMemset(cur().err_word, 0, sizeof(int));
+    int words[ERR_WORDS] = {}, v = 0;
+    if (cudaMemcpy(words, cur().err_word, sizeof words, cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
+    const int which = next_device_error(words);
+    if (which >= 0) {
+        v = words[which];
+        cudaMemset(cur().err_word + which, 0, sizeof(int));
         if (v == AXB_DEVERR_ROWS) fail(AXB_ERR_INVALID_SHAPE, "a sequence's length and new tokens do not fit its cache rows (code %d)", v);
         else if (v == AXB_DEVERR_KEEP) fail(AXB_ERR_INVALID_SHAPE, "an accepted-token list is not ascending indices of the drafted rows (code %d)", v);
         else fail(AXB_ERR_BACKEND, "a kernel gave up on a bounded wait (code %d)", v);

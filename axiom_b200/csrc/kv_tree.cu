@@ -590,7 +590,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
             }
         }
         if (!ok) {
-            if (lane == 0 && a.err) atomicCAS(a.err, 0, (int)TERR_PRODUCER);
+            if (lane == 0 && a.err) atomicCAS(a.err + ERR_GAVE_UP, 0, (int)TERR_PRODUCER);
             // copies in flight land before the CTA's memory goes away
             for (uint32_t i = it > C::STAGES ? it - C::STAGES : 0; i < it; ++i) mbar_wait_bounded(full_bar(v, i % C::STAGES), (i / C::STAGES) & 1);
         }
@@ -650,7 +650,7 @@ kv_tree_kernel(const __grid_constant__ KvTreeArgs a, const __grid_constant__ Tre
             consumers_sync();   // the merge area and the tokens are free again
         }
     }
-    if (!ok && lane == 0 && a.err) atomicCAS(a.err, 0, (int)TERR_CONSUMER);
+    if (!ok && lane == 0 && a.err) atomicCAS(a.err + ERR_GAVE_UP, 0, (int)TERR_CONSUMER);
 }
 
 template <int VEC>
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(256) kv_compact_kernel(float *K, float *V, con
         }
     bad = __syncthreads_or(bad);
     if (blockIdx.y == 0 && threadIdx.x == 0) {
-        if (bad && err) atomicCAS(err, 0, (int)AXB_DEVERR_KEEP);
+        if (bad && err) atomicCAS(err + ERR_KEEP, 0, (int)AXB_DEVERR_KEEP);
         if (lens_out) lens_out[b] = bad ? len : len + n;
     }
     if (bad) return;   // refused whole

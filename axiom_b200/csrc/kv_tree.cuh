@@ -22,7 +22,7 @@ struct KvTreeArgs {
     KvTreeShared *shared;        // kv_tree_workspace_bytes(): one per SM, then
     float *slots;                // partial results, two slots per SM
     int64_t max_seq, mask_stride;
-    int *err;
+    int *err;                    // the words of device_error.cuh
     float c_log2;                // scale * log2(e)
     int B, H, Hkv, T, dk, words;
 };

@@ -3,6 +3,7 @@
 // CTAs that share an item are consecutive and each holds a tile of it.
 #pragma once
 #include "../../include/axiom_b200.h"
+#include "device_error.cuh"
 #include "kv_tree.cuh"
 
 namespace axb {
@@ -59,7 +60,7 @@ __device__ __forceinline__ bool tree_start(const KvTreeArgs &a, const TreeLine &
         if (b >= a.B) return 0;
         bool bad;
         const TreeSeq s = tree_seq(a, ln, b, &bad);
-        if (bad && blockIdx.x == 0 && a.err) atomicCAS(a.err, 0, (int)AXB_DEVERR_ROWS);
+        if (bad && blockIdx.x == 0 && a.err) atomicCAS(a.err + ERR_ROWS, 0, (int)AXB_DEVERR_ROWS);
         return tree_tiles(a, s);
     };
     int mine = 0;

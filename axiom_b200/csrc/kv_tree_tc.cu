@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     float (*s_max)[2][ROWS] = reinterpret_cast<float (*)[2][ROWS]>(sm + 1024);   // [block parity][half][row]
     if (threadIdx.x == 0) a.shared[blockIdx.x] = KvTreeShared{ 0, 0, 0, 0, 0, 0 };   // (this thread replaces it where the CTA begins a shared item)
     if (base & 1023) {   // the swizzles are functions of the address (it starts at a multiple of 1 KB; refused, should it ever not)
-        if (threadIdx.x == 0 && a.err) atomicCAS(a.err, 0, (int)CERR_LOAD);
+        if (threadIdx.x == 0 && a.err) atomicCAS(a.err + ERR_GAVE_UP, 0, (int)CERR_LOAD);
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
     };
     auto give_up = [&](int code) {
         s_gave_up = 1;
-        if (a.err) atomicCAS(a.err, 0, code);
+        if (a.err) atomicCAS(a.err + ERR_GAVE_UP, 0, code);
     };
     TreePiece p;
     uint32_t it = 0;      // key blocks since the start

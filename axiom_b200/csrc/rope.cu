@@ -26,6 +26,8 @@
 // place of the pieces.
 #include "rope.cuh"
 
+#include "device_error.cuh"
+
 #include <math.h>
 
 namespace axb {
@@ -171,7 +173,7 @@ __device__ __forceinline__ RopeToken rope_token(const RopeArgs &a, int tok)
         const int len = a.lens[t.b], n = a.n_new ? a.n_new[t.b] : a.T;
         // a sequence that does not fit its rows is refused whole: nothing of it is read or written
         const bool bad = len < 0 || n < 0 || n > a.T || (int64_t)len + n > a.kv_rows;
-        if (bad && a.err && (threadIdx.x & 31) == 0) atomicCAS(a.err, 0, (int)AXB_DEVERR_ROWS);
+        if (bad && a.err && (threadIdx.x & 31) == 0) atomicCAS(a.err + ERR_ROWS, 0, (int)AXB_DEVERR_ROWS);
         valid = !bad && t.s < n;
         if (valid) t.kv += len;
     }

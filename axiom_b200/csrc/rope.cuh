@@ -19,7 +19,7 @@ struct RopeArgs {
     float *dqkv;                 // backward: the gradient of qkv
     float *partial;              // backward, qkv_norm_rope_bwd_bytes(): [grid][2*dk] partial sums of the norm weights' gradients
     int64_t kv_rows;             // T, or the rows of a cache
-    int *err;
+    int *err;                    // the words of device_error.cuh
     float eps, amplitude;
     int B, T, H, Hkv, dk, pairs, interleaved;
 };

@@ -77,7 +77,8 @@ AXB_API int axb_set_fp32_mode(int mode);        /* AXB_FP32_* */
 AXB_API int axb_get_fp32_mode(void);
 AXB_API const char *axb_last_error(void);
 /* Non-zero when a kernel gave up on a bounded wait (its code) or refused values that only the device sees
-   (AXB_DEVERR_*); reading clears it. */
+   (AXB_DEVERR_*).  One report a call, a kernel that gave up first; reading clears what was reported, the next call reports
+   the next. */
 AXB_API int axb_device_error(void);
 /* Kernels enqueued by this library since the counter was last reset. */
 AXB_API int64_t axb_launch_count(int reset);

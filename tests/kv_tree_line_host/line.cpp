@@ -7,6 +7,14 @@
 
 using namespace axb;
 
+extern "C" int next_error(const int *words, int count)
+{
+    if (count != ERR_WORDS) return -2;
+    int w[ERR_WORDS];
+    std::copy(words, words + count, w);
+    return next_device_error(w);
+}
+
 // what tree_start finds, by a plain walk
 static bool start(const KvTreeArgs &a, const TreeLine &ln, int cta, int ctas, TreeCursor &c)
 {

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import rope_kv_ref as ref
-from test_gpu_rope_kv import U, gen, randn
+from test_gpu_rope_kv import U, gen, ints, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +31,21 @@ def test_one_gradient_buffer_for_both_norm_weights(engine, B, S, H, Hkv, dk):
     want = start.double() + alone[0].double() + alone[1].double()
     room = U * (alone[0].abs() + alone[1].abs() + first.abs()).double() * 1.001
     assert bool(((first.double() - want).abs() <= room).all())
+
+
+def test_every_kind_of_refusal_is_reported(engine):
+    """Two calls that each refuse a sequence, one reading after the other: neither report hides the other."""
+    B, T, H, Hkv, dk, max_seq = 2, 3, 2, 1, 32, 16
+    g = gen(3)
+    K, V, Q = randn(g, B * Hkv, max_seq, dk), randn(g, B * Hkv, max_seq, dk), randn(g, B * H, T, dk)
+    qkv = randn(g, B * T, (H + 2 * Hkv) * dk)
+    assert engine.device_error() == 0
+    for rows_first in (True, False):
+        for rows in (rows_first, not rows_first):
+            if rows:
+                engine.kv_cache_extend(qkv, Q, K, V, ints([2, 15]))
+            else:
+                engine.kv_cache_compact(K, V, ints([[0, 1, 0], [1, 0, 0]]), ints([2, 2]), ints([2, 2]))
+        engine.synchronize()
+        assert [engine.device_error() for _ in range(3)] == [101, 102, 0]
+    assert "ascending" in engine.last_error()

@@ -48,3 +48,8 @@ def test_the_work_line_and_its_counters(line, how, give_up):
         assert line.line_check(1000 * give_up + seed, B, T, per, Hkv, max_seq, *how, ctas, give_up, C.byref(left)) == 0, seed
         would_stay += left.value
     assert (would_stay > 0) == (give_up > 0)      # without the arrivals of those that gave up, counters would stay behind
+
+
+def test_a_refusal_does_not_hide_a_kernel_that_gave_up(line):
+    for words, first in (([0, 0, 0], -1), ([94, 101, 102], 0), ([94, 0, 0], 0), ([0, 101, 102], 1), ([0, 0, 102], 2)):
+        assert line.next_error((C.c_int * 3)(*words), 3) == first
