@@ -63,27 +63,37 @@ _i64 = C.c_int64
 _f = C.c_float
 
 
-# The addresses of the buffers of the calls that run in a few microseconds on the device: written for the time it takes.
 _TYPE_NAME = {}   # element types met so far, by name ("torch.float32": the binding imports no torch)
 
 
-def _addr(t, dtype="float32"):
-    """t's address: a contiguous device tensor of the named element type, an address already, or None."""
-    if t is None:
-        return None
-    try:
-        if _TYPE_NAME[t.dtype] == dtype and t.is_cuda and t.is_contiguous():
-            return t.data_ptr()
-    except (AttributeError, KeyError):
-        if isinstance(t, int):
-            return t
-        _TYPE_NAME[t.dtype] = str(t.dtype)[6:]
-        return _addr(t, dtype)
-    if _TYPE_NAME[t.dtype] != dtype:
-        raise ValueError(f"a {dtype} tensor is wanted, got {t.dtype}")
-    if not t.is_contiguous():
-        raise ValueError(f"a contiguous tensor is wanted, got strides {tuple(t.stride())}")
-    raise ValueError(f"a tensor on the engine's device is wanted, got {t.device}")
+def _addresses(device):
+    """(addr, place) for an engine on this device (None: it was not told; its tensors' word is taken for it).  addr gives the address
+    of a buffer of the calls that run in a few microseconds on the device, and is written for the time it takes; place
+    refuses a tensor elsewhere."""
+    def place(t):
+        if not t.is_cuda or (device is not None and t.get_device() != device):
+            raise ValueError(f"a tensor on the engine's device is wanted, got {t.device}")
+
+    def addr(t, dtype="float32"):
+        """t's address: a contiguous tensor of the named element type on the engine's device, an address already, or None."""
+        if t is None:
+            return None
+        try:
+            if _TYPE_NAME[t.dtype] == dtype and t.get_device() == device and t.is_contiguous():
+                return t.data_ptr()
+        except (AttributeError, KeyError):
+            if isinstance(t, int):
+                return t
+            _TYPE_NAME[t.dtype] = str(t.dtype)[6:]
+            return addr(t, dtype)
+        if _TYPE_NAME[t.dtype] != dtype:
+            raise ValueError(f"a {dtype} tensor is wanted, got {t.dtype}")
+        place(t)
+        if not t.is_contiguous():
+            raise ValueError(f"a contiguous tensor is wanted, got strides {tuple(t.stride())}")
+        return t.data_ptr()
+
+    return addr, place
 
 
 class Engine:
@@ -95,6 +105,7 @@ class Engine:
                 f"{so_path} is missing: build it with `python -m axiom_b200.build` (no CPU fallback exists)")
         self.lib = C.CDLL(so_path)
         self.stream_ptr = 0          # the stream the engine enqueues on (0 = legacy default stream)
+        self._on(None)
         L = self.lib
         L.axb_last_error.restype = C.c_char_p
         L.axb_storage_alloc.restype = C.c_void_p
@@ -116,7 +127,7 @@ class Engine:
         L.axb_kv_cache_attend_tree.argtypes = [vp] * 4 + [C.c_int] + [vp] * 3 + [i64] * 6 + [C.c_float, vp]
         L.axb_kv_cache_compact.argtypes = [vp] * 6 + [i64] * 5
         if device is not None:
-            self._check(L.axb_init(int(device)))
+            self.init(device)
 
     # ---- plumbing ------------------------------------------------------
     def _check(self, status):
@@ -125,6 +136,11 @@ class Engine:
 
     def init(self, device=-1):
         self._check(self.lib.axb_init(int(device)))
+        if int(device) >= 0:
+            self._on(int(device))
+
+    def _on(self, device):
+        self._addr, self._place = _addresses(device)
 
     def synchronize(self):
         self.lib.axb_synchronize()
@@ -433,7 +449,7 @@ class Engine:
         raise ValueError(what)
 
     def _rope(self, rows, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos):
-        width, p = (H + 2 * Hkv) * dk, _addr
+        width, p = (H + 2 * Hkv) * dk, self._addr
         if qkv is not None and qkv.shape != (rows, width) and not qkv.shape[0] == rows == 0:
             self._wants(f"qkv: [{rows}, {width}] is wanted")
         if bias is not None and bias.numel() != width:
@@ -459,7 +475,7 @@ class Engine:
         H, Hkv, S, rows, dk = self._heads(B, Qh, Kh, Vh, "Qh, Kh, Vh")
         if rows != S:
             self._wants("Qh, Kh, Vh: head-major shapes")
-        p = _addr
+        p = self._addr
         self._check(self.lib.axb_qkv_norm_rope(*self._rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos),
                                                B, S, H, Hkv, dk, p(Qh), p(Kh), p(Vh)))
         return Qh, Kh, Vh
@@ -472,7 +488,7 @@ class Engine:
             self._wants("dQh, dKh, dVh: head-major shapes")
         if dqkv.shape != (B * S, (H + 2 * Hkv) * dk) or any(g is not None and g.numel() != dk for g in (dgq, dgk)):
             self._wants("dqkv, dgq, dgk: shapes")
-        p = _addr
+        p = self._addr
         self._check(self.lib.axb_qkv_norm_rope_bwd(*self._rope(B * S, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos),
                                                    p(dQh), p(dKh), p(dVh), B, S, H, Hkv, dk, p(dqkv), p(dgq), p(dgk),
                                                    self._workspace(workspace)))
@@ -487,6 +503,7 @@ class Engine:
     def _workspace(self, ws):
         if ws is None or isinstance(ws, int):
             return ws
+        self._place(ws)
         if not ws.is_contiguous() or ws.numel() * ws.element_size() < self.attention_workspace_bytes():
             self._wants("workspace: too small")
         return ws.data_ptr()
@@ -499,7 +516,7 @@ class Engine:
         H, Hkv, T, max_seq, dk = self._heads(B, Qh, K_cache, V_cache, "Qh, K_cache, V_cache")
         if n_new is not None and n_new.numel() != B:
             self._wants("n_new: one count for each sequence")
-        p = _addr
+        p = self._addr
         self._check(self.lib.axb_kv_cache_extend(*self._rope(B * T, H, Hkv, dk, qkv, bias, gq, gk, eps, freq, pairing, amplitude, pos),
                                                  p(lens, "int32"), p(n_new, "int32"), B, T, H, Hkv, max_seq, dk, p(Qh), p(K_cache),
                                                  p(V_cache)))
@@ -519,7 +536,7 @@ class Engine:
                 self._wants(f"mask: [{B}, {T}, {words}] or [{T}, {words}] is wanted")
         if n_new is not None and n_new.numel() != B:
             self._wants("n_new: one count for each sequence")
-        p = _addr
+        p = self._addr
         self._check(self.lib.axb_kv_cache_attend_tree(p(K_cache), p(V_cache), p(Q), p(mask, "int64"), each, p(lens, "int32"),
                                                       p(n_new, "int32"), p(out), B, H, Hkv, T, max_seq, dk, scale,
                                                       self._workspace(workspace)))
@@ -532,7 +549,7 @@ class Engine:
         if (B * Hkv != BHkv or K_cache.shape != V_cache.shape or keep.numel() != B * T or n_keep.numel() != B or
                 (lens_out is not None and lens_out.numel() != B)):
             self._wants("K_cache, V_cache, keep, n_keep, lens_out: shapes")
-        p = _addr
+        p = self._addr
         self._check(self.lib.axb_kv_cache_compact(p(K_cache), p(V_cache), p(keep, "int32"), p(n_keep, "int32"), p(lens, "int32"),
                                                   p(lens_out, "int32"), B, Hkv, T, max_seq, dk))
         return lens_out

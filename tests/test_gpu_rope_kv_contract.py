@@ -49,3 +49,14 @@ def test_every_kind_of_refusal_is_reported(engine):
         engine.synchronize()
         assert [engine.device_error() for _ in range(3)] == [101, 102, 0]
     assert "ascending" in engine.last_error()
+
+
+def test_binding_refuses_a_host_workspace(engine):
+    """Large enough, but its address means nothing to a kernel: refused before anything is launched."""
+    z = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    ws = torch.zeros(engine.attention_workspace_bytes(), dtype=torch.uint8)
+    before = engine.launch_count()
+    for w in (ws, ws.pin_memory()):
+        with pytest.raises(ValueError, match="engine's device"):
+            engine.kv_cache_attend_tree(z(2, 8, 16), z(2, 8, 16), z(2, 3, 16), z(2, 3, 16), ints([2]), 1.0, workspace=w)
+    assert engine.launch_count() == before

@@ -53,3 +53,46 @@ def test_the_work_line_and_its_counters(line, how, give_up):
 def test_a_refusal_does_not_hide_a_kernel_that_gave_up(line):
     for words, first in (([0, 0, 0], -1), ([94, 101, 102], 0), ([94, 0, 0], 0), ([0, 101, 102], 1), ([0, 0, 102], 2)):
         assert line.next_error((C.c_int * 3)(*words), 3) == first
+
+
+class OtherGpusTensor:
+    """What the binding asks of a tensor, of one that lies on GPU 1."""
+    is_cuda, device = True, "cuda:1"
+
+    def __init__(self, host):
+        self.host, self.dtype, self.shape = host, host.dtype, host.shape
+
+    def __getattr__(self, name):
+        return getattr(self.host, name)
+
+    def get_device(self):
+        return 1
+
+
+@pytest.fixture
+def eng_on_0():
+    from axiom_b200.engine import Engine
+    e = Engine()
+    e._on(0)            # as init(0) leaves it, where there is a device
+    return e
+
+
+def test_binding_refuses_a_workspace_elsewhere(eng, eng_on_0):  # noqa: F811
+    import torch
+    host = torch.zeros(1 << 25, dtype=torch.uint8)
+    for e, ws in ((eng, host), (eng_on_0, host), (eng_on_0, OtherGpusTensor(host))):
+        with pytest.raises(ValueError, match="engine's device"):
+            e._workspace(ws)
+    assert eng._workspace(None) is None and eng._workspace(4096) == 4096
+
+
+def test_binding_refuses_another_gpus_tensors(eng_on_0):
+    import torch
+    z = lambda *s, dtype=torch.float32: OtherGpusTensor(torch.zeros(*s, dtype=dtype))  # noqa: E731
+    lens, k = z(2, dtype=torch.int32), z(4, 32, 16)
+    with pytest.raises(ValueError, match="engine's device is wanted, got cuda:1"):
+        eng_on_0.kv_cache_attend_tree(k, k, z(8, 3, 16), z(8, 3, 16), lens, 1.0)
+    with pytest.raises(ValueError, match="engine's device"):
+        eng_on_0.qkv_norm_rope(z(6, 128), z(8, 3, 16), z(4, 3, 16), z(4, 3, 16), 2)
+    with pytest.raises(ValueError, match="engine's device"):
+        eng_on_0.kv_cache_compact(k, k, z(2, 5, dtype=torch.int32), lens, lens)
