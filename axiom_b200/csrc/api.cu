@@ -1430,17 +1430,22 @@ int attn_workspace(const char *what, void *&ws)
     }
     if (!cur().attn_ws) {
         cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(cur().stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone)
+        if (cudaStreamIsCapturing(cur().stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) {
+            cudaGetLastError();
             return fail(AXB_ERR_ALLOC, "%s: the first call that needs the engine's workspace may not be captured", what);
+        }
+        // it becomes the engine's only once its counters are zero for every stream; a failure (another stream's capture forbids
+        // these calls) leaves nothing behind, the runtime's last error included, which the next launch would be taken to task for
         const size_t bytes = attn_workspace_bytes();
-        cudaError_t e = cudaMalloc(&cur().attn_ws, bytes);
+        void *made = nullptr;
+        cudaError_t e = cudaMalloc(&made, bytes);
+        if (e == cudaSuccess && (e = cudaMemset(made, 0, kAttnCounters)) == cudaSuccess) e = cudaDeviceSynchronize();
         if (e != cudaSuccess) {
-            cur().attn_ws = nullptr;
+            if (made) cudaFree(made);
+            cudaGetLastError();
             return fail(AXB_ERR_ALLOC, "%s: workspace of %zu bytes: %s", what, bytes, cudaGetErrorString(e));
         }
-        // before any call on any stream: the counters start at zero
-        if ((e = cudaMemset(cur().attn_ws, 0, kAttnCounters)) == cudaSuccess) e = cudaDeviceSynchronize();
-        if (e != cudaSuccess) return cuda_fail(what, e);
+        cur().attn_ws = made;
     }
     ws = cur().attn_ws;
     return AXB_OK;

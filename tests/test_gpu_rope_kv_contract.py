@@ -2,10 +2,15 @@
 workspaces, accuracy where a lost tile or term would show.
 
 Tolerances are bounds, stated beside their use (u = 2^-24, half a step of fp32)."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
 import rope_kv_ref as ref
+from conftest import ROOT
 from test_gpu_rope_kv import U, gen, ints, randn
 
 pytestmark = pytest.mark.gpu
@@ -60,3 +65,48 @@ def test_binding_refuses_a_host_workspace(engine):
         with pytest.raises(ValueError, match="engine's device"):
             engine.kv_cache_attend_tree(z(2, 8, 16), z(2, 8, 16), z(2, 3, 16), z(2, 3, 16), ints([2]), 1.0, workspace=w)
     assert engine.launch_count() == before
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+from axiom_b200.engine import Engine, EngineError
+from test_gpu_rope_kv import attend_case, check_attend, run_attend
+eng = Engine(0)
+s = attend_case((3, 1, 8, 2, 128, [63, 64, 700], False, None), 7)
+torch.cuda.synchronize()
+side, refused = torch.cuda.Stream(), 0
+for mode in ("relaxed", "global"):
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.stream(side):
+            graph.capture_begin(capture_error_mode=mode)
+            try:
+                if {own}:
+                    eng.set_stream(side.cuda_stream)
+                eng.kv_cache_attend_tree(s["K"], s["V"], s["Q"], s["out"], s["lens"], s["scale"])
+            except EngineError as e:
+                refused += 1
+                assert "workspace" in str(e), e
+            finally:
+                eng.set_stream(0)
+                graph.capture_end()
+    except (RuntimeError, torch.AcceleratorError):
+        pass                      # a capture that the refused call spoilt
+    del graph
+assert refused == 2, refused
+check_attend(s, run_attend(eng, s))
+check_attend(s, run_attend(eng, s))
+assert eng.device_error() == 0
+print("served")
+"""
+
+
+@pytest.mark.parametrize("own", [False, True], ids=["another-stream", "the-engines-stream"])
+def test_a_first_call_under_a_capture_leaves_no_workspace_behind(own):
+    """The engine's workspace cannot be made while a stream is captured: the call is refused, and the next one, outside, makes it
+    with its counters at zero and is served."""
+    code = FIRST_CALL.format(root=ROOT, tests=os.path.join(ROOT, "tests"), own=own)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "served" in r.stdout, r.stdout + r.stderr
