@@ -25,6 +25,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <initializer_list>
+
 using namespace axb;
 
 namespace {
@@ -1407,10 +1409,23 @@ inline void wrote_operands()
     cur().chain_hi = reinterpret_cast<const char *>(UINTPTR_MAX);
 }
 
-inline bool overlaps(const void *p, int64_t n, const void *q, int64_t m)   // n, m floats
+struct Span {
+    const void *p;
+    int64_t n;   // 4-byte elements
+};
+
+inline bool overlap(const Span &x, const Span &y)
 {
-    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
-    return p && q && a < b + (size_t)m * sizeof(float) && b < a + (size_t)n * sizeof(float);
+    const uintptr_t a = (uintptr_t)x.p, b = (uintptr_t)y.p;
+    return a && b && a < b + (size_t)y.n * 4 && b < a + (size_t)x.n * 4;
+}
+
+inline bool overlap(std::initializer_list<Span> outs, std::initializer_list<Span> ins)
+{
+    for (const Span &o : outs)
+        for (const Span &i : ins)
+            if (overlap(o, i)) return true;
+    return false;
 }
 
 static_assert(sizeof(int) * 256 <= kAttnCounters && sizeof(KvTreeShared) * 256 <= KT_SHARED_BYTES, "per SM: a counter, a shared item");
@@ -1522,9 +1537,10 @@ extern "C" int axb_qkv_norm_rope(const float *qkv, const float *bqkv, const floa
     if (B == 0 || S == 0) return ensure_ready();   // nothing to read or write: the pointers may be NULL
     if (!qkv || !Qh || !Kh || !Vh) return fail(AXB_ERR_NULL_ARG, "qkv_norm_rope: NULL");
     const int64_t nq = B * S * H * dk, nk = B * S * Hkv * dk, n = nq + 2 * nk;
-    if (overlaps(qkv, n, Qh, nq) || overlaps(qkv, n, Kh, nk) || overlaps(qkv, n, Vh, nk))
-        return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope: an output overlaps qkv");
-    if (overlaps(Qh, nq, Kh, nk) || overlaps(Qh, nq, Vh, nk) || overlaps(Kh, nk, Vh, nk))
+    if (overlap({ { Qh, nq }, { Kh, nk }, { Vh, nk } },
+                { { qkv, n }, { bqkv, (H + 2 * Hkv) * dk }, { gq, dk }, { gk, dk }, { freq, rot }, { pos, B * S } }))
+        return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope: an output overlaps an input");
+    if (overlap({ { Qh, nq } }, { { Kh, nk }, { Vh, nk } }) || overlap({ Kh, nk }, { Vh, nk }))
         return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope: two outputs overlap");
     if ((st = ensure_ready())) return st;
     OnDevice on;
@@ -1547,9 +1563,10 @@ extern "C" int axb_qkv_norm_rope_bwd(const float *qkv, const float *bqkv, const 
     if (B == 0 || S == 0) return ensure_ready();
     if (!dQh || !dKh || !dVh || !dqkv || ((gq || gk) && !qkv)) return fail(AXB_ERR_NULL_ARG, "qkv_norm_rope_bwd: NULL");
     const int64_t nq = B * S * H * dk, nk = B * S * Hkv * dk, n = nq + 2 * nk;
-    if (overlaps(dqkv, n, dQh, nq) || overlaps(dqkv, n, dKh, nk) || overlaps(dqkv, n, dVh, nk) || ((gq || gk) && overlaps(dqkv, n, qkv, n)))
+    if (overlap({ { dqkv, n } }, { { dQh, nq }, { dKh, nk }, { dVh, nk }, { gq || gk ? qkv : nullptr, n }, { bqkv, (H + 2 * Hkv) * dk }, { gq, dk },
+                                   { gk, dk }, { freq, rot }, { pos, B * S } }))
         return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope_bwd: dqkv overlaps an input");
-    if (overlaps(dqkv, n, dgq, dk) || overlaps(dqkv, n, dgk, dk) || (dgq != dgk && overlaps(dgq, dk, dgk, dk)))
+    if (overlap({ { dqkv, n } }, { { dgq, dk }, { dgk, dk } }) || (dgq != dgk && overlap({ dgq, dk }, { dgk, dk })))
         return fail(AXB_ERR_INVALID_SHAPE, "qkv_norm_rope_bwd: two outputs overlap");
     if ((st = ensure_ready())) return st;
     OnDevice on;
@@ -1578,9 +1595,10 @@ extern "C" int axb_kv_cache_extend(const float *qkv, const float *bqkv, const fl
     if (B == 0 || T == 0) return ensure_ready();
     if (!qkv || !lens || !Qh || !K_cache || !V_cache) return fail(AXB_ERR_NULL_ARG, "kv_cache_extend: NULL");
     const int64_t nq = B * T * H * dk, n = nq + 2 * B * T * Hkv * dk, nc = B * Hkv * max_seq * dk;
-    if (overlaps(qkv, n, Qh, nq) || overlaps(qkv, n, K_cache, nc) || overlaps(qkv, n, V_cache, nc))
-        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_extend: an output overlaps qkv");
-    if (overlaps(Qh, nq, K_cache, nc) || overlaps(Qh, nq, V_cache, nc) || overlaps(K_cache, nc, V_cache, nc))
+    if (overlap({ { Qh, nq }, { K_cache, nc }, { V_cache, nc } }, { { qkv, n }, { bqkv, (H + 2 * Hkv) * dk }, { gq, dk }, { gk, dk }, { freq, rot },
+                                                                    { pos, B * T }, { lens, B }, { n_new, B } }))
+        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_extend: an output overlaps an input");
+    if (overlap({ { Qh, nq } }, { { K_cache, nc }, { V_cache, nc } }) || overlap({ K_cache, nc }, { V_cache, nc }))
         return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_extend: two outputs overlap");
     if ((st = ensure_ready())) return st;
     OnDevice on;
@@ -1609,8 +1627,8 @@ extern "C" int axb_kv_cache_attend_tree(const float *K_cache, const float *V_cac
     if (!isfinite(scale)) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: scale %g", (double)scale);
     if (B == 0 || T == 0) return ensure_ready();
     if (!K_cache || !V_cache || !Q || !lens || !out) return fail(AXB_ERR_NULL_ARG, "kv_cache_attend_tree: NULL");
-    const int64_t nq = B * H * T * dk, nc = B * Hkv * max_seq * dk;
-    if (overlaps(out, nq, Q, nq) || overlaps(out, nq, K_cache, nc) || overlaps(out, nq, V_cache, nc))
+    const int64_t nq = B * H * T * dk, nc = B * Hkv * max_seq * dk, words = (T + 63) / 64;
+    if (overlap({ { out, nq } }, { { Q, nq }, { K_cache, nc }, { V_cache, nc }, { mask, 2 * (mask_per_seq ? B : 1) * T * words }, { lens, B }, { n_new, B } }))
         return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: out overlaps an input");
     int st = ensure_ready();
     if (st) return st;
@@ -1621,7 +1639,7 @@ extern "C" int axb_kv_cache_attend_tree(const float *K_cache, const float *V_cac
     a.counters = (int *)workspace;
     a.shared = reinterpret_cast<KvTreeShared *>((char *)workspace + kAttnCounters);
     a.slots = reinterpret_cast<float *>((char *)workspace + kAttnCounters + KT_SHARED_BYTES);
-    a.words = (int)((T + 63) / 64);
+    a.words = (int)words;
     a.mask_stride = mask_per_seq ? T * a.words : 0;
     a.max_seq = max_seq; a.err = cur().err_word; a.c_log2 = scale * 1.4426950408889634f;
     a.B = (int)B; a.H = (int)H; a.Hkv = (int)Hkv; a.T = (int)T; a.dk = (int)dk;
@@ -1644,10 +1662,11 @@ extern "C" int axb_kv_cache_compact(float *K_cache, float *V_cache, const int32_
         return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_compact: dimension too large");
     if (B == 0) return ensure_ready();
     if (!K_cache || !V_cache || (!keep && T > 0) || !n_keep || !lens) return fail(AXB_ERR_NULL_ARG, "kv_cache_compact: NULL");
-    if (lens_out == lens || overlaps(lens_out, B, lens, B) || overlaps(lens_out, B, n_keep, B) || overlaps(lens_out, B, keep, B * T))
-        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_compact: lens_out overlaps an input");
     const int64_t nc = B * Hkv * max_seq * dk;
-    if (overlaps(K_cache, nc, V_cache, nc)) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_compact: the caches overlap");
+    if (overlap({ { lens_out, B }, { K_cache, nc }, { V_cache, nc } }, { { lens, B }, { n_keep, B }, { keep, B * T } }))
+        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_compact: lens_out or a cache overlaps an input");
+    if (overlap({ { K_cache, nc } }, { { V_cache, nc }, { lens_out, B } }) || overlap({ V_cache, nc }, { lens_out, B }))
+        return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_compact: the caches overlap, or lens_out lies in one");
     int st = ensure_ready();
     if (st) return st;
     OnDevice on;

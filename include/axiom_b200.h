@@ -456,7 +456,7 @@ AXB_API int axb_rope_frequencies(int64_t rot, double base, int scaling, double f
      rotation of the first rot elements by p * freq[i], the results times amplitude   (rot == 0: none, freq may be NULL)
    p = pos[b*S + s] (int32), or s when pos is NULL.  freq: [rot/2] doubles on the device.  H is a multiple of Hkv; rot is
    even and at most dk; dk <= 256.  The outputs may overlap
-   neither qkv nor one another. */
+   neither an input nor one another, here and in the calls below. */
 AXB_API int axb_qkv_norm_rope(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
                               const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos, int64_t B,
                               int64_t S, int64_t H, int64_t Hkv, int64_t dk, float *Qh, float *Kh, float *Vh);
@@ -464,7 +464,7 @@ AXB_API int axb_qkv_norm_rope(const float *qkv, const float *bqkv, const float *
    dgq [dk], dgk [dk] += ... (each may be NULL; both may be the same buffer, of one weight for queries and keys, which then
    receives both sums; they may overlap neither otherwise nor dqkv).  qkv, bqkv, gq, gk and the rest are those of the forward call; qkv may be
    NULL when neither gq nor gk is given.  The gradient of bqkv is the column sums of dqkv (axb_gemm with a row of ones).
-   dqkv may not overlap an input.  workspace: see axb_attention_workspace_bytes; needed only when dgq or dgk is wanted.
+   dqkv may not overlap an input (qkv counts as one where it is read).  workspace: see axb_attention_workspace_bytes; needed only when dgq or dgk is wanted.
    Bitwise repeatable. */
 AXB_API int axb_qkv_norm_rope_bwd(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
                                   const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos,

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 from conftest import ROOT
-from test_rope_kv_host import INVALID_SHAPE, P, bwd_call, eng  # noqa: F401
+from test_rope_kv_host import INVALID_SHAPE, P, attend_call, bwd_call, compact_call, eng, extend_call, rope_call  # noqa: F401
 
 
 @pytest.mark.parametrize("override", [dict(dgk=P[9] + 64), dict(dgq=P[10] + 252), dict(dgq=P[8] + 128), dict(dgk=P[8]), dict(dgk=P[8] + 4 * (2 * 8 * 64 - 1))])
@@ -96,3 +96,35 @@ def test_binding_refuses_another_gpus_tensors(eng_on_0):
         eng_on_0.qkv_norm_rope(z(6, 128), z(8, 3, 16), z(4, 3, 16), z(4, 3, 16), 2)
     with pytest.raises(ValueError, match="engine's device"):
         eng_on_0.kv_cache_compact(k, k, z(2, 5, dtype=torch.int32), lens, lens)
+
+
+# every input that a call reads while it writes, met by an output at its first or last bytes
+MEETS = (
+    [("axb_qkv_norm_rope", rope_call, dict(bqkv=P[5], gq=P[6], gk=P[7], pos=P[8]), o) for o in [
+        dict(Q=P[5] + 4 * 511), dict(K=P[6] + 252), dict(V=P[7] - 4 * (2 * 2 * 64 - 1)), dict(Q=P[1] + 252), dict(K=P[8] + 4), dict(V=P[8] - 4)]] +
+    [("axb_qkv_norm_rope_bwd", bwd_call, dict(bqkv=P[5], pos=P[11]), o) for o in [
+        dict(dqkv=P[5] + 4 * 511), dict(dqkv=P[6] + 252), dict(dqkv=P[7]), dict(dqkv=P[1] + 252), dict(dqkv=P[11] + 4)]] +
+    [("axb_kv_cache_extend", extend_call, dict(bqkv=P[6], gq=P[7], gk=P[8], pos=P[9], n_new=P[10]), o) for o in [
+        dict(Q=P[6]), dict(K=P[7] + 252), dict(V=P[8]), dict(Q=P[1]), dict(K=P[9] + 4), dict(V=P[5]), dict(Q=P[10])]] +
+    [("axb_kv_cache_attend_tree", attend_call, dict(mask=P[5], n_new=P[6]), o) for o in [
+        dict(out=P[5] + 8), dict(out=P[3]), dict(out=P[6]), dict(out=P[5] + 24, per_seq=1, B=2)]] +
+    [("axb_kv_cache_compact", compact_call, dict(), o) for o in [
+        dict(K=P[2] + 28), dict(V=P[3] + 4), dict(K=P[4]), dict(lens_out=P[0] + 64), dict(lens_out=P[1] + 4 * (2 * 2 * 128 * 64 - 1))]])
+
+
+@pytest.mark.parametrize("name,call,base,override", MEETS, ids=lambda v: v if isinstance(v, str) else None)
+def test_outputs_that_meet_any_input_are_refused(eng, name, call, base, override):  # noqa: F811
+    assert getattr(eng.lib, name)(*call(**{**base, **override})) == INVALID_SHAPE
+    assert "overlap" in eng.last_error() or "lies in" in eng.last_error()
+
+
+@pytest.mark.parametrize("name,call,base", sorted({(n, c, tuple(sorted(b.items()))) for n, c, b, _ in MEETS}, key=lambda v: v[0]), ids=lambda v: v if isinstance(v, str) else None)
+def test_outputs_beside_their_inputs_are_not(eng, name, call, base):  # noqa: F811
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("needs a machine without a GPU")
+    beside = {"axb_qkv_norm_rope": dict(Q=P[5] + 4 * 512, V=P[8] + 8), "axb_qkv_norm_rope_bwd": dict(dqkv=P[6] + 256),
+              "axb_kv_cache_extend": dict(Q=P[7] + 256, K=P[9] + 8), "axb_kv_cache_attend_tree": dict(out=P[5] + 16),
+              "axb_kv_cache_compact": dict(K=P[2] + 32, lens_out=P[1] + 4 * 2 * 2 * 128 * 64)}[name]
+    assert getattr(eng.lib, name)(*call(**{**dict(base), **beside})) != INVALID_SHAPE
+    assert "no CUDA device" in eng.last_error()
