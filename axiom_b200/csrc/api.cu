@@ -1624,7 +1624,8 @@ extern "C" int axb_kv_cache_attend_tree(const float *K_cache, const float *V_cac
     // the work line counts tiles of at least 32 keys and 8 query rows, and up to 8 more an item, in 31 bits
     if (B && (max_seq / 32 + 9) > (1 << 30) / (B * Hkv) / ((H / Hkv * T + 7) / 8 > 0 ? (H / Hkv * T + 7) / 8 : 1))
         return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: more than 2^30 tiles");
-    if (!isfinite(scale)) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: scale %g", (double)scale);
+    const float c_log2 = scale * 1.4426950408889634f;   // (infinite from 2.36e38 on: it would make NaN of a score of 0)
+    if (!isfinite(c_log2)) return fail(AXB_ERR_INVALID_SHAPE, "kv_cache_attend_tree: scale %g", (double)scale);
     if (B == 0 || T == 0) return ensure_ready();
     if (!K_cache || !V_cache || !Q || !lens || !out) return fail(AXB_ERR_NULL_ARG, "kv_cache_attend_tree: NULL");
     const int64_t nq = B * H * T * dk, nc = B * Hkv * max_seq * dk, words = (T + 63) / 64;
@@ -1641,7 +1642,7 @@ extern "C" int axb_kv_cache_attend_tree(const float *K_cache, const float *V_cac
     a.slots = reinterpret_cast<float *>((char *)workspace + kAttnCounters + KT_SHARED_BYTES);
     a.words = (int)words;
     a.mask_stride = mask_per_seq ? T * a.words : 0;
-    a.max_seq = max_seq; a.err = cur().err_word; a.c_log2 = scale * 1.4426950408889634f;
+    a.max_seq = max_seq; a.err = cur().err_word; a.c_log2 = c_log2;
     a.B = (int)B; a.H = (int)H; a.Hkv = (int)Hkv; a.T = (int)T; a.dk = (int)dk;
     mark(0);
     mark(1);

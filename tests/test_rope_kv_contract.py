@@ -128,3 +128,13 @@ def test_outputs_beside_their_inputs_are_not(eng, name, call, base):  # noqa: F8
               "axb_kv_cache_compact": dict(K=P[2] + 32, lens_out=P[1] + 4 * 2 * 2 * 128 * 64)}[name]
     assert getattr(eng.lib, name)(*call(**{**dict(base), **beside})) != INVALID_SHAPE
     assert "no CUDA device" in eng.last_error()
+
+
+def test_a_scale_that_is_infinite_in_the_kernels_domain_is_refused(eng):  # noqa: F811
+    """Scores are taken to base 2: scale / ln 2 has to be finite as well."""
+    import torch
+    for scale in (2.4e38, -3e38, float("inf"), float("nan")):
+        assert eng.lib.axb_kv_cache_attend_tree(*attend_call(scale=scale)) == INVALID_SHAPE and "scale" in eng.last_error()
+    if not torch.cuda.is_available():
+        for scale in (2.3e38, -2.3e38, 1e-45, 0.0):
+            assert eng.lib.axb_kv_cache_attend_tree(*attend_call(scale=scale)) != INVALID_SHAPE
