@@ -55,6 +55,7 @@ struct Engine {
     // output range of the last skinny kernel, which lets the next one start under it: a skinny call whose WEIGHTS lie
     // in that range must not prefetch them early
     const char *chain_lo = nullptr, *chain_hi = nullptr;
+    bool chain_any = false;   // the last call wrote more than one range: the next one prefetches nothing early
     int64_t launches = 0;
     // grow-only buffer for intermediate results a fused route cannot avoid (the unfused qkv projection)
     void *aux = nullptr;
@@ -117,6 +118,19 @@ inline void mark(int i)
     if (!slot[i]) cudaEventCreate(&slot[i]);
     cudaEventRecord(slot[i], cur().stream);
     if (i == 2) cur().ev_count++;
+}
+
+// whether a skinny call may request the weights in [lo, hi) before the call before it has finished; afterwards, what it writes itself
+inline bool may_prefetch(const char *lo, const char *hi)
+{
+    return !cur().chain_any && !(cur().chain_lo && lo < cur().chain_hi && cur().chain_lo < hi);
+}
+
+inline void wrote(const float *out, int64_t M, int64_t N)
+{
+    cur().chain_any = false;
+    cur().chain_lo = reinterpret_cast<const char *>(out);
+    cur().chain_hi = cur().chain_lo + (size_t)M * N * sizeof(float);
 }
 
 int ensure_ready()
@@ -285,9 +299,8 @@ int gemm_skinny(const float *X, const float *W, const float *bias, float *Y, int
     // back-to-back skinny calls (a decode step walks a chain of them) overlap: this call may request its first weight
     // tiles while the previous one drains, unless those weights are what the previous call wrote
     const char *w_lo = reinterpret_cast<const char *>(W), *w_hi = w_lo + (size_t)K * N * sizeof(float);
-    const int pdl = !(cur().chain_lo && w_lo < cur().chain_hi && cur().chain_lo < w_hi);
-    cur().chain_lo = reinterpret_cast<const char *>(Y);
-    cur().chain_hi = cur().chain_lo + (size_t)M * N * sizeof(float);
+    const int pdl = may_prefetch(w_lo, w_hi);
+    wrote(Y, M, N);
     // above 8 rows the fp32 pipe, not memory, paces the FMA kernels: the tensor-core variant takes over
     if (M >= 9 && skinny_tc_applicable(M, N, K, X, W)) {
         SkinnyArgs a;
@@ -485,6 +498,7 @@ extern "C" void axb_set_stream(void *cuda_stream)
 {
     cur().stream = (cudaStream_t)cuda_stream;
     cur().chain_lo = cur().chain_hi = nullptr;
+    cur().chain_any = false;
 }
 
 extern "C" int axb_set_fp32_mode(int mode)
@@ -1019,9 +1033,8 @@ extern "C" int axb_qdense_w8a32(const float *a, const int8_t *q, const float *sc
         // (a call of up to 4 rows is one kernel that lets its successor start early: as on the fp32 skinny route, the
         // successor may only do so when this call's output is not what it streams as weights)
         const char *w_lo = reinterpret_cast<const char *>(q), *w_hi = w_lo + (size_t)N * K;
-        const int pdl = !(cur().chain_lo && w_lo < cur().chain_hi && cur().chain_lo < w_hi);
-        cur().chain_lo = reinterpret_cast<const char *>(out);
-        cur().chain_hi = cur().chain_lo + (size_t)M * N * sizeof(float);
+        const int pdl = may_prefetch(w_lo, w_hi);
+        wrote(out, M, N);
         int e = launch_qskinny_tc(a, q, scales, bias, act, out, M, N, K, cur().ws, cur().err_word, cur().sm_count, cur().stream, pdl);
         mark(2);
         cur().launches += M <= 4 ? 1 : 2;
@@ -1402,12 +1415,7 @@ struct OnDevice {
 
 // a skinny GEMM after this call must not request its weights before the call has finished: it may be multiplying by the
 // cache or the queries written here
-inline void wrote_operands()
-{
-    cur().chain_lo = nullptr;
-    cur().chain_lo += 1;
-    cur().chain_hi = reinterpret_cast<const char *>(UINTPTR_MAX);
-}
+inline void wrote_operands() { cur().chain_any = true; }
 
 struct Span {
     const void *p;

@@ -88,13 +88,6 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The lo part of x: what the tensor core, which reads the upper 19 bits of an operand, leaves of x as a hi operand; rounded
-// to the bits it will read (cut, it would keep the sign of x — a bias that the sums over columns and keys add up).
-__device__ __forceinline__ uint32_t tf32_lo(float x)
-{
-    return __float_as_uint(x - __uint_as_float(__float_as_uint(x) & 0xffffe000u)) + 0x1000u;
-}
-
 __device__ __forceinline__ float4 lds128(const uint8_t *p) { return *reinterpret_cast<const float4 *>(p); }
 
 // byte offset of 16-byte chunk `chunk` (0..7) of 32-column slab `slab` of row `row` of a tile

@@ -1,6 +1,6 @@
 // kv_tree_line.cuh — how the kernels of kv_cache_attend_tree divide a ragged batch between their CTAs, on the device.
 // The key tiles of all (sequence, key head, row block) items form one line, cut into equal stretches, one a CTA; the
-// CTAs that share an item are consecutive and each holds a tile of it.
+// CTAs that share an item are consecutive and each holds a tile of it.  And the few device functions that they share.
 #pragma once
 #include "../../include/axiom_b200.h"
 #include "device_error.cuh"
@@ -169,6 +169,13 @@ __device__ __forceinline__ bool tree_sees(const KvTreeArgs &a, int b, int t, int
 {
     if (!a.mask) return j <= t;
     return (__ldg(a.mask + b * a.mask_stride + (int64_t)t * a.words + (j >> 6)) >> (j & 63)) & 1;
+}
+
+// The lo part of x: what the tensor core, which reads the upper 19 bits of an operand, leaves of x as a hi operand; rounded
+// to the bits it will read (cut, it would keep the sign of x — a bias that the sums over columns and keys add up).
+__device__ __forceinline__ uint32_t tf32_lo(float x)
+{
+    return __float_as_uint(x - __uint_as_float(__float_as_uint(x) & 0xffffe000u)) + 0x1000u;
 }
 
 __device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }

@@ -69,10 +69,7 @@ struct TreeTcMaps {
     CUtensorMap k, v;   // [B*Hkv][max_seq][dk], boxes of 32 columns x KB rows (v: 32-byte swizzle atoms)
 };
 
-__device__ __forceinline__ uint32_t lo_bits(uint32_t x)
-{
-    return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u)) + 0x1000u;
-}
+__device__ __forceinline__ uint32_t lo_bits(uint32_t x) { return tf32_lo(__uint_as_float(x)); }
 
 // The three products of a block's scores / outputs, issued by one thread: four steps of eight at a time, in loops.  Unrolled whole
 // the thread takes 55 cycles a product instead of 70 to 100, but the kernel's roles share the SM's instruction cache, and the call
@@ -597,7 +594,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) kv_tree_tc_kernel(const __grid_
 // The shared items' pieces added up, in line order within each of a unit's groups of threads and then over the groups.  A unit is
 // a few rows of an item: fewer where more pieces want more groups.  (The CTA that arrived last used to do it, one piece after the
 // other on one SM and with a counter's round trip for every piece: 30 us for 148 pieces of 128 rows.)
-template <int DKP, int ROWS>
+template <int DKP>
 struct TreeJoin {
     static constexpr int COLS = DKP / 4, RG = COLS > 16 ? 16 : COLS > 8 ? 32 : 64, THREADS = RG * COLS;   // rows x groups of a unit
     // as many groups as leave each four pieces, and two rows to a unit (the rows of a 16-byte column then fill a 32-byte sector)
@@ -610,9 +607,9 @@ struct TreeJoin {
 };
 
 template <int DKP, int ROWS>
-__global__ void __launch_bounds__(TreeJoin<DKP, ROWS>::THREADS, 2) kv_tree_join_kernel(const KvTreeArgs a, int ctas)
+__global__ void __launch_bounds__(TreeJoin<DKP>::THREADS, 2) kv_tree_join_kernel(const KvTreeArgs a, int ctas)
 {
-    using J = TreeJoin<DKP, ROWS>;
+    using J = TreeJoin<DKP>;
     __shared__ float4 s_o[J::THREADS];
     __shared__ float2 s_ml[J::RG];
     __shared__ int s_upto[256], s_warp[8], s_unit[2];
@@ -710,7 +707,7 @@ static int launch_tc(const KvTreeArgs &a, int sm_count, cudaStream_t st)
     if (e) return e;
     kv_tree_tc_kernel<NSLAB, FEW><<<sm_count, TT_THREADS, C::SMEM, st>>>(a, tm);
     if ((e = (int)cudaGetLastError()) != 0) return e;
-    using J = TreeJoin<C::DKP, C::ROWS>;
+    using J = TreeJoin<C::DKP>;
     kv_tree_join_kernel<C::DKP, C::ROWS><<<2 * sm_count, J::THREADS, 0, st>>>(a, sm_count);
     return (int)cudaGetLastError();
 }

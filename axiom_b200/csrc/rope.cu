@@ -532,11 +532,11 @@ __global__ void __launch_bounds__(512) rope_dgamma_kernel(const float *partial, 
 
 // ---------------------------------------------------------------------- host
 
-static bool rope_vec(const RopeArgs &a, const float *dgq, const float *dgk)
+static bool rope_vec(const RopeArgs &a)
 {
     uintptr_t m = 0;
     for (const void *p : { (const void *)a.qkv, (const void *)a.bias, (const void *)a.gq, (const void *)a.gk, (const void *)a.q,
-                           (const void *)a.k, (const void *)a.v, (const void *)a.dqkv, (const void *)dgq, (const void *)dgk })
+                           (const void *)a.k, (const void *)a.v, (const void *)a.dqkv })
         m |= reinterpret_cast<uintptr_t>(p);
     // whole 16-byte pieces on either side of every pair: half split 2*pairs floats cut in two, interleaved two pairs a piece
     return (m & 15) == 0 && a.dk % 4 == 0 && a.pairs % (a.interleaved ? 2 : 4) == 0;
@@ -573,7 +573,7 @@ static size_t rope_smem(const RopeArgs &a, const RopePlan &p, bool backward)
 
 int launch_qkv_norm_rope(const RopeArgs &a, int sm_count, cudaStream_t st)
 {
-    const bool vec = rope_vec(a, nullptr, nullptr);
+    const bool vec = rope_vec(a);
     const RopePlan p = rope_plan(a, vec, sm_count, false);
     const int grid = p.blocks;
     const size_t smem = rope_smem(a, p, false);
@@ -591,7 +591,7 @@ size_t qkv_norm_rope_bwd_bytes(int sm_count)
 
 int launch_qkv_norm_rope_bwd(const RopeArgs &a, float *dgq, float *dgk, int sm_count, cudaStream_t st, int *launches)
 {
-    const bool vec = rope_vec(a, nullptr, nullptr);
+    const bool vec = rope_vec(a);
     const RopePlan p = rope_plan(a, vec, sm_count, true);
     const int grid = p.blocks;
     const size_t smem = rope_smem(a, p, true);

@@ -20,6 +20,7 @@ template <typename T>
 static T __ldg(const T *p) { return *p; }
 static int atomicAdd(int *p, int v) { const int old = *p; *p += v; return old; }
 static int atomicCAS(int *p, int cmp, int v) { const int old = *p; if (old == cmp) *p = v; return old; }
+static float __uint_as_float(unsigned u) { float x; std::memcpy(&x, &u, 4); return x; }
 static unsigned __float_as_uint(float x) { unsigned u; std::memcpy(&u, &x, 4); return u; }
 // the search of tree_start, a whole warp's work: never called here
 template <typename T>
