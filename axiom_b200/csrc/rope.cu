@@ -32,7 +32,7 @@
 
 namespace axb {
 
-static constexpr int RP_THREADS = 128, RP_WARPS = RP_THREADS / 32, RP_FWD_CTAS = 8, RP_BWD_CTAS = 5;
+static constexpr int RP_THREADS = 128, RP_WARPS = RP_THREADS / 32, RP_FWD_CTAS = 8, RP_BWD_CTAS = 5, RP_BWD_SETS = 8;
 static constexpr double RP_INV_2PI = 0.15915494309189533577;
 
 // which pieces (VEC floats each) of a head row unit u of a lane covers, and whether they form rotated pairs
@@ -554,12 +554,13 @@ static RopePlan rope_plan(const RopeArgs &a, bool vec, int sm_count, bool backwa
     const int64_t steps = (int64_t)a.B * a.T * p.steps, need = (steps + RP_WARPS - 1) / RP_WARPS;
     // One set of resident CTAs; where that leaves a warp more than 16 steps, up to four sets, so that an SM that is done early
     // takes more (the forward of 16384 tokens above: one set 148 us, two 136, four 134; 768 tokens: 7.8, 8.6 and 11.1).  The
-    // backward keeps to one, every CTA of it being a term of the norm weights' sums.
+    // backward, every CTA of it being a term of the norm weights' sums, keeps to one up to 256 steps a warp and to stretches of no
+    // more than some 256 from there, up to eight sets: a lane adds in 32 bits, and the error of its sum grows with the root of its
+    // terms (262,144 tokens of 16 + 2*8 heads of 128: 4.6e-7 of the gradient's norm with one set, 2100 us; 64 steps 1.7e-7, but 1 to
+    // 2 per cent slower from 32,768 tokens on).
     int64_t most = (int64_t)sm_count * (backward ? RP_BWD_CTAS : RP_FWD_CTAS);
-    if (!backward) {
-        const int64_t sets = need / (16 * most);
-        most *= sets < 1 ? 1 : sets > 4 ? 4 : sets;
-    }
+    const int64_t sets = need / ((backward ? 256 : 16) * most), limit = backward ? RP_BWD_SETS : 4;
+    most *= sets < 1 ? 1 : sets > limit ? limit : sets;
     p.blocks = (int)(need < most ? need : most);
     return p;
 }
@@ -586,7 +587,7 @@ int launch_qkv_norm_rope(const RopeArgs &a, int sm_count, cudaStream_t st)
 
 size_t qkv_norm_rope_bwd_bytes(int sm_count)
 {
-    return (size_t)sm_count * RP_BWD_CTAS * 2 * 256 * sizeof(float);
+    return (size_t)sm_count * RP_BWD_CTAS * RP_BWD_SETS * 2 * 256 * sizeof(float);
 }
 
 int launch_qkv_norm_rope_bwd(const RopeArgs &a, float *dgq, float *dgk, int sm_count, cudaStream_t st, int *launches)

@@ -246,3 +246,22 @@ def test_norm_gradients_in_the_norm(engine, B, S, H, Hkv, dk, rot, pairing):
                 turned = ref.rope_head(d[b * heads + h].double(), None, 0.0, -pos, freq, pairing, 1.25)      # the transposed rotation
                 want += (turned * unit).sum(0)
         assert float((got.double() - want).norm() / want.norm()) <= 4e-6
+
+
+def test_norm_gradients_of_many_tokens_keep_their_accuracy(engine):
+    """A lane's chain of fp32 additions does not grow with the batch: 262,144 tokens of 16 + 2*8 heads of 128 make at most 142 additions
+    of query terms a lane (283 steps, every second one of query heads), u sqrt(142 / 6) = 2.9e-7 of the sum's norm at most, and the
+    terms' own errors add 0.8e-7 in square: 3.0e-7.  (A chain of all 708 that one set of CTAs makes is at 4.6e-7.)"""
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 20 GB")
+    S, H, Hkv, dk = 262144, 16, 8, 128
+    g = gen(181)
+    qkv, w, dg = randn(g, S, (H + 2 * Hkv) * dk), 1 + 0.3 * randn(g, dk), torch.zeros(dk, device="cuda")
+    grads = [randn(g, h, S, dk) for h in (H, Hkv, Hkv)]
+    freq, pos = torch.tensor(ref.frequencies(dk), dtype=torch.float64).cuda(), torch.arange(S, device="cuda")
+    engine.qkv_norm_rope_bwd(*grads, torch.empty_like(qkv), 1, qkv=qkv, gq=w, gk=w, freq=freq, dgq=dg)
+    want = torch.zeros(dk, dtype=torch.float64, device="cuda")
+    for h in range(H):
+        xh = qkv.view(S, -1, dk)[:, h].double()
+        want += (ref.rope_head(grads[0][h].double(), None, 0.0, -pos, freq, "half", 1.0) * xh * torch.rsqrt((xh * xh).mean(-1, keepdim=True) + 1e-6)).sum(0)
+    assert float((dg.double() - want).norm() / want.norm()) <= 3.5e-7
