@@ -489,7 +489,8 @@ AXB_API int axb_kv_cache_extend(const float *qkv, const float *bqkv, const float
    see; query head h uses key head h / (H / Hkv).  mask: bit j % 64 of word j / 64 of mask[b][t][ceil(T/64)] says whether
    token t sees new token j (its ancestors and itself, in a drafted tree; bits from n_new[b] on are ignored); mask_per_seq
    == 0: one [T][ceil(T/64)] mask for all sequences.  mask NULL: token t sees new tokens 0 .. t.  A token that sees
-   nothing gets 0.  Values in rows a token does not see do not reach it, infinities and NaN included.  T = 1 is
+   nothing gets 0.  Values in rows a token does not see do not reach it, infinities and NaN included; an infinity in a key it
+   does see is a score of that infinity or makes the result NaN, one in a value makes that column infinite or NaN.  T = 1 is
    single-token decode at every sequence's own length.  dk <= 128, max_seq <= 2^30, H <= 65535, |scale| < 2.3e38, and
    B * Hkv * ceil(H/Hkv * T / 8) * (max_seq / 32 + 9) <= 2^30.  out may not overlap an input.  workspace: below.
    Bitwise repeatable. */

@@ -265,3 +265,28 @@ def test_norm_gradients_of_many_tokens_keep_their_accuracy(engine):
         xh = qkv.view(S, -1, dk)[:, h].double()
         want += (ref.rope_head(grads[0][h].double(), None, 0.0, -pos, freq, "half", 1.0) * xh * torch.rsqrt((xh * xh).mean(-1, keepdim=True) + 1e-6)).sum(0)
     assert float((dg.double() - want).norm() / want.norm()) <= 3.5e-7
+
+
+@pytest.mark.parametrize("T,H,dk", [(1, 2, 64), (5, 4, 50), (16, 8, 128), (40, 8, 64)])
+def test_infinities_that_a_token_sees(engine, T, H, dk):
+    """A cached key with an infinity is, for every row, an infinite score as the formula has it, or NaN (its two parts, as operands of
+    the products, meet zeros); a cached value with one makes its column infinite or NaN; the other key head's and the other
+    sequence's results keep their bits."""
+    s = attend_case((2, T, H, 2, dk, [90, 200], False, None), 191)
+    clean = run_attend(engine, s).view(2, 2, -1, dk)          # [sequence][key head][rows]
+    for x, row in (("K", 33), ("V", 77)):
+        bad = {**s, x: s[x].clone()}
+        bad[x].view(2, 2, -1, dk)[1, 0, row, 5] = float("inf")
+        got = run_attend(engine, bad).view(2, 2, -1, dk)
+        assert torch.equal(got[0], clean[0]) and torch.equal(got[1, 1], clean[1, 1])
+        if x == "K":
+            k, v = (bad[w].view(2, 2, -1, dk)[1, 0, :200 + T].double() for w in "KV")
+            score = s["scale"] * s["Q"].view(2, 2, -1, dk)[1, 0].double() @ k.T
+            token = torch.arange(score.shape[0], device="cuda") % T
+            p = torch.softmax(score.masked_fill(torch.arange(200 + T, device="cuda") > 200 + token[:, None], -torch.inf), -1)
+            want, nan = p @ v, got[1, 0].isnan().all(-1)
+            assert bool((nan | want.isfinite().all(-1)).all())                       # +inf: nothing but NaN
+            assert float((got[1, 0].double() - want)[~nan].norm()) <= 5e-6 * float(want[~nan].norm())
+        else:
+            assert not bool(got[1, 0, :, 5].isfinite().any())
+            assert torch.equal(got[1, 0, :, :5], clean[1, 0, :, :5]) and torch.equal(got[1, 0, :, 6:], clean[1, 0, :, 6:])
