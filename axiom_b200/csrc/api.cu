@@ -94,8 +94,10 @@ inline Engine &cur()
 constexpr size_t kSplitScratch = (size_t)64 << 20;
 constexpr int kSplitCounters = 1024;
 
+// (what failed is reported with this call: the runtime's last error must not be there for the next call's launch to find)
 int fail(int status, const char *fmt, ...)
 {
+    cudaGetLastError();
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(cur().msg, sizeof cur().msg, fmt, ap);
@@ -358,6 +360,7 @@ int axb::engine_device() { return tl_device >= 0 ? tl_device : g_default_device;
 
 int axb::set_error(int status, const char *fmt, ...)
 {
+    cudaGetLastError();
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(cur().msg, sizeof cur().msg, fmt, ap);
@@ -1453,19 +1456,16 @@ int attn_workspace(const char *what, void *&ws)
     }
     if (!cur().attn_ws) {
         cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(cur().stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) {
-            cudaGetLastError();
+        if (cudaStreamIsCapturing(cur().stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone)
             return fail(AXB_ERR_ALLOC, "%s: the first call that needs the engine's workspace may not be captured", what);
-        }
         // it becomes the engine's only once its counters are zero for every stream; a failure (another stream's capture forbids
-        // these calls) leaves nothing behind, the runtime's last error included, which the next launch would be taken to task for
+        // these calls) leaves nothing behind
         const size_t bytes = attn_workspace_bytes();
         void *made = nullptr;
         cudaError_t e = cudaMalloc(&made, bytes);
         if (e == cudaSuccess && (e = cudaMemset(made, 0, kAttnCounters)) == cudaSuccess) e = cudaDeviceSynchronize();
         if (e != cudaSuccess) {
             if (made) cudaFree(made);
-            cudaGetLastError();
             return fail(AXB_ERR_ALLOC, "%s: workspace of %zu bytes: %s", what, bytes, cudaGetErrorString(e));
         }
         cur().attn_ws = made;

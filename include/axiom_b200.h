@@ -462,10 +462,10 @@ AXB_API int axb_qkv_norm_rope(const float *qkv, const float *bqkv, const float *
                               int64_t S, int64_t H, int64_t Hkv, int64_t dk, float *Qh, float *Kh, float *Vh);
 /* Its gradient: dQh, dKh, dVh head-major -> dqkv flat (overwritten), and the norm weights' gradients, ACCUMULATED:
    dgq [dk], dgk [dk] += ... (each may be NULL; both may be the same buffer, of one weight for queries and keys, which then
-   receives both sums; they may overlap neither otherwise nor dqkv).  qkv, bqkv, gq, gk and the rest are those of the forward call; qkv may be
-   NULL when neither gq nor gk is given.  The gradient of bqkv is the column sums of dqkv (axb_gemm with a row of ones).
-   dqkv may not overlap an input (qkv counts as one where it is read).  workspace: see axb_attention_workspace_bytes; needed only when dgq or dgk is wanted.
-   Bitwise repeatable. */
+   receives both sums; they may overlap neither otherwise nor dqkv).  qkv, bqkv, gq, gk and the rest are those of the forward
+   call; qkv may be NULL when neither gq nor gk is given.  The gradient of bqkv is the column sums of dqkv (axb_gemm with a
+   row of ones).  dqkv may not overlap an input (qkv counts as one where it is read).  workspace: see
+   axb_attention_workspace_bytes; needed only when dgq or dgk is wanted.  Bitwise repeatable. */
 AXB_API int axb_qkv_norm_rope_bwd(const float *qkv, const float *bqkv, const float *gq, const float *gk, float eps,
                                   const double *freq, int64_t rot, int pairing, float amplitude, const int32_t *pos,
                                   const float *dQh, const float *dKh, const float *dVh, int64_t B, int64_t S, int64_t H,

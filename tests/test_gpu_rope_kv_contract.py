@@ -290,3 +290,13 @@ def test_infinities_that_a_token_sees(engine, T, H, dk):
         else:
             assert not bool(got[1, 0, :, 5].isfinite().any())
             assert torch.equal(got[1, 0, :, :5], clean[1, 0, :, :5]) and torch.equal(got[1, 0, :, 6:], clean[1, 0, :, 6:])
+
+
+def test_a_failed_allocation_is_not_the_next_calls_error(engine):
+    """The runtime keeps the error of a call that failed; it has been reported, and the launches behind it are not to blame."""
+    H, dk = 2, 32
+    qkv, out = torch.randn(3, 3 * H * dk, device="cuda"), [torch.zeros(H, 3, dk, device="cuda") for _ in range(3)]
+    for _ in range(2):
+        assert engine.lib.axb_storage_alloc(1 << 50) is None and "storage_alloc" in engine.last_error()
+        engine.qkv_norm_rope(qkv, *out, 1)
+    assert torch.equal(out[2], qkv.view(3, 3, H, dk)[:, 2].transpose(0, 1))
